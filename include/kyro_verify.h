@@ -16,6 +16,8 @@
  *   kyro_paged_kv_append     replaces  KVCacheManager::append_kv (src/model/kv_cache.rs:49-75)
  *                                       as called before attention (src/model/llama.rs:80-84),
  *                                       for a block-table cache instead of per-request tensors
+ *   kyro_qkv_append          the same with the head norms and the rotation of RotaryEmbedding
+ *                                       (src/model/layers.rs:21-62) before it, in one launch
  *
  * Everything else here is plumbing a Rust `extern "C"` block (or ctypes, or C++) binds to:
  * a per-device context that owns a HIP stream and a scratch arena, opaque device buffers,
@@ -43,7 +45,7 @@
 extern "C" {
 #endif
 
-#define KYRO_ABI_VERSION 9
+#define KYRO_ABI_VERSION 10
 
 typedef enum kyro_status {
     KYRO_OK = 0,
@@ -366,6 +368,57 @@ int kyro_paged_kv_append(kyro_ctx ctx, const kyro_kv_append_params* params,
                          const void* key, const void* value, const int32_t* q_start_loc,
                          const int64_t* block_table, const int64_t* context_lens,
                          void* key_cache, void* value_cache);
+
+/* ---------------------------------------------------------------- norm, rotation and paged write */
+
+typedef struct kyro_qkv_append_params {
+    int32_t block_size;          /* tokens per KV block */
+    int32_t num_heads;           /* query heads H */
+    int32_t num_kv_heads;        /* Hkv; H % Hkv == 0 */
+    int32_t head_dim;            /* D: a multiple of 8, at most 256 */
+    int32_t batch_size;          /* B */
+    int32_t total_q;             /* rows of query / key / value: B when q_start_loc is NULL */
+    int32_t max_blocks_per_seq;  /* width of block_table */
+    int32_t num_blocks;          /* leading dim of the caches */
+    int32_t src_dtype;           /* kyro_dtype of query, key and value */
+    int32_t cache_dtype;         /* kyro_dtype of the caches and out_query */
+    int32_t rotary_dim;          /* R: elements of a head that turn, the first ones; 0 => no rotation. A
+                                    multiple of 4 in halves, of 2 interleaved */
+    int32_t interleaved;         /* 0: element i turns with i + R/2; 1: 2i with 2i + 1 */
+    int32_t max_position;        /* rows of cos / sin */
+    int32_t norm;                /* 1: root-mean-square norm of each query and key head before the rotation */
+    int32_t weight_dtype;        /* kyro_dtype of q_weight / k_weight */
+    float eps;                   /* added to the mean square */
+    float weight_offset;         /* added to the weights (1 for models that store w - 1) */
+    int64_t query_stride;        /* elements from one row of query to the next (0 => H * D); a */
+    int64_t key_stride;          /* multiple of 8. Slices of one projection's [total_q, (H + 2 Hkv) * D] */
+    int64_t value_stride;        /* output have (H + 2 Hkv) * D (0 => Hkv * D) */
+} kyro_qkv_append_params;
+
+/*
+ * What an attention layer does between its projections and kyro_paged_attention_mq, in one pass over
+ * the new rows. For row j of sequence b (rows as for kyro_paged_kv_append, its slot p = context_lens[b]
+ * - q_len + j):
+ *   queries and keys, each head x: with norm, x <- x * (w + weight_offset) / sqrt(mean(x^2) + eps)
+ *     (w = 1 without weights); then with angle row t = positions[row] (NULL: t = p) of cos and sin,
+ *     (x_i, x_i') <- (x_i cos[t][i] - x_i' sin[t][i], x_i' cos[t][i] + x_i sin[t][i]) for i < R/2;
+ *   out_query [total_q, H, D] gets the queries, the caches' slots the keys and the values.
+ * In 32 bits, rounded once to cache_dtype (to nearest even); values keep their bits where src_dtype
+ * is cache_dtype.
+ *   query [total_q, H, D], key, value [total_q, Hkv, D]   src_dtype, rows at their strides, heads dense
+ *   q_start_loc, block_table, context_lens, caches         as for kyro_paged_kv_append
+ *   positions [total_q] int64 or NULL: needed where a token's position is not its slot, as after
+ *     kyro_kv_evict
+ *   cos, sin [max_position, R/2] f32 (R = 0: NULL); q_weight, k_weight [D] weight_dtype, both or neither
+ *   out_query may be query itself where that is contiguous and of cache_dtype; it overlaps no other input
+ * Pointers are on 16-byte boundaries. Rows of no sequence are left alone. A bad block id, context length,
+ * q_start_loc or position latches KYRO_EINVAL for the next kyro_sync, and such a row is not written.
+ */
+int kyro_qkv_append(kyro_ctx ctx, const kyro_qkv_append_params* params, const void* query, const void* key,
+                    const void* value, const int32_t* q_start_loc, const int64_t* positions,
+                    const int64_t* block_table, const int64_t* context_lens, const float* cos, const float* sin,
+                    const void* q_weight, const void* k_weight, void* key_cache, void* value_cache,
+                    void* out_query);
 
 #ifdef __cplusplus
 }

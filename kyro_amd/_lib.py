@@ -68,6 +68,14 @@ class KvAppendParams(ctypes.Structure):
         "num_blocks", "src_dtype", "cache_dtype", "max_q_len")]
 
 
+class QkvAppendParams(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "block_size", "num_heads", "num_kv_heads", "head_dim", "batch_size", "total_q", "max_blocks_per_seq",
+        "num_blocks", "src_dtype", "cache_dtype", "rotary_dim", "interleaved", "max_position", "norm",
+        "weight_dtype")] + [("eps", ctypes.c_float), ("weight_offset", ctypes.c_float)] + [
+        (n, ctypes.c_int64) for n in ("query_stride", "key_stride", "value_stride")]
+
+
 class CopyBlocksParams(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("block_size", "num_kv_heads", "head_dim", "num_blocks", "dtype")]
 
@@ -76,7 +84,7 @@ class SampleParams(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("batch_size", "vocab_size", "logits_dtype", "num_masks")]
 
 
-ABI_VERSION = 9  # KYRO_ABI_VERSION of include/kyro_verify.h
+ABI_VERSION = 10  # KYRO_ABI_VERSION of include/kyro_verify.h
 
 _lib = None
 _lib_lock = threading.Lock()
@@ -110,6 +118,7 @@ _SIGNATURES = {
     "kyro_paged_attention_describe": ([_P, ctypes.POINTER(PagedAttentionParams), ctypes.c_int, ctypes.c_char_p,
                                        ctypes.c_size_t, ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
     "kyro_paged_kv_append": ([_P, ctypes.POINTER(KvAppendParams)] + [_P] * 7, ctypes.c_int),
+    "kyro_qkv_append": ([_P, ctypes.POINTER(QkvAppendParams)] + [_P] * 14, ctypes.c_int),
     # include/kyro_blocks.h
     "kyro_radix_create": ([ctypes.c_int32, ctypes.c_int64, ctypes.POINTER(_P)], ctypes.c_int),
     "kyro_radix_destroy": ([_P], ctypes.c_int),

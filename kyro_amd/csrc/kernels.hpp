@@ -14,7 +14,8 @@ enum ErrorBits : int {
     ERR_TOKEN = 8,      // draft token id >= vocab_size
     ERR_NUM_DRAFT = 16, // num_draft outside [0, max_draft]
     ERR_NO_DRAFT = 32,  // a sampled sequence with drafts but no draft_logits
-    ERR_PLAN = 64       // balanced attention schedule: more partial-state slots than the host sized
+    ERR_PLAN = 64,      // balanced attention schedule: more partial-state slots than the host sized
+    ERR_POSITION = 128  // a row's position outside [0, max_position)
 };
 
 
@@ -316,6 +317,36 @@ struct KvAppendArgs {
 };
 
 hipError_t launch_kv_append(const KvAppendArgs& a, hipStream_t stream);
+
+struct QkvAppendArgs {
+    const void* query;       // [total_q, H, D] src dtype, rows q_stride elements apart
+    const void* key;         // [total_q, Hkv, D]
+    const void* value;
+    const int32_t* q_start;  // [B+1] or nullptr
+    const int64_t* positions;  // [total_q] or nullptr (the slot)
+    const int64_t* table;
+    const int64_t* ctx_lens;
+    const float* cos;        // [max_position, rotary / 2]
+    const float* sin;
+    const void* q_weight;    // [D] or nullptr
+    const void* k_weight;
+    void* kc;                // [num_blocks, Hkv, bs, D] dst dtype
+    void* vc;
+    void* out_query;         // [total_q, H, D] dst dtype
+    int* err;
+    int64_t q_stride, k_stride, v_stride;
+    int B, H, Hkv, D, bs, max_blocks, num_blocks, total_q;
+    int rotary, interleaved, max_position, norm, weight_bf16;
+    int src_bf16, dst_bf16;
+    float eps, weight_offset;
+    // Set by qkv_append_setup: elements of a lane's chunk, units of two paired chunks (rotated in
+    // halves), log2 of the lanes of a head row, waves of a packed row.
+    int chunk, pairs, lp_shift, waves_per_row;
+};
+
+// False for sizes that one launch does not carry.
+bool qkv_append_setup(QkvAppendArgs& a);
+hipError_t launch_qkv_append(const QkvAppendArgs& a, hipStream_t stream);
 
 // Whole-block copies within a cache pair (copy-on-write of a prefix block).
 constexpr int kCopyInline = 240;  // block pairs passed in the kernel arguments (2 x 240 x 4 B)

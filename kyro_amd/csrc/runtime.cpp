@@ -143,6 +143,7 @@ int sync_and_report(kyro_ctx ctx) {
     if (err & kyro::ERR_PLAN)
         msg += " balanced attention schedule: the plan needs more partial-state slots than were sized "
                "(internal error; no item ran);";
+    if (err & kyro::ERR_POSITION) msg += " a position outside [0, max_position);";
     return fail(KYRO_EINVAL, "%s", msg.c_str());
 }
 
@@ -1142,6 +1143,108 @@ int kyro_paged_kv_append(kyro_ctx ctx, const kyro_kv_append_params* p, const voi
         KYRO_HIP(dg.status);
         a.err = ctx->err;
         KYRO_HIP(kyro::launch_kv_append(a, ctx->stream));
+        return KYRO_OK;
+    });
+}
+
+int kyro_qkv_append(kyro_ctx ctx, const kyro_qkv_append_params* p, const void* query, const void* key,
+                    const void* value, const int32_t* q_start_loc, const int64_t* positions,
+                    const int64_t* block_table, const int64_t* context_lens, const float* cos, const float* sin,
+                    const void* q_weight, const void* k_weight, void* key_cache, void* value_cache,
+                    void* out_query) {
+    return guarded([&]() -> int {
+        if (!p) return fail(KYRO_EINVAL, "qkv_append: params is null");
+        if (p->block_size <= 0 || p->num_heads <= 0 || p->num_kv_heads <= 0 || p->head_dim <= 0 || p->batch_size < 0 ||
+            p->total_q < 0 || p->max_blocks_per_seq <= 0 || p->num_blocks <= 0)
+            return fail(KYRO_EINVAL, "qkv_append: sizes must be positive (batch_size, total_q >= 0)");
+        if (p->num_heads % p->num_kv_heads != 0)
+            return fail(KYRO_EINVAL, "qkv_append: num_heads %d is not a multiple of num_kv_heads %d", p->num_heads,
+                        p->num_kv_heads);
+        if (p->head_dim % 8 != 0 || p->head_dim > 256)
+            return fail(KYRO_EUNSUPPORTED, "qkv_append: head_dim %d is not supported (multiples of 8 up to 256)",
+                        p->head_dim);
+        if (p->rotary_dim < 0 || p->rotary_dim > p->head_dim || p->rotary_dim % 2 != 0)
+            return fail(KYRO_EINVAL, "qkv_append: rotary_dim %d must be even and in [0, head_dim]", p->rotary_dim);
+        if (!p->interleaved && p->rotary_dim % 4 != 0)
+            return fail(KYRO_EUNSUPPORTED, "qkv_append: rotary_dim %d in halves is not a multiple of 4", p->rotary_dim);
+        if ((p->src_dtype != KYRO_F32 && p->src_dtype != KYRO_BF16) ||
+            (p->cache_dtype != KYRO_F32 && p->cache_dtype != KYRO_BF16) ||
+            (p->weight_dtype != KYRO_F32 && p->weight_dtype != KYRO_BF16))
+            return fail(KYRO_EINVAL, "qkv_append: unknown dtype");
+        if (p->rotary_dim > 0 && (!cos || !sin || p->max_position <= 0))
+            return fail(KYRO_EINVAL, "qkv_append: rotary_dim > 0 needs cos, sin and max_position > 0");
+        if (p->norm != 0 && (!(p->eps >= 0.f) || !std::isfinite(p->eps) || !std::isfinite(p->weight_offset)))
+            return fail(KYRO_EINVAL, "qkv_append: eps must be finite and >= 0, weight_offset finite");
+        if ((p->norm == 0 && (q_weight || k_weight)) || (!q_weight != !k_weight))
+            return fail(KYRO_EINVAL, "qkv_append: norm weights come together, and with norm set");
+        if (!q_start_loc && p->total_q != p->batch_size)
+            return fail(KYRO_EINVAL, "qkv_append: without q_start_loc total_q must equal batch_size");
+        const int64_t q_row = (int64_t)p->num_heads * p->head_dim, kv_row = (int64_t)p->num_kv_heads * p->head_dim;
+        const int64_t qs = p->query_stride ? p->query_stride : q_row, ks = p->key_stride ? p->key_stride : kv_row,
+                      vs = p->value_stride ? p->value_stride : kv_row;
+        if (qs < q_row || ks < kv_row || vs < kv_row || qs % 8 != 0 || ks % 8 != 0 || vs % 8 != 0)
+            return fail(KYRO_EINVAL, "qkv_append: row strides must be multiples of 8 and hold a row's heads");
+        if (p->batch_size == 0 || p->total_q == 0) return check_ctx(ctx);
+        if (!query || !key || !value || !block_table || !context_lens || !key_cache || !value_cache || !out_query)
+            return fail(KYRO_EINVAL, "qkv_append: null device pointer");
+        const auto at = [](const void* x) { return reinterpret_cast<uintptr_t>(x); };
+        if ((at(query) | at(key) | at(value) | at(key_cache) | at(value_cache) | at(out_query) | at(cos) | at(sin) |
+             at(q_weight) | at(k_weight)) % 16 != 0)
+            return fail(KYRO_EINVAL, "qkv_append: tensors must be 16-byte aligned");
+        // A lane reads its elements before it writes them, so the query may be rotated where it lies; any
+        // other overlap would be read after it was written.
+        const size_t in_size = p->src_dtype == KYRO_BF16 ? 2 : 4, out_size = p->cache_dtype == KYRO_BF16 ? 2 : 4;
+        const auto overlaps = [&](const void* x, int64_t stride, int64_t row) {
+            const uintptr_t in0 = at(x), in1 = in0 + ((size_t)(p->total_q - 1) * stride + row) * in_size;
+            const uintptr_t out0 = at(out_query), out1 = out0 + (size_t)p->total_q * q_row * out_size;
+            return in0 < out1 && out0 < in1;
+        };
+        const bool in_place = out_query == query && qs == q_row && p->src_dtype == p->cache_dtype;
+        if ((!in_place && overlaps(query, qs, q_row)) || overlaps(key, ks, kv_row) || overlaps(value, vs, kv_row))
+            return fail(KYRO_EINVAL, "qkv_append: out_query overlaps an input (only the contiguous query itself may)");
+        kyro::QkvAppendArgs a{};
+        a.query = query;
+        a.key = key;
+        a.value = value;
+        a.q_start = q_start_loc;
+        a.positions = positions;
+        a.table = block_table;
+        a.ctx_lens = context_lens;
+        a.cos = cos;
+        a.sin = sin;
+        a.q_weight = q_weight;
+        a.k_weight = k_weight;
+        a.kc = key_cache;
+        a.vc = value_cache;
+        a.out_query = out_query;
+        a.q_stride = qs;
+        a.k_stride = ks;
+        a.v_stride = vs;
+        a.B = p->batch_size;
+        a.H = p->num_heads;
+        a.Hkv = p->num_kv_heads;
+        a.D = p->head_dim;
+        a.bs = p->block_size;
+        a.max_blocks = p->max_blocks_per_seq;
+        a.num_blocks = p->num_blocks;
+        a.total_q = p->total_q;
+        a.rotary = p->rotary_dim;
+        a.interleaved = p->interleaved != 0;
+        a.max_position = p->max_position;
+        a.norm = p->norm != 0;
+        a.weight_bf16 = p->weight_dtype == KYRO_BF16;
+        a.src_bf16 = p->src_dtype == KYRO_BF16;
+        a.dst_bf16 = p->cache_dtype == KYRO_BF16;
+        a.eps = p->eps;
+        a.weight_offset = p->weight_offset;
+        if (!kyro::qkv_append_setup(a))
+            return fail(KYRO_EUNSUPPORTED, "qkv_append: total_q x heads, or head_dim %d with rotary_dim %d, is more than one launch carries",
+                        p->head_dim, p->rotary_dim);
+        if (int rc = check_ctx(ctx)) return rc;  // last, so that a host without a device can have the rest checked
+        DeviceGuard dg(ctx->device);
+        KYRO_HIP(dg.status);
+        a.err = ctx->err;
+        KYRO_HIP(kyro::launch_qkv_append(a, ctx->stream));
         return KYRO_OK;
     });
 }

@@ -31,6 +31,44 @@ def _require(t, name, dtypes, ndim, device):
         raise ValueError(f"{name} must be contiguous")
 
 
+def rope_tables(max_position: int, rotary_dim: int, base: float = 10000.0, *, inv_freq=None, scale: float = 1.0,
+                device=None):
+    """(cos, sin) of every position's angles, [max_position, rotary_dim / 2] float32 each, for
+    :meth:`PagedKVCache.append_qkv` (RotaryEmbedding, src/model/layers.rs:21-62). Frequency i is
+    base^(-2 i / rotary_dim), or ``inv_freq`` (rotary_dim / 2 numbers) for a model that scales them;
+    ``scale`` multiplies both tables. The angles are computed in 64 bits: in 32, position 100000 would be
+    off by 0.004 radians."""
+    max_position, rotary_dim = int(max_position), int(rotary_dim)
+    if max_position <= 0 or rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError("max_position must be positive and rotary_dim a positive even number")
+    if inv_freq is None:
+        freq = float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    else:
+        freq = torch.as_tensor(inv_freq, dtype=torch.float64, device="cpu").reshape(-1)
+        if freq.numel() != rotary_dim // 2:
+            raise ValueError(f"inv_freq has {freq.numel()} entries, expected {rotary_dim // 2}")
+    angle = torch.outer(torch.arange(max_position, dtype=torch.float64), freq)
+    return tuple((f(angle) * scale).to(torch.float32).to(device) for f in (torch.cos, torch.sin))
+
+
+def _rows(t, name, dtype, shape, device):
+    """Element stride between the rows of a [rows, heads, D] tensor whose heads are dense (a slice of a
+    wider projection's output may be)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    n, h, d = shape
+    st = t.stride()
+    if (d > 1 and st[2] != 1) or (h > 1 and st[1] != d):
+        raise ValueError(f"{name}'s heads must be dense: strides (any, {d}, 1), got {st}")
+    return st[0] if n > 1 else h * d  # torch gives a single row any stride
+
+
 class PagedKVCache:
     """Writes new K/V rows into block-table caches (kv_cache.rs:21-35 holds num_kv_heads and
     head_dim; the block size is the paged layout's)."""
@@ -83,6 +121,106 @@ class PagedKVCache:
         _lib.check(_lib.lib().kyro_paged_kv_append(
             ctx.handle, ctypes.byref(params), ptr(key), ptr(value), ptr(q_start_loc),
             ptr(block_table), ptr(context_lens), ptr(key_cache), ptr(value_cache)))
+
+    def append_qkv_async(self, query, key, value, key_cache, value_cache, block_table, context_lens, *, cos=None,
+                         sin=None, positions=None, q_weight=None, k_weight=None, norm_eps=None, weight_offset=0.0,
+                         interleaved=False, q_start_loc=None, out=None):
+        """Queues the pass on torch's current stream and returns the query; see :meth:`append_qkv`."""
+        dev = query.device
+        if dev.type != "cuda":
+            raise ValueError("append_qkv runs on a GPU device; got " + str(dev))
+        if query.dtype not in _DTYPES:
+            raise TypeError(f"query has dtype {query.dtype}, expected one of {tuple(_DTYPES)}")
+        if query.dim() != 3:
+            raise ValueError(f"query must be 3-D, got shape {tuple(query.shape)}")
+        src, (total_q, heads, d) = query.dtype, query.shape
+        hkv, bs = self.num_kv_heads, self.block_size
+        if d != self.head_dim:
+            raise ValueError(f"query heads have {d} elements, expected {self.head_dim}")
+        q_stride = _rows(query, "query", src, (total_q, heads, d), dev)
+        k_stride = _rows(key, "key", src, (total_q, hkv, d), dev)
+        v_stride = _rows(value, "value", src, (total_q, hkv, d), dev)
+        _require(key_cache, "key_cache", (torch.float32, torch.bfloat16), 4, dev)
+        _require(value_cache, "value_cache", (key_cache.dtype,), 4, dev)
+        _require(block_table, "block_table", (torch.int64,), 2, dev)
+        _require(context_lens, "context_lens", (torch.int64,), 1, dev)
+        nb = key_cache.shape[0]
+        if key_cache.shape != (nb, hkv, bs, d) or value_cache.shape != (nb, hkv, bs, d):
+            raise ValueError(f"caches must be {(nb, hkv, bs, d)}")
+        B = context_lens.shape[0]
+        if block_table.shape[0] != B:
+            raise ValueError("block_table and context_lens disagree on the batch size")
+        if q_start_loc is not None:
+            _require(q_start_loc, "q_start_loc", (torch.int32,), 1, dev)
+            if q_start_loc.shape[0] != B + 1:
+                raise ValueError("q_start_loc must have batch+1 entries")
+        elif total_q != B:
+            raise ValueError("without q_start_loc query must have one row per sequence")
+        if positions is not None:
+            _require(positions, "positions", (torch.int64,), 1, dev)
+            if positions.shape[0] != total_q:
+                raise ValueError("positions must have one entry per row")
+        rotary = max_position = 0
+        if (cos is None) != (sin is None):
+            raise ValueError("cos and sin come together")
+        if cos is not None:
+            _require(cos, "cos", (torch.float32,), 2, dev)
+            _require(sin, "sin", (torch.float32,), 2, dev)
+            if cos.shape != sin.shape:
+                raise ValueError("cos and sin must have the same shape")
+            max_position, rotary = cos.shape[0], 2 * cos.shape[1]
+        weight_dtype = src
+        if (q_weight is None) != (k_weight is None):
+            raise ValueError("q_weight and k_weight come together")
+        if q_weight is not None:
+            if norm_eps is None:
+                raise ValueError("norm weights need norm_eps")
+            weight_dtype = q_weight.dtype
+            _require(q_weight, "q_weight", (torch.float32, torch.bfloat16), 1, dev)
+            _require(k_weight, "k_weight", (weight_dtype,), 1, dev)
+            if q_weight.shape[0] != d or k_weight.shape[0] != d:
+                raise ValueError(f"norm weights must have {d} entries")
+        if out is None:
+            out = torch.empty((total_q, heads, d), dtype=key_cache.dtype, device=dev)
+        else:
+            _require(out, "out", (key_cache.dtype,), 3, dev)
+            if out.shape != query.shape:
+                raise ValueError("out has the wrong shape")
+        params = _lib.QkvAppendParams(bs, heads, hkv, d, B, total_q, block_table.shape[1], nb, _DTYPES[src],
+                                      _DTYPES[key_cache.dtype], rotary, 1 if interleaved else 0, max_position,
+                                      0 if norm_eps is None else 1, _DTYPES[weight_dtype],
+                                      0.0 if norm_eps is None else float(norm_eps), float(weight_offset), q_stride,
+                                      k_stride, v_stride)
+        ctx = _lib.context(dev.index or 0)
+        ctx.set_stream(_lib.current_stream(dev.index or 0))
+        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+        _lib.check(_lib.lib().kyro_qkv_append(
+            ctx.handle, ctypes.byref(params), query.data_ptr(), key.data_ptr(), value.data_ptr(), ptr(q_start_loc),
+            ptr(positions), block_table.data_ptr(), context_lens.data_ptr(), ptr(cos), ptr(sin), ptr(q_weight),
+            ptr(k_weight), key_cache.data_ptr(), value_cache.data_ptr(), out.data_ptr()))
+        return out
+
+    def append_qkv(self, query, key, value, key_cache, value_cache, block_table, context_lens, *, cos=None, sin=None,
+                   positions=None, q_weight=None, k_weight=None, norm_eps=None, weight_offset=0.0, interleaved=False,
+                   q_start_loc=None, out=None):
+        """Head norms, rotation and :meth:`append_kv` of a step's new rows in one launch; returns the query
+        that :class:`kyro_amd.PagedAttention` takes, [total_q, H, D] in the caches' dtype (or ``out``, which
+        may be ``query`` itself where that is contiguous and of the caches' dtype).
+
+        ``query`` [total_q, H, D], ``key`` and ``value`` [total_q, Hkv, D] are the projections' rows; they may
+        be slices of one [total_q, H + 2 Hkv, D] output. ``cos`` and ``sin`` (:func:`rope_tables`) turn the
+        first ``2 * cos.shape[1]`` elements of each query and key head, element i with i + half of them, or
+        neighbours with ``interleaved``; without them nothing turns. ``positions`` (int64 [total_q]) are the
+        tables' rows; by default a row's slot in its sequence, which it no longer is after
+        :meth:`kyro_amd.CacheEviction.evict`. ``norm_eps`` asks for the root-mean-square norm of each query
+        and key head, scaled by ``q_weight`` / ``k_weight`` (+ ``weight_offset``) where given. The call
+        synchronises, so a bad block id, context length or position raises KyroError here."""
+        out = self.append_qkv_async(query, key, value, key_cache, value_cache, block_table, context_lens, cos=cos,
+                                    sin=sin, positions=positions, q_weight=q_weight, k_weight=k_weight,
+                                    norm_eps=norm_eps, weight_offset=weight_offset, interleaved=interleaved,
+                                    q_start_loc=q_start_loc, out=out)
+        _lib.context(query.device.index or 0).sync()
+        return out
 
     def append_kv(self, key, value, key_cache, value_cache, block_table, context_lens, *,
                   q_start_loc=None, max_q_len=None):
