@@ -79,6 +79,12 @@ int kyro_bm_allocate(kyro_bm bm, uint64_t request_id, int64_t num_tokens);
 int kyro_bm_append_slots(kyro_bm bm, uint64_t request_id, int64_t n);
 /* Shrinks a request to num_tokens (>= its prompt length), releasing blocks no longer needed. */
 int kyro_bm_truncate(kyro_bm bm, uint64_t request_id, int64_t num_tokens);
+/* Before a request's cached tokens are moved (kyro_kv_evict): replaces every block that the prefix cache or
+ * another request shares by one of its own, with a pending copy (kyro_bm_take_copies), and forgets the
+ * prompt, whose tokens the blocks no longer hold in order: kyro_bm_free then caches nothing, and
+ * kyro_bm_truncate may cut below it. KYRO_ENOSPACE when the free pool (after evicting cache leaves) cannot
+ * hold the copies; the request is unchanged then. */
+int kyro_bm_make_private(kyro_bm bm, uint64_t request_id);
 /* Ends a request. cache_prompt != 0 hands its prompt blocks to the prefix cache (their K/V must
  * have been written); 0 releases them. */
 int kyro_bm_free(kyro_bm bm, uint64_t request_id, int32_t cache_prompt);

@@ -76,6 +76,19 @@ class QkvAppendParams(ctypes.Structure):
         (n, ctypes.c_int64) for n in ("query_stride", "key_stride", "value_stride")]
 
 
+class AttnWeightsParams(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "block_size", "num_heads", "head_dim", "num_kv_heads", "batch_size", "total_q", "max_blocks_per_seq",
+        "num_blocks", "dtype", "causal")] + [("scale", ctypes.c_float)] + [
+        (n, ctypes.c_int32) for n in ("max_q_len", "num_state_rows", "max_tokens")]
+
+
+class KvEvictParams(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "block_size", "num_kv_heads", "head_dim", "batch_size", "max_blocks_per_seq", "num_blocks", "dtype", "budget",
+        "sink", "recent", "num_state_rows", "max_tokens")]
+
+
 class CopyBlocksParams(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("block_size", "num_kv_heads", "head_dim", "num_blocks", "dtype")]
 
@@ -132,6 +145,7 @@ _SIGNATURES = {
     "kyro_bm_allocate": ([_P, ctypes.c_uint64, ctypes.c_int64], ctypes.c_int),
     "kyro_bm_append_slots": ([_P, ctypes.c_uint64, ctypes.c_int64], ctypes.c_int),
     "kyro_bm_truncate": ([_P, ctypes.c_uint64, ctypes.c_int64], ctypes.c_int),
+    "kyro_bm_make_private": ([_P, ctypes.c_uint64], ctypes.c_int),
     "kyro_bm_free": ([_P, ctypes.c_uint64, ctypes.c_int32], ctypes.c_int),
     "kyro_bm_request_blocks": ([_P, ctypes.c_uint64, _P, ctypes.c_int64, _P, _P], ctypes.c_int),
     "kyro_bm_take_copies": ([_P, _P, _P, ctypes.c_int64, _P], ctypes.c_int),
@@ -141,6 +155,12 @@ _SIGNATURES = {
     "kyro_bm_match_prefix": ([_P, _P, ctypes.c_int64, _P, ctypes.c_int64, _P, _P], ctypes.c_int),
     "kyro_bm_write_tables": ([_P, _P, _P, ctypes.c_int32, ctypes.c_int32, _P, _P, _P], ctypes.c_int),
     "kyro_copy_blocks": ([_P, ctypes.POINTER(CopyBlocksParams), _P, _P, _P, _P, ctypes.c_int64], ctypes.c_int),
+    # include/kyro_evict.h
+    "kyro_attn_weights": ([_P, ctypes.POINTER(AttnWeightsParams)] + [_P] * 10, ctypes.c_int),
+    "kyro_attn_weights_workspace": ([_P, ctypes.POINTER(AttnWeightsParams), ctypes.c_int,
+                                     ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
+    "kyro_kv_evict": ([_P, ctypes.POINTER(KvEvictParams)] + [_P] * 10, ctypes.c_int),
+    "kyro_kv_evict_workspace": ([ctypes.POINTER(KvEvictParams), ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
     # include/kyro_sample.h
     "kyro_sample_tokens": ([_P, ctypes.POINTER(SampleParams)] + [_P] * 14, ctypes.c_int),
     "kyro_penalty_adds": ([_P, ctypes.c_int64, ctypes.c_float, ctypes.c_float, ctypes.c_int32, _P, _P,

@@ -152,6 +152,16 @@ class BlockManager:
     def truncate(self, request_id: int, num_tokens: int) -> None:
         _lib.check(_lib.lib().kyro_bm_truncate(self._h, int(request_id), int(num_tokens)))
 
+    def make_private(self, request_id: int) -> bool:
+        """Before :meth:`kyro_amd.CacheEviction.evict`: the request gets blocks of its own for those it
+        shares (:meth:`take_copies` has the copies to queue) and its prompt is no longer handed to the prefix
+        cache, nor a floor for :meth:`truncate`. False, and nothing changes, when no blocks are left."""
+        rc = _lib.lib().kyro_bm_make_private(self._h, int(request_id))
+        if rc == _lib.KYRO_ENOSPACE:
+            return False
+        _lib.check(rc)
+        return True
+
     def free(self, request_id: int, cache_prompt: bool = True) -> None:
         """block_manager.rs:128-153: the prompt's blocks go to the prefix cache."""
         _lib.check(_lib.lib().kyro_bm_free(self._h, int(request_id), 1 if cache_prompt else 0))

@@ -261,6 +261,31 @@ int BlockManager::truncate(uint64_t rid, int64_t num_tokens) {
     return OK;
 }
 
+// A request whose cached tokens are about to be moved (eviction) owns its blocks alone: every one that
+// another holder shares is replaced by a fresh block and a pending copy. Its blocks no longer hold its
+// prompt in order, so the prompt is forgotten: it is not handed to the prefix cache when the request ends,
+// and truncate may cut below it. Evicting cache leaves to make room can only lower reference counts, so
+// the blocks are looked at again after it.
+int BlockManager::make_private(uint64_t rid) {
+    auto it = table_.find(rid);
+    if (it == table_.end()) return EINVAL_;
+    Request& r = it->second;
+    int64_t need = 0;
+    for (int64_t b : r.blocks) need += ref_[(size_t)b] > 1;
+    if (!reserve(need)) return ENOSPACE;
+    for (int64_t& b : r.blocks) {
+        if (ref_[(size_t)b] <= 1) continue;
+        const int64_t fresh = free_.back();
+        free_.pop_back();
+        ref_[(size_t)fresh] = 1;
+        copies_.push_back({b, fresh});  // the request's reference on b is the copy's from here on
+        b = fresh;
+    }
+    r.prompt.clear();
+    r.has_prompt = false;
+    return OK;
+}
+
 // block_manager.rs:128-153 hands the request's blocks to the cache with the prompt. Here the
 // cache takes its own reference on the blocks it did not already hold, then the request drops
 // its reference on all of its blocks, so each block is freed when its last holder lets go.

@@ -1,13 +1,16 @@
 // C ABI of the block manager, the prefix cache, the device block-table writer and block copies
-// (include/kyro_blocks.h). Host logic lives in block_manager.cpp; this file validates arguments,
+// (include/kyro_blocks.h), and of the accumulated attention weights and the eviction by them
+// (include/kyro_evict.h). Host logic lives in block_manager.cpp; this file validates arguments,
 // converts statuses and queues the device work on the context's stream.
 #include <algorithm>
+#include <cmath>
 #include <vector>
 
 #include "block_manager.hpp"
 #include "context.hpp"
 #include "kernels.hpp"
 #include "kyro_blocks.h"
+#include "kyro_evict.h"
 
 using namespace kyro::rt;
 
@@ -41,6 +44,116 @@ int copy_match(const std::pair<std::vector<int64_t>, int64_t>& m, int64_t* out, 
     if (out_n) *out_n = nb;
     if (out_matched) *out_matched = m.second;
     if (out) std::copy(m.first.begin(), m.first.begin() + std::min(nb, std::max<int64_t>(cap, 0)), out);
+    return KYRO_OK;
+}
+
+uintptr_t at(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+// Do two arrays of `bytes` share memory without being the same one?
+bool half_over(const void* x, const void* y, size_t bytes) {
+    return x != y && at(x) < at(y) + bytes && at(y) < at(x) + bytes;
+}
+
+// Tokens a sequence may have: as many as its table and its state hold.
+int64_t token_cap(int32_t max_blocks, int32_t block_size, int32_t max_tokens) {
+    return std::min((int64_t)max_blocks * block_size, (int64_t)max_tokens);
+}
+
+// Sizes, variant and scratch of a kyro_attn_weights call, from its params alone.
+int weights_setup(const kyro_attn_weights_params* p, bool has_q_start, int num_cus, kyro::AttnWeightsArgs& a,
+                  size_t& bytes) {
+    bytes = 0;
+    if (!p) return fail(KYRO_EINVAL, "attn_weights: params is null");
+    if (p->block_size <= 0 || p->num_heads <= 0 || p->head_dim <= 0 || p->num_kv_heads <= 0 || p->batch_size < 0 ||
+        p->total_q < 0 || p->max_blocks_per_seq <= 0 || p->num_blocks <= 0 || p->max_q_len < 0 ||
+        p->num_state_rows <= 0 || p->max_tokens <= 0)
+        return fail(KYRO_EINVAL, "attn_weights: sizes must be positive (batch_size, total_q, max_q_len >= 0)");
+    if (p->num_heads % p->num_kv_heads != 0)
+        return fail(KYRO_EINVAL, "attn_weights: num_heads %d is not a multiple of num_kv_heads %d", p->num_heads,
+                    p->num_kv_heads);
+    if (p->head_dim % 8 != 0 || p->head_dim > 256)
+        return fail(KYRO_EUNSUPPORTED, "attn_weights: head_dim %d is not supported (multiples of 8 up to 256)", p->head_dim);
+    if (p->dtype != KYRO_F32 && p->dtype != KYRO_BF16) return fail(KYRO_EINVAL, "attn_weights: unknown dtype");
+    if (!std::isfinite(p->scale)) return fail(KYRO_EINVAL, "attn_weights: scale is not finite");
+    if (!has_q_start && p->total_q != p->batch_size)
+        return fail(KYRO_EINVAL, "attn_weights: without q_start_loc total_q must equal batch_size");
+    a.B = p->batch_size;
+    a.H = p->num_heads;
+    a.Hkv = p->num_kv_heads;
+    a.group = a.H / a.Hkv;
+    a.D = p->head_dim;
+    a.bs = p->block_size;
+    a.bs_shift = -1;
+    for (int i = 0; i < 31; ++i)
+        if (a.bs == 1 << i) a.bs_shift = i;
+    a.max_blocks = p->max_blocks_per_seq;
+    a.num_blocks = p->num_blocks;
+    a.total_q = p->total_q;
+    a.max_q_len = !has_q_start ? 1 : p->max_q_len > 0 ? p->max_q_len : p->total_q;
+    a.num_state_rows = p->num_state_rows;
+    a.max_tokens = p->max_tokens;
+    a.causal = p->causal != 0;
+    a.bf16 = p->dtype == KYRO_BF16;
+    a.cap = token_cap(a.max_blocks, a.bs, a.max_tokens);
+    const double scale = p->scale != 0.f ? (double)p->scale : 1.0 / std::sqrt((double)a.D);
+    a.scale_log2 = (float)(scale * 1.4426950408889634);
+    if (a.B == 0 || a.total_q == 0) return KYRO_OK;
+    const int64_t rows = (int64_t)std::min(a.max_q_len, a.total_q) * a.group;
+    if (a.cap > (1 << 30) || rows > (1 << 30) || (int64_t)a.total_q * a.H > INT32_MAX)
+        return fail(KYRO_EUNSUPPORTED, "attn_weights: more tokens or query rows than one launch carries");
+    a.tiles = rows <= 16 ? 1 : 2;
+    const int64_t row_groups = (rows + 16 * a.tiles - 1) / (16 * a.tiles);
+    const auto stat_items = [&](int64_t chunk) { return a.B * ((a.cap + chunk - 1) / chunk) * a.Hkv * row_groups; };
+    const auto part_bytes = [&](int64_t chunk) {
+        return (size_t)((a.cap + chunk - 1) / chunk) * a.total_q * a.H * sizeof(float2);
+    };
+    int64_t chunk = 64;
+    while (chunk < 1024 && stat_items(2 * chunk) >= 4 * num_cus) chunk *= 2;
+    while (part_bytes(chunk) > ((size_t)64 << 20) && chunk < a.cap) chunk *= 2;
+    a.chunk = (int)chunk;
+    // 64 sequences' items are counted in 32 bits.
+    if ((double)((a.cap + chunk - 1) / chunk) * a.Hkv * row_groups * 64 > INT32_MAX ||
+        (double)((a.cap + 63) / 64) * a.Hkv * 64 > INT32_MAX)
+        return fail(KYRO_EUNSUPPORTED, "attn_weights: more work items a sequence than one launch carries");
+    a.sum_tokens = a.B * ((a.cap + 255) / 256) * a.Hkv >= 2 * num_cus ? 64 : 16;
+    a.stat_grid = (int)std::min<int64_t>(stat_items(chunk), 8 * (int64_t)num_cus);
+    a.sum_grid = (int)std::min<int64_t>(a.B * ((a.cap + 63) / 64) * a.Hkv, 8 * (int64_t)num_cus);
+    bytes = align_up(part_bytes(chunk), 256);
+    return KYRO_OK;
+}
+
+int evict_setup(const kyro_kv_evict_params* p, kyro::EvictArgs& a, size_t& bytes) {
+    bytes = 0;
+    if (!p) return fail(KYRO_EINVAL, "kv_evict: params is null");
+    if (p->block_size <= 0 || p->num_kv_heads <= 0 || p->head_dim <= 0 || p->batch_size < 0 ||
+        p->max_blocks_per_seq <= 0 || p->num_blocks <= 0 || p->num_state_rows <= 0 || p->max_tokens <= 0)
+        return fail(KYRO_EINVAL, "kv_evict: sizes must be positive (batch_size >= 0)");
+    if (p->head_dim % 8 != 0 || p->head_dim > 256)
+        return fail(KYRO_EUNSUPPORTED, "kv_evict: head_dim %d is not supported (multiples of 8 up to 256)", p->head_dim);
+    if (p->dtype != KYRO_F32 && p->dtype != KYRO_BF16) return fail(KYRO_EINVAL, "kv_evict: unknown dtype");
+    if (p->budget <= 0 || p->sink < 0 || p->recent < 0 || (int64_t)p->sink + p->recent > p->budget)
+        return fail(KYRO_EINVAL, "kv_evict: need budget > 0, sink >= 0, recent >= 0 and sink + recent <= budget");
+    a.cap = token_cap(p->max_blocks_per_seq, p->block_size, p->max_tokens);
+    if (a.cap > (1 << 30) || (int64_t)p->batch_size * p->num_kv_heads > (1 << 24))
+        return fail(KYRO_EUNSUPPORTED, "kv_evict: more tokens or sequences than one launch carries");
+    a.B = p->batch_size;
+    a.Hkv = p->num_kv_heads;
+    a.bs = p->block_size;
+    a.max_blocks = p->max_blocks_per_seq;
+    a.num_blocks = p->num_blocks;
+    a.num_state_rows = p->num_state_rows;
+    a.max_tokens = p->max_tokens;
+    a.row_vecs = p->head_dim * (p->dtype == KYRO_BF16 ? 2 : 4) / 16;
+    a.budget = p->budget;
+    a.sink = p->sink;
+    a.recent = p->recent;
+    a.max_moves = (int)std::max<int64_t>(0, std::min<int64_t>(a.budget, a.cap - a.budget));
+    a.lds_keys = (int)std::min<int64_t>(a.cap, kyro::kEvictLdsKeys);
+    // About 4096 workgroups in all for the copies, each with at least 1024 vectors where the most tokens move.
+    const int64_t units = std::max<int64_t>(1, (int64_t)a.B * a.Hkv);
+    a.move_wgs = (int)std::max<int64_t>(1, std::min<int64_t>((4096 + units - 1) / units, ((int64_t)a.max_moves * a.row_vecs + 1023) / 1024));
+    bytes = align_up((size_t)a.B * a.Hkv * sizeof(int), 256) +
+            align_up((size_t)a.B * a.Hkv * 2 * a.max_moves * sizeof(int32_t), 256);
     return KYRO_OK;
 }
 
@@ -147,6 +260,13 @@ int kyro_bm_truncate(kyro_bm bm, uint64_t request_id, int64_t num_tokens) {
     return guarded([&]() -> int {
         if (!bm) return fail(KYRO_EINVAL, "bm_truncate: null handle");
         return bm_status(bm->m.truncate(request_id, num_tokens), "bm_truncate", request_id);
+    });
+}
+
+int kyro_bm_make_private(kyro_bm bm, uint64_t request_id) {
+    return guarded([&]() -> int {
+        if (!bm) return fail(KYRO_EINVAL, "bm_make_private: null handle");
+        return bm_status(bm->m.make_private(request_id), "bm_make_private", request_id);
     });
 }
 
@@ -300,6 +420,109 @@ int kyro_copy_blocks(kyro_ctx ctx, const kyro_copy_blocks_params* p, void* key_c
         a.vc = static_cast<uint4*>(value_cache);
         KYRO_HIP(kyro::launch_copy_blocks(a, ctx->stream));
         return KYRO_OK;
+    });
+}
+
+// ----------------------------------------------------- attention weights and eviction
+
+int kyro_attn_weights(kyro_ctx ctx, const kyro_attn_weights_params* p, const void* query, const int32_t* q_start_loc,
+                      const int64_t* row_positions, const void* key_cache, const int64_t* block_table,
+                      const int64_t* context_lens, const int32_t* state_rows, const float* weights,
+                      float* out_weights, int32_t* positions) {
+    return guarded([&]() -> int {
+        kyro::AttnWeightsArgs a{};
+        size_t bytes = 0;
+        if (int rc = weights_setup(p, q_start_loc != nullptr, ctx ? ctx->num_cus : 256, a, bytes)) return rc;
+        if (a.B == 0 || a.total_q == 0) return check_ctx(ctx);
+        if (!query || !key_cache || !block_table || !context_lens || !weights || !out_weights || !positions)
+            return fail(KYRO_EINVAL, "attn_weights: null device pointer");
+        if ((at(query) | at(key_cache)) % 16 != 0)
+            return fail(KYRO_EINVAL, "attn_weights: query and key_cache must be 16-byte aligned");
+        if (!state_rows && a.B > a.num_state_rows)
+            return fail(KYRO_EINVAL, "attn_weights: without state_rows the batch needs a state row each");
+        if (half_over(weights, out_weights, (size_t)a.num_state_rows * a.Hkv * a.max_tokens * sizeof(float)))
+            return fail(KYRO_EINVAL, "attn_weights: out_weights overlaps weights (only weights itself may)");
+        if (int rc = check_ctx(ctx)) return rc;  // last, so that a host without a device can have the rest checked
+        a.q = query;
+        a.q_start = q_start_loc;
+        a.row_pos = row_positions;
+        a.k = key_cache;
+        a.table = block_table;
+        a.ctx_lens = context_lens;
+        a.state_rows = state_rows;
+        a.w = weights;
+        a.out_w = out_weights;
+        a.positions = positions;
+        DeviceGuard dg(ctx->device);
+        KYRO_HIP(dg.status);
+        if (int rc = ensure_arena(ctx, bytes)) return rc;
+        a.part = static_cast<float2*>(ctx->arena);
+        a.err = ctx->err;
+        KYRO_HIP(kyro::launch_attn_weights(a, ctx->stream));
+        return KYRO_OK;
+    });
+}
+
+int kyro_attn_weights_workspace(kyro_ctx ctx, const kyro_attn_weights_params* p, int has_q_start_loc, size_t* bytes) {
+    return guarded([&]() -> int {
+        if (!bytes) return fail(KYRO_EINVAL, "attn_weights_workspace: bytes is null");
+        kyro::AttnWeightsArgs a{};
+        return weights_setup(p, has_q_start_loc != 0, ctx ? ctx->num_cus : 256, a, *bytes);
+    });
+}
+
+int kyro_kv_evict(kyro_ctx ctx, const kyro_kv_evict_params* p, void* key_cache, void* value_cache,
+                  const int64_t* block_table, const int64_t* context_lens, const int32_t* state_rows,
+                  const float* weights, const int32_t* positions, float* out_weights, int32_t* out_positions,
+                  int64_t* out_context_lens) {
+    return guarded([&]() -> int {
+        kyro::EvictArgs a{};
+        size_t bytes = 0;
+        if (int rc = evict_setup(p, a, bytes)) return rc;
+        if (a.B == 0) return check_ctx(ctx);
+        if (!key_cache || !value_cache || !block_table || !context_lens || !weights || !positions || !out_weights ||
+            !out_positions || !out_context_lens)
+            return fail(KYRO_EINVAL, "kv_evict: null device pointer");
+        if ((at(key_cache) | at(value_cache)) % 16 != 0) return fail(KYRO_EINVAL, "kv_evict: caches must be 16-byte aligned");
+        if (!state_rows && a.B > a.num_state_rows)
+            return fail(KYRO_EINVAL, "kv_evict: without state_rows the batch needs a state row each");
+        const size_t state = (size_t)a.num_state_rows * a.Hkv * a.max_tokens * 4;
+        if (half_over(weights, out_weights, state) || half_over(positions, out_positions, state) ||
+            at(weights) == at(out_positions) || at(positions) == at(out_weights) || at(out_weights) == at(out_positions) ||
+            half_over(weights, out_positions, state) || half_over(positions, out_weights, state) ||
+            half_over(out_weights, out_positions, state))
+            return fail(KYRO_EINVAL, "kv_evict: out_weights and out_positions overlap an input (only their own input may)");
+        const size_t lens = (size_t)a.B * sizeof(int64_t);
+        if (context_lens == out_context_lens || half_over(context_lens, out_context_lens, lens))
+            return fail(KYRO_EINVAL, "kv_evict: out_context_lens overlaps context_lens");
+        if (int rc = check_ctx(ctx)) return rc;  // last, so that a host without a device can have the rest checked
+        a.kc = static_cast<uint4*>(key_cache);
+        a.vc = static_cast<uint4*>(value_cache);
+        a.table = block_table;
+        a.ctx_lens = context_lens;
+        a.state_rows = state_rows;
+        a.weights = weights;
+        a.positions = positions;
+        a.out_weights = out_weights;
+        a.out_positions = out_positions;
+        a.out_ctx_lens = out_context_lens;
+        DeviceGuard dg(ctx->device);
+        KYRO_HIP(dg.status);
+        if (int rc = ensure_arena(ctx, bytes)) return rc;
+        a.num_moves = static_cast<int*>(ctx->arena);
+        a.moves = reinterpret_cast<int32_t*>(static_cast<char*>(ctx->arena) +
+                                             align_up((size_t)a.B * a.Hkv * sizeof(int), 256));
+        a.err = ctx->err;
+        KYRO_HIP(kyro::launch_kv_evict(a, ctx->stream));
+        return KYRO_OK;
+    });
+}
+
+int kyro_kv_evict_workspace(const kyro_kv_evict_params* p, size_t* bytes) {
+    return guarded([&]() -> int {
+        if (!bytes) return fail(KYRO_EINVAL, "kv_evict_workspace: bytes is null");
+        kyro::EvictArgs a{};
+        return evict_setup(p, a, *bytes);
     });
 }
 

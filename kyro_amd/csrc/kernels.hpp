@@ -15,7 +15,8 @@ enum ErrorBits : int {
     ERR_NUM_DRAFT = 16, // num_draft outside [0, max_draft]
     ERR_NO_DRAFT = 32,  // a sampled sequence with drafts but no draft_logits
     ERR_PLAN = 64,      // balanced attention schedule: more partial-state slots than the host sized
-    ERR_POSITION = 128  // a row's position outside [0, max_position)
+    ERR_POSITION = 128, // a row's position outside [0, max_position)
+    ERR_STATE_ROW = 256 // a state row outside [0, num_state_rows), or named by two sequences
 };
 
 
@@ -347,6 +348,56 @@ struct QkvAppendArgs {
 // False for sizes that one launch does not carry.
 bool qkv_append_setup(QkvAppendArgs& a);
 hipError_t launch_qkv_append(const QkvAppendArgs& a, hipStream_t stream);
+
+// Accumulated attention weight per cached token.
+constexpr int kWeightRows = 32;       // query rows a workgroup of the sum pass stages at a time
+struct AttnWeightsArgs {
+    const void* q;              // [total_q, H, D]
+    const int32_t* q_start;     // [B+1] or nullptr
+    const int64_t* row_pos;     // [total_q] or nullptr
+    const void* k;              // [num_blocks, Hkv, bs, D]
+    const int64_t* table;
+    const int64_t* ctx_lens;
+    const int32_t* state_rows;  // [B] or nullptr
+    const float* w;             // [num_state_rows, Hkv, max_tokens]
+    float* out_w;
+    int32_t* positions;
+    float2* part;               // [chunks, total_q, H]: a row's (max, sum) over a chunk's tokens
+    int* err;
+    int B, H, Hkv, group, D, bs, bs_shift, max_blocks, num_blocks, total_q, max_q_len, num_state_rows, max_tokens;
+    int causal, bf16;
+    int64_t cap;                // tokens a sequence may have: the least of the table's and the state's
+    float scale_log2;
+    int chunk;                  // tokens of a chunk of the statistics pass
+    int tiles;                  // 16-row tiles a wave of the statistics pass holds (1, 2)
+    int sum_tokens;             // tokens a wave of the sum pass holds
+    int stat_grid, sum_grid;    // workgroups
+};
+
+hipError_t launch_attn_weights(const AttnWeightsArgs& a, hipStream_t stream);
+
+// Eviction by accumulated weight.
+constexpr int kEvictLdsKeys = 12288;  // keys the selection keeps in LDS (48 KiB: two workgroups a CU)
+struct EvictArgs {
+    uint4* kc;
+    uint4* vc;
+    const int64_t* table;
+    const int64_t* ctx_lens;
+    const int32_t* state_rows;  // [B] or nullptr
+    const float* weights;       // [num_state_rows, Hkv, max_tokens]
+    const int32_t* positions;
+    float* out_weights;
+    int32_t* out_positions;
+    int64_t* out_ctx_lens;
+    int* num_moves;             // [B, Hkv]
+    int32_t* moves;             // [B, Hkv, 2, max_moves]: holes, then movers
+    int* err;
+    int64_t cap;
+    int B, Hkv, bs, max_blocks, num_blocks, num_state_rows, max_tokens, row_vecs;
+    int budget, sink, recent, max_moves, lds_keys, move_wgs;
+};
+
+hipError_t launch_kv_evict(const EvictArgs& a, hipStream_t stream);
 
 // Whole-block copies within a cache pair (copy-on-write of a prefix block).
 constexpr int kCopyInline = 240;  // block pairs passed in the kernel arguments (2 x 240 x 4 B)

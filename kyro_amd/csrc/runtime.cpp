@@ -60,7 +60,7 @@ int ensure_arena(kyro_ctx ctx, size_t bytes) {
     if (cap != hipStreamCaptureStatusNone)
         return fail(KYRO_EINVAL, "the call needs %zu bytes of scratch arena and the context holds %zu; the stream "
                     "is capturing a graph, so the arena cannot grow now: call kyro_ctx_reserve(ctx, %zu) "
-                    "(or the size queries kyro_paged_attention_workspace / kyro_spec_verify_workspace) "
+                    "(or the kyro_*_workspace size queries) "
                     "before capturing", bytes, ctx->arena_bytes, bytes);
     const size_t want = align_up(std::max(bytes, ctx->arena_bytes * 3 / 2), size_t(1) << 20);
     KYRO_HIP(hipStreamSynchronize(ctx->stream));
@@ -135,7 +135,7 @@ int sync_and_report(kyro_ctx ctx) {
     std::string msg = "device-side validation failed:";
     if (err & kyro::ERR_BLOCK_ID) msg += " block_table entry outside [0, num_blocks);";
     if (err & kyro::ERR_CTX_LEN)
-        msg += " context length < 0 or > max_blocks_per_seq * block_size (or, for kv_append, below the new rows);";
+        msg += " context length < 0 or > max_blocks_per_seq * block_size (or max_tokens, or below the rows of an append);";
     if (err & kyro::ERR_Q_LAYOUT) msg += " q_start_loc not monotone / out of range, or q_len > max_q_len;";
     if (err & kyro::ERR_TOKEN) msg += " a draft, bias or penalty token id >= vocab_size, or a mask_row >= num_masks;";
     if (err & kyro::ERR_NUM_DRAFT) msg += " num_draft outside [0, max_draft];";
@@ -143,6 +143,7 @@ int sync_and_report(kyro_ctx ctx) {
     if (err & kyro::ERR_PLAN)
         msg += " balanced attention schedule: the plan needs more partial-state slots than were sized "
                "(internal error; no item ran);";
+    if (err & kyro::ERR_STATE_ROW) msg += " a state row outside [0, num_state_rows) or named by two sequences;";
     if (err & kyro::ERR_POSITION) msg += " a position outside [0, max_position);";
     return fail(KYRO_EINVAL, "%s", msg.c_str());
 }
