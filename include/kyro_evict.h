@@ -42,7 +42,7 @@ typedef struct kyro_attn_weights_params {
     int32_t num_blocks;          /* leading dim of the cache */
     int32_t dtype;               /* kyro_dtype of query and key_cache */
     int32_t causal;              /* as for kyro_paged_attention_mq */
-    float scale;                 /* 0 => 1/sqrt(head_dim) */
+    float scale;                 /* >= 0; 0 => 1/sqrt(head_dim) */
     int32_t max_q_len;           /* upper bound on query rows per sequence; 0 => 1 without q_start_loc,
                                     total_q with it */
     int32_t num_state_rows;      /* leading dim of weights and positions */

@@ -21,7 +21,7 @@ LIB = os.path.join(HERE, "libkyro_verify.so")
 STATIC_LIB = os.path.join(HERE, "libkyro_verify.a")
 SOURCES = ["runtime.cpp", "upload.hip", "blocks_abi.cpp", "block_manager.cpp", "sample_abi.cpp", "ngram_abi.cpp",
            "paged_attention.hip", "paged_attention_hd.hip", "paged_attention_hd_wide.hip", "paged_attention_hd_f32.hip",
-           "prefill_attention.hip", "prefill_attention_wide.hip", "prefill_attention_f32.hip", "spec_verify.hip", "kv_append.hip", "qkv_append.hip", "attn_weights.hip", "kv_evict.hip",
+           "prefill_attention.hip", "prefill_attention_wide.hip", "prefill_attention_f32.hip", "spec_verify.hip", "kv_append.hip", "qkv_append.hip", "attn_weights.hip", "attn_weights_f32.hip", "kv_evict.hip",
            "sample.hip", "ngram.hip", "noalloc.hip"]
 ARCH = "gfx950"
 # Per-source flags. paged_attention.hip (the head-dim-128 MFMA kernels, bf16 and f32) takes MFMA
@@ -33,7 +33,8 @@ ARCH = "gfx950"
 # short product chains up in VGPRs and take the same form (head dim 112, 64 sequences of 1000 tokens,
 # 5 rows, 32/8 heads: 143.6 -> 106.8 us). The other head dims' bf16 kernels keep the
 # default (head dim 160 measured 271.7 -> 298.2 us and 256 432.5 -> 445.7 us in VGPR form).
-EXTRA_FLAGS = {s: ["-mllvm", "-amdgpu-mfma-vgpr-form=true"] for s in ("paged_attention.hip", "paged_attention_hd_f32.hip")}
+EXTRA_FLAGS = {s: ["-mllvm", "-amdgpu-mfma-vgpr-form=true"] for s in ("paged_attention.hip", "paged_attention_hd_f32.hip", "attn_weights.hip",
+                                                                             "attn_weights_f32.hip")}
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 

@@ -74,7 +74,8 @@ int weights_setup(const kyro_attn_weights_params* p, bool has_q_start, int num_c
     if (p->head_dim % 8 != 0 || p->head_dim > 256)
         return fail(KYRO_EUNSUPPORTED, "attn_weights: head_dim %d is not supported (multiples of 8 up to 256)", p->head_dim);
     if (p->dtype != KYRO_F32 && p->dtype != KYRO_BF16) return fail(KYRO_EINVAL, "attn_weights: unknown dtype");
-    if (!std::isfinite(p->scale)) return fail(KYRO_EINVAL, "attn_weights: scale is not finite");
+    if (!(p->scale >= 0.f) || !std::isfinite(p->scale))
+        return fail(KYRO_EINVAL, "attn_weights: scale must be finite and >= 0");
     if (!has_q_start && p->total_q != p->batch_size)
         return fail(KYRO_EINVAL, "attn_weights: without q_start_loc total_q must equal batch_size");
     a.B = p->batch_size;
@@ -99,26 +100,47 @@ int weights_setup(const kyro_attn_weights_params* p, bool has_q_start, int num_c
     a.scale_log2 = (float)(scale * 1.4426950408889634);
     if (a.B == 0 || a.total_q == 0) return KYRO_OK;
     const int64_t rows = (int64_t)std::min(a.max_q_len, a.total_q) * a.group;
-    if (a.cap > (1 << 30) || rows > (1 << 30) || (int64_t)a.total_q * a.H > INT32_MAX)
+    const double block_elems = (double)a.Hkv * a.bs * a.D;
+    if (a.cap > (1 << 30) || rows > (1 << 30) || (int64_t)a.total_q * a.H > INT32_MAX || block_elems > UINT32_MAX)
         return fail(KYRO_EUNSUPPORTED, "attn_weights: more tokens or query rows than one launch carries");
-    a.tiles = rows <= 16 ? 1 : 2;
-    const int64_t row_groups = (rows + 16 * a.tiles - 1) / (16 * a.tiles);
-    const auto stat_items = [&](int64_t chunk) { return a.B * ((a.cap + chunk - 1) / chunk) * a.Hkv * row_groups; };
+    a.block_elems = (uint32_t)block_elems;
+    const int most_few = kyro::attn_weights_few_rows(a.bf16, a.D), hold = kyro::attn_weights_many_hold(a.bf16, a.D);
+    const bool many = rows > most_few;
+    a.few_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : most_few;
+    const int64_t groups = many ? (rows + hold - 1) / hold : 1;
+    const auto items = [&](int64_t chunk) { return a.B * ((a.cap + chunk - 1) / chunk) * a.Hkv * groups; };
     const auto part_bytes = [&](int64_t chunk) {
         return (size_t)((a.cap + chunk - 1) / chunk) * a.total_q * a.H * sizeof(float2);
     };
-    int64_t chunk = 64;
-    while (chunk < 1024 && stat_items(2 * chunk) >= 4 * num_cus) chunk *= 2;
+    a.kept_rows = (int)((rows + 3) / 4 * 4);
+    // Scores are kept where writing and reading them (8 bytes a row and token) is enough less than reading the
+    // keys again: 64 x 4096 tokens, 32/8 heads of 128 in bf16 (256 bytes a key) took 231 us kept and 205 us
+    // computed again at 32 rows; f32 keys of 512 bytes 87 and 133 us at 5 rows.
+    const bool keep = !many && (rows <= 16 || (rows <= 32 && 10 * a.kept_rows <= a.D * (a.bf16 ? 2 : 4)));
+    // Chunks as long as they may be while there are a few for each CU: a chunk costs its start (a walk to its
+    // sequence, its queries, its first keys), the last ones leave CUs idle. 8 x 2048 and 16 x 1024 tokens a CU
+    // measured best on the two cases above.
+    int64_t chunk = many ? 256 : 64;
+    while (chunk < (keep ? 1024 : 2048) && items(2 * chunk) >= (keep ? 8 : 4) * num_cus) chunk *= 2;
     while (part_bytes(chunk) > ((size_t)64 << 20) && chunk < a.cap) chunk *= 2;
     a.chunk = (int)chunk;
     // 64 sequences' items are counted in 32 bits.
-    if ((double)((a.cap + chunk - 1) / chunk) * a.Hkv * row_groups * 64 > INT32_MAX ||
-        (double)((a.cap + 63) / 64) * a.Hkv * 64 > INT32_MAX)
-        return fail(KYRO_EUNSUPPORTED, "attn_weights: more work items a sequence than one launch carries");
-    a.sum_tokens = a.B * ((a.cap + 255) / 256) * a.Hkv >= 2 * num_cus ? 64 : 16;
-    a.stat_grid = (int)std::min<int64_t>(stat_items(chunk), 8 * (int64_t)num_cus);
-    a.sum_grid = (int)std::min<int64_t>(a.B * ((a.cap + 63) / 64) * a.Hkv, 8 * (int64_t)num_cus);
-    bytes = align_up(part_bytes(chunk), 256);
+    if ((double)((a.cap + 63) / 64) * a.Hkv * groups * 64 > INT32_MAX)
+        return fail(KYRO_EUNSUPPORTED, "attn_weights: more work items than one launch carries");
+    // Where some sequences have fewer rows than the largest, the few-row kernels take those they can.
+    const int64_t most = 8 * (int64_t)num_cus;
+    const bool mixed = many && (int64_t)a.total_q < (int64_t)a.B * a.max_q_len;
+    if (many && !mixed) a.few_rows = 0;
+    a.few_items_most = many && !mixed ? 0 : a.B * ((a.cap + chunk - 1) / chunk) * a.Hkv;
+    a.few_grid = (int)std::min(most, a.few_items_most);
+    a.many_stat_grid = many ? (int)std::min(most, items(chunk)) : 0;
+    a.many_sum_grid = many ? (int)std::min(most, a.B * ((a.cap + hold - 1) / hold) * a.Hkv) : 0;
+    bytes = align_up(part_bytes(chunk), 256) + (many ? align_up((size_t)a.total_q * a.H * sizeof(float), 256) : 0);
+    if (keep) {  // at most 256 MiB of them: items past that are computed again
+        const size_t item = (size_t)chunk * a.kept_rows * sizeof(float);
+        a.kept_items = std::min<int64_t>(a.few_items_most, (int64_t)(((size_t)256 << 20) / item));
+        bytes += align_up((size_t)a.kept_items * item, 256);
+    }
     return KYRO_OK;
 }
 
@@ -456,7 +478,14 @@ int kyro_attn_weights(kyro_ctx ctx, const kyro_attn_weights_params* p, const voi
         DeviceGuard dg(ctx->device);
         KYRO_HIP(dg.status);
         if (int rc = ensure_arena(ctx, bytes)) return rc;
-        a.part = static_cast<float2*>(ctx->arena);
+        char* base = static_cast<char*>(ctx->arena);
+        a.part = reinterpret_cast<float2*>(base);
+        base += align_up((size_t)((a.cap + a.chunk - 1) / a.chunk) * a.total_q * a.H * sizeof(float2), 256);
+        if (a.many_stat_grid) {
+            a.lse = reinterpret_cast<float*>(base);
+            base += align_up((size_t)a.total_q * a.H * sizeof(float), 256);
+        }
+        a.kept = reinterpret_cast<float*>(base);
         a.err = ctx->err;
         KYRO_HIP(kyro::launch_attn_weights(a, ctx->stream));
         return KYRO_OK;

@@ -350,7 +350,6 @@ bool qkv_append_setup(QkvAppendArgs& a);
 hipError_t launch_qkv_append(const QkvAppendArgs& a, hipStream_t stream);
 
 // Accumulated attention weight per cached token.
-constexpr int kWeightRows = 32;       // query rows a workgroup of the sum pass stages at a time
 struct AttnWeightsArgs {
     const void* q;              // [total_q, H, D]
     const int32_t* q_start;     // [B+1] or nullptr
@@ -363,18 +362,28 @@ struct AttnWeightsArgs {
     float* out_w;
     int32_t* positions;
     float2* part;               // [chunks, total_q, H]: a row's (max, sum) over a chunk's tokens
+    float* lse;                 // [total_q, H]: merged over the chunks (many-row kernels)
+    float* kept;                // [kept_items, kept_rows / 4, chunk, 4]: scores, in base 2
     int* err;
     int B, H, Hkv, group, D, bs, bs_shift, max_blocks, num_blocks, total_q, max_q_len, num_state_rows, max_tokens;
     int causal, bf16;
+    uint32_t block_elems;       // Hkv * bs * D
     int64_t cap;                // tokens a sequence may have: the least of the table's and the state's
     float scale_log2;
-    int chunk;                  // tokens of a chunk of the statistics pass
-    int tiles;                  // 16-row tiles a wave of the statistics pass holds (1, 2)
-    int sum_tokens;             // tokens a wave of the sum pass holds
-    int stat_grid, sum_grid;    // workgroups
+    int chunk;                  // tokens of a chunk of the statistics pass, a multiple of 64
+    int few_rows;               // sequences of up to as many rows a kv head go to the few-row kernels (16, 32, 64)
+    int kept_rows;              // rows of a kept token's scores, a multiple of 4
+    int few_grid, many_stat_grid, many_sum_grid;  // workgroups; 0: not launched
+    int64_t few_items_most;     // work items of the few-row kernels where every context is as long as it may be
+    int64_t kept_items;         // items whose scores have room; 0: scores are not kept
 };
 
+// Rows a kv head up to which a sequence can go to the few-row kernels.
+int attn_weights_few_rows(bool bf16, int D);
+// Rows (statistics) or tokens (sums) that a workgroup of the many-row kernels holds.
+int attn_weights_many_hold(bool bf16, int D);
 hipError_t launch_attn_weights(const AttnWeightsArgs& a, hipStream_t stream);
+void launch_attn_weights_f32(const AttnWeightsArgs& a, hipStream_t stream);
 
 // Eviction by accumulated weight.
 constexpr int kEvictLdsKeys = 12288;  // keys the selection keeps in LDS (48 KiB: two workgroups a CU)
