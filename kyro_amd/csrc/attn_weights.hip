@@ -14,6 +14,8 @@
 // element 8 (lane / 16), so keys and queries go from memory straight into them, 16 bytes a lane, whatever
 // the block size; the result has the first operand's index in the lane's four registers and the second's
 // in the lane. The f32 caches take 16x16x4 products on 4-element pieces, the same pieces for both operands.
+#include <type_traits>
+
 #include "common.hpp"
 #include "kernels.hpp"
 
@@ -148,15 +150,20 @@ __device__ __forceinline__ int64_t key_offset(const AttnWeightsArgs& a, int64_t 
     return (int64_t)((uint64_t)(uint32_t)blk * a.block_elems + in_block);
 }
 
+// r / group: group_magic is 2^32 / group rounded up, exact while r * group < 2^32.
+__device__ __forceinline__ int step_row(const AttnWeightsArgs& a, int r) {
+    return a.group == 1 ? r : (int)__umulhi((uint32_t)r, a.group_magic);
+}
+
 // Row r (of a kv head's n * group rows, row by row) in the query, counted in rows of D.
 __device__ __forceinline__ size_t query_row(const AttnWeightsArgs& a, const Sequence& s, int h, int r) {
-    const int j = r / a.group;
+    const int j = step_row(a, r);
     return (size_t)(s.q0 + j) * a.H + (size_t)h * a.group + (r - j * a.group);
 }
 
 // The last token that row r sees.
 __device__ __forceinline__ int last_seen(const AttnWeightsArgs& a, const Sequence& s, int r) {
-    return a.causal ? s.ctx - s.n + r / a.group : s.ctx - 1;
+    return a.causal ? s.ctx - s.n + step_row(a, r) : s.ctx - 1;
 }
 
 // A row at element off, or zeros for off < 0.
@@ -530,7 +537,11 @@ __global__ __launch_bounds__(kThreads) void kept_sum_kernel(AttnWeightsArgs a) {
 // registers, with a streamed one that the four waves share through LDS, double buffered, kTile vectors at
 // a time, laid out as the operands of the products.
 //   stats  stationary: query rows;  streamed: a chunk's keys.    Item: (sequence, chunk, kv head, row group)
-//   sum    stationary: keys;        streamed: the query rows.    Item: (sequence, run of tokens, kv head)
+//   sum    stationary: keys;        streamed: the query rows.    Item: (sequence, run of tokens, kv head, part
+//          of the rows); with several parts (few tokens, many rows) their sums are joined by join_kernel
+// A streamed tile is worked on without a branch: whether any of its scores is hidden is decided once for the
+// wave, since a branch per 16 x 16 scores kept the products of one from running beside the exponentials of
+// another (stats 150 -> 141 us, sum 122 -> 107 us on 2 x 512 rows at 8192 tokens, 32/8 heads of 128).
 template <bool BF16, int STEPS>
 constexpr int many_tiles() { return BF16 || STEPS <= 4 ? 4 : 2; }
 template <bool BF16, int STEPS>
@@ -543,26 +554,31 @@ __global__ __launch_bounds__(kThreads) void many_kernel(AttnWeightsArgs a) {
     constexpr int kLoads = (kSub * STEPS + kWaves - 1) / kWaves;  // operands of a tile, for each wave
     __shared__ Frag<BF16> tile[2][kSub * STEPS][64];
     __shared__ float lse[2][kTile];  // sum: of the streamed rows
-    __shared__ int last[2][kTile];   // sum: the last token each streamed row sees; stats: -1 for a bad block
+    __shared__ int last[2][kTile];   // sum: the last token each streamed row sees; stats: -1 for no token
+    __shared__ int gap[2];           // stats: some token of the tile is not there
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int col = lane & 15, quad = lane >> 4;
     const auto items_of = [&](int ctx, int n) {
         const int rows = n * a.group;
         if (rows <= a.few_rows) return 0;
-        return SUM ? (ctx + kHold - 1) / kHold * a.Hkv
+        return SUM ? (ctx + kHold - 1) / kHold * a.Hkv * a.row_parts
                    : (ctx + a.chunk - 1) / a.chunk * a.Hkv * ((rows + kHold - 1) / kHold);
     };
     Walk walk;
     Sequence s;
     for (int64_t item = blockIdx.x; walk.find(a, SUM, item, items_of, s); item += gridDim.x) {
         const int rows = s.n * a.group, old = s.ctx - s.n;
-        int rest = (int)(item - s.first), row0 = 0, h, chunk = 0, run0 = 0;
+        int rest = (int)(item - s.first), row0 = 0, h, chunk = 0, run0 = 0, part = 0;
         int64_t row = 0;
         if constexpr (SUM) {
+            part = rest % a.row_parts;
+            rest /= a.row_parts;
             h = rest % a.Hkv;
             run0 = ((s.ctx + kHold - 1) / kHold - 1 - rest / a.Hkv) * kHold;
-            row = state_row(a, s.b);
-            if (row < 0) continue;
+            if (a.row_parts == 1) {
+                row = state_row(a, s.b);
+                if (row < 0) continue;
+            }
         } else {
             const int groups = (rows + kHold - 1) / kHold;
             // The last rows see the most tokens: their groups first.
@@ -594,7 +610,9 @@ __global__ __launch_bounds__(kThreads) void many_kernel(AttnWeightsArgs a) {
         int from, to;
         if constexpr (SUM) {
             from = a.causal ? max(0, run0 - old) * a.group / kTile * kTile : 0;
-            to = rows;
+            const int per = ((rows - from + kTile - 1) / kTile + a.row_parts - 1) / a.row_parts * kTile;
+            from += part * per;
+            to = min(rows, from + per);
         } else {
             from = chunk * a.chunk;
             to = min(min(s.ctx, from + a.chunk), last_seen(a, s, min(rows, row0 + kHold) - 1) + 1);
@@ -626,8 +644,8 @@ __global__ __launch_bounds__(kThreads) void many_kernel(AttnWeightsArgs a) {
             if (threadIdx.x < kTile) {
                 const int v = v0 + threadIdx.x;
                 if constexpr (SUM) {
-                    buf_lse = v < rows ? a.lse[query_row(a, s, h, v)] : -kNegInf;
-                    buf_last = v < rows ? last_seen(a, s, v) : -1;
+                    buf_lse = v < to ? a.lse[query_row(a, s, h, v)] : -kNegInf;
+                    buf_last = v < to ? last_seen(a, s, v) : -1;
                 } else {
                     buf_last = v < to && blk_last >= 0 && blk_last < a.num_blocks ? v : -1;
                 }
@@ -649,6 +667,10 @@ __global__ __launch_bounds__(kThreads) void many_kernel(AttnWeightsArgs a) {
             if (threadIdx.x < kTile) {
                 lse[at][threadIdx.x] = buf_lse;
                 last[at][threadIdx.x] = buf_last;
+                if (!SUM) {
+                    const bool any = __ballot(buf_last < 0) != 0;
+                    if (threadIdx.x == 0) gap[at] = any;
+                }
             }
         };
         float m[NT], l[NT];  // stats: running maximum and sum; sum: l is the token's weight
@@ -665,72 +687,80 @@ __global__ __launch_bounds__(kThreads) void many_kernel(AttnWeightsArgs a) {
         }
         __syncthreads();
         const bool mine = hold0 < (SUM ? s.ctx : rows);
-        const int hold_last = hold0 + NT * 16 - 1;  // sum: the wave's last token
-        const int whole = SUM ? 0 : last_seen(a, s, min(hold0, rows - 1));
+        const int whole = SUM ? 0 : last_seen(a, s, min(hold0, rows - 1));  // seen by all of the wave's rows
+        // A streamed tile. EDGE: some of its scores are hidden.
+        const auto work = [&](auto edge, int v0, int at) {
+            constexpr bool EDGE = decltype(edge)::value;
+#pragma unroll
+            for (int sub = 0; sub < kSub; ++sub) {
+                f32x4 c[NT];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) c[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) {
+                    const Frag<BF16> y = tile[at][sub * STEPS + i][lane];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) c[nt] = Frag<BF16>::mma(y, x[nt][i], c[nt]);
+                }
+                float set[4];
+                int see[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (SUM) set[i] = lse[at][sub * 16 + quad * 4 + i];
+                    if (EDGE) see[i] = last[at][sub * 16 + quad * 4 + i];
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float p[4];
+                    if constexpr (SUM) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            p[i] = fast_exp2(c[nt][i] * a.scale_log2 - set[i]);
+                            if (EDGE) p[i] = hold0 + nt * 16 + col > see[i] ? 0.f : p[i];
+                        }
+                        l[nt] += (p[0] + p[1]) + (p[2] + p[3]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            p[i] = c[nt][i] * a.scale_log2;
+                            if (EDGE) {
+                                const bool hidden = (see[i] < 0) | (v0 + sub * 16 + quad * 4 + i > limit[nt]);
+                                p[i] = hidden ? kNegInf : p[i];
+                            }
+                        }
+                        add_scores<4>(m[nt], l[nt], p);
+                    }
+                }
+            }
+        };
         int at = 0;
         for (int v0 = from; v0 < to; v0 += kTile, at ^= 1) {
             const bool more = v0 + kTile < to;
             if (more) fetch(v0 + kTile);
             if (mine) {
-#pragma unroll
-                for (int sub = 0; sub < kSub; ++sub) {
-                    Frag<BF16> y[STEPS];
-#pragma unroll
-                    for (int i = 0; i < STEPS; ++i) y[i] = tile[at][sub * STEPS + i][lane];
-                    const int u0 = v0 + sub * 16;
-                    float set[4];
-                    int see[4];
-                    bool edge;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if constexpr (SUM) set[i] = lse[at][sub * 16 + quad * 4 + i];
-                        see[i] = last[at][sub * 16 + quad * 4 + i];
-                    }
-                    if constexpr (SUM) edge = hold_last > last[at][sub * 16];
-                    else edge = u0 + 15 > whole || u0 + 16 > to || __ballot(see[0] < 0 || see[1] < 0 || see[2] < 0 || see[3] < 0) != 0;
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        f32x4 c = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int i = 0; i < STEPS; ++i) c = Frag<BF16>::mma(y[i], x[nt][i], c);
-                        if constexpr (SUM) {
-                            float p[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) p[i] = fast_exp2(c[i] * a.scale_log2 - set[i]);
-                            if (edge) {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) p[i] = hold0 + nt * 16 + col > see[i] ? 0.f : p[i];
-                            }
-                            l[nt] += (p[0] + p[1]) + (p[2] + p[3]);
-                        } else {
-                            float p[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) p[i] = c[i] * a.scale_log2;
-                            if (edge) {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const bool hidden = (see[i] < 0) | (u0 + quad * 4 + i > limit[nt]);
-                                    p[i] = hidden ? kNegInf : p[i];
-                                }
-                            }
-                            add_scores(m[nt], l[nt], p);
-                        }
-                    }
-                }
+                // sum: the wave's last token against what the tile's first row sees.
+                const bool edge = SUM ? hold0 + NT * 16 - 1 > __builtin_amdgcn_readfirstlane(last[at][0])
+                                      : v0 + kTile - 1 > whole || __builtin_amdgcn_readfirstlane(gap[at]) != 0;
+                if (edge) work(std::true_type{}, v0, at);
+                else work(std::false_type{}, v0, at);
             }
             if (more) stage(at ^ 1);
             __syncthreads();
         }
         if constexpr (SUM) {
             const size_t base = ((size_t)row * a.Hkv + h) * a.max_tokens;
+            float* parts = a.row_sums + (((size_t)part * a.B + s.b) * a.Hkv + h) * a.run_tokens;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const int t = hold0 + nt * 16 + col;
                 float w = l[nt];
                 w += shfl_xor_f(w, 16);
                 w += shfl_xor_f(w, 32);
-                if (quad == 0 && t < s.ctx)
-                    store_weight(a, s, base, t, old_weight(a, s, base, t, s.ctx) + (there[nt] ? w : 0.f));
+                w = there[nt] ? w : 0.f;
+                if (quad == 0 && t < s.ctx) {
+                    if (a.row_parts == 1) store_weight(a, s, base, t, old_weight(a, s, base, t, s.ctx) + w);
+                    else parts[t] = w;
+                }
             }
         } else {
 #pragma unroll
@@ -742,6 +772,25 @@ __global__ __launch_bounds__(kThreads) void many_kernel(AttnWeightsArgs a) {
                     a.part[(size_t)chunk * a.total_q * a.H + query_row(a, s, h, r)] = make_float2(m[nt], l[nt]);
             }
         }
+    }
+}
+
+// Adds up the parts of the many-row sums, in their order. Item: (sequence, run of kThreads tokens, kv head).
+__global__ __launch_bounds__(kThreads) void join_kernel(AttnWeightsArgs a) {
+    const auto items_of = [&](int ctx, int n) {
+        return n * a.group <= a.few_rows ? 0 : (ctx + kThreads - 1) / kThreads * a.Hkv;
+    };
+    Walk walk;
+    Sequence s;
+    for (int64_t item = blockIdx.x; walk.find(a, false, item, items_of, s); item += gridDim.x) {
+        const int rest = (int)(item - s.first), h = rest % a.Hkv, t = rest / a.Hkv * kThreads + threadIdx.x;
+        const int64_t row = state_row(a, s.b);
+        if (row < 0 || t >= s.ctx) continue;
+        const size_t base = ((size_t)row * a.Hkv + h) * a.max_tokens;
+        const float* parts = a.row_sums + ((size_t)s.b * a.Hkv + h) * a.run_tokens + t;
+        float w = 0.f;
+        for (int i = 0; i < a.row_parts; ++i) w += parts[(size_t)i * a.B * a.Hkv * a.run_tokens];
+        store_weight(a, s, base, t, old_weight(a, s, base, t, s.ctx) + w);
     }
 }
 
@@ -796,6 +845,7 @@ void launch_steps(const AttnWeightsArgs& a, hipStream_t stream) {
         many_kernel<BF16, STEPS, FULL, false><<<a.many_stat_grid, kThreads, 0, stream>>>(a);
         merge_kernel<<<(unsigned)(((int64_t)a.total_q * a.H + kThreads - 1) / kThreads), kThreads, 0, stream>>>(a);
         many_kernel<BF16, STEPS, FULL, true><<<a.many_sum_grid, kThreads, 0, stream>>>(a);
+        if (a.row_parts > 1) join_kernel<<<a.many_sum_grid, kThreads, 0, stream>>>(a);
     }
 }
 

@@ -101,9 +101,11 @@ int weights_setup(const kyro_attn_weights_params* p, bool has_q_start, int num_c
     if (a.B == 0 || a.total_q == 0) return KYRO_OK;
     const int64_t rows = (int64_t)std::min(a.max_q_len, a.total_q) * a.group;
     const double block_elems = (double)a.Hkv * a.bs * a.D;
-    if (a.cap > (1 << 30) || rows > (1 << 30) || (int64_t)a.total_q * a.H > INT32_MAX || block_elems > UINT32_MAX)
+    if (a.cap > (1 << 30) || rows > (1 << 30) || rows * a.group > INT32_MAX || (int64_t)a.total_q * a.H > INT32_MAX ||
+        block_elems > UINT32_MAX)
         return fail(KYRO_EUNSUPPORTED, "attn_weights: more tokens or query rows than one launch carries");
     a.block_elems = (uint32_t)block_elems;
+    a.group_magic = a.group > 1 ? (uint32_t)((((uint64_t)1 << 32) + a.group - 1) / a.group) : 0;
     const int most_few = kyro::attn_weights_few_rows(a.bf16, a.D), hold = kyro::attn_weights_many_hold(a.bf16, a.D);
     const bool many = rows > most_few;
     a.few_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : most_few;
@@ -134,8 +136,14 @@ int weights_setup(const kyro_attn_weights_params* p, bool has_q_start, int num_c
     a.few_items_most = many && !mixed ? 0 : a.B * ((a.cap + chunk - 1) / chunk) * a.Hkv;
     a.few_grid = (int)std::min(most, a.few_items_most);
     a.many_stat_grid = many ? (int)std::min(most, items(chunk)) : 0;
-    a.many_sum_grid = many ? (int)std::min(most, a.B * ((a.cap + hold - 1) / hold) * a.Hkv) : 0;
+    // Few runs of tokens for the CUs (short contexts of many rows): the rows are split, into parts of at least
+    // 256, until there are two workgroups a CU.
+    const int64_t runs = a.B * ((a.cap + hold - 1) / hold) * a.Hkv;
+    a.row_parts = many ? (int)std::max<int64_t>(1, std::min<int64_t>((2 * num_cus + runs - 1) / runs, rows / 256)) : 1;
+    a.run_tokens = (a.cap + hold - 1) / hold * hold;
+    a.many_sum_grid = many ? (int)std::min(most, runs * a.row_parts) : 0;
     bytes = align_up(part_bytes(chunk), 256) + (many ? align_up((size_t)a.total_q * a.H * sizeof(float), 256) : 0);
+    if (a.row_parts > 1) bytes += align_up((size_t)a.row_parts * a.B * a.Hkv * a.run_tokens * sizeof(float), 256);
     if (keep) {  // at most 256 MiB of them: items past that are computed again
         const size_t item = (size_t)chunk * a.kept_rows * sizeof(float);
         a.kept_items = std::min<int64_t>(a.few_items_most, (int64_t)(((size_t)256 << 20) / item));
@@ -485,7 +493,8 @@ int kyro_attn_weights(kyro_ctx ctx, const kyro_attn_weights_params* p, const voi
             a.lse = reinterpret_cast<float*>(base);
             base += align_up((size_t)a.total_q * a.H * sizeof(float), 256);
         }
-        a.kept = reinterpret_cast<float*>(base);
+        // A call has either parts of sums or kept scores.
+        a.row_sums = a.kept = reinterpret_cast<float*>(base);
         a.err = ctx->err;
         KYRO_HIP(kyro::launch_attn_weights(a, ctx->stream));
         return KYRO_OK;

@@ -368,12 +368,16 @@ struct AttnWeightsArgs {
     int B, H, Hkv, group, D, bs, bs_shift, max_blocks, num_blocks, total_q, max_q_len, num_state_rows, max_tokens;
     int causal, bf16;
     uint32_t block_elems;       // Hkv * bs * D
+    uint32_t group_magic;       // 2^32 / group, rounded up (group > 1)
     int64_t cap;                // tokens a sequence may have: the least of the table's and the state's
     float scale_log2;
     int chunk;                  // tokens of a chunk of the statistics pass, a multiple of 64
     int few_rows;               // sequences of up to as many rows a kv head go to the few-row kernels (16, 32, 64)
     int kept_rows;              // rows of a kept token's scores, a multiple of 4
     int few_grid, many_stat_grid, many_sum_grid;  // workgroups; 0: not launched
+    int row_parts;              // parts that the rows of a many-row sum are split in
+    int64_t run_tokens;         // entries of a kv head in row_sums
+    float* row_sums;            // [row_parts, B, Hkv, run_tokens]: the parts' sums, where there are several
     int64_t few_items_most;     // work items of the few-row kernels where every context is as long as it may be
     int64_t kept_items;         // items whose scores have room; 0: scores are not kept
 };
