@@ -15,8 +15,6 @@ budget move into the slots of the ones that go, so caches, block tables and cont
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
@@ -69,6 +67,58 @@ class CacheEviction:
     def accumulate_async(self, query, key_cache, block_table, context_lens, weights, positions, *, q_start_loc=None,
                          max_q_len=None, row_positions=None, state_rows=None, causal=True, scale=None, out=None):
         """Queues the work on torch's current stream and returns the weights; see :meth:`accumulate`."""
+        # One expression for a call whose tensors are as they should be; _accumulate_require names what is not.
+        hkv, bs, h, d = self.num_kv_heads, self.block_size, self.num_heads, self.head_dim
+        if out is None:
+            out = weights
+        try:
+            idx, dtype = query.get_device(), query.dtype
+            total_q = query.shape[0]
+            B, width = block_table.shape
+            cache, state = key_cache.shape, weights.shape
+            nb = cache[0]
+            plain = (idx >= 0 and dtype in _DTYPES and query.shape == (total_q, h, d) and query.is_contiguous()
+                     and key_cache.dtype == dtype and cache == (nb, hkv, bs, d) and key_cache.is_contiguous()
+                     and key_cache.get_device() == idx and len(state) == 3 and state[1] == hkv
+                     and weights.dtype == torch.float32 and out.dtype == torch.float32 and positions.dtype == torch.int32
+                     and out.shape == state and positions.shape == state and weights.is_contiguous()
+                     and out.is_contiguous() and positions.is_contiguous() and weights.get_device() == idx
+                     and out.get_device() == idx and positions.get_device() == idx
+                     and block_table.dtype == torch.int64 and block_table.is_contiguous()
+                     and block_table.get_device() == idx and context_lens.dtype == torch.int64
+                     and context_lens.shape == (B,) and context_lens.is_contiguous() and context_lens.get_device() == idx
+                     and (total_q == B if q_start_loc is None else
+                          max_q_len is not None and q_start_loc.dtype == torch.int32 and q_start_loc.shape == (B + 1,)
+                          and q_start_loc.is_contiguous() and q_start_loc.get_device() == idx)
+                     and (state[0] >= B if state_rows is None else
+                          state_rows.dtype == torch.int32 and state_rows.shape == (B,) and state_rows.is_contiguous()
+                          and state_rows.get_device() == idx)
+                     and (row_positions is None or (
+                         row_positions.dtype == torch.int64 and row_positions.shape == (total_q,)
+                         and row_positions.is_contiguous() and row_positions.get_device() == idx)))
+        except (AttributeError, ValueError, IndexError):  # not a tensor, or not of the right rank
+            plain = False
+        if not plain:
+            max_q_len = self._accumulate_require(query, key_cache, block_table, context_lens, weights, positions, out,
+                                                 q_start_loc, max_q_len, row_positions, state_rows)
+            idx, dtype, total_q = query.get_device(), query.dtype, query.shape[0]
+            (B, width), state, nb = block_table.shape, weights.shape, key_cache.shape[0]
+        params = _lib.pack_attn_weights(bs, h, d, hkv, B, total_q, width, nb, _DTYPES[dtype], 1 if causal else 0,
+                                        scale or 0.0, 1 if q_start_loc is None else max_q_len, state[0], state[2])
+        ctx = _lib.context(idx)
+        ctx.set_stream(_lib.current_stream(idx))
+        _lib.check(_lib.lib().kyro_attn_weights(
+            ctx.handle, params, query.data_ptr(), None if q_start_loc is None else q_start_loc.data_ptr(),
+            None if row_positions is None else row_positions.data_ptr(), key_cache.data_ptr(), block_table.data_ptr(),
+            context_lens.data_ptr(), None if state_rows is None else state_rows.data_ptr(), weights.data_ptr(),
+            out.data_ptr(), positions.data_ptr()))
+        return out
+
+    def _accumulate_require(self, query, key_cache, block_table, context_lens, weights, positions, out, q_start_loc,
+                            max_q_len, row_positions, state_rows):
+        """Raises what is wrong with accumulate's tensors; the most rows of a sequence where nothing is."""
+        if not isinstance(query, torch.Tensor):
+            raise TypeError("query must be a torch.Tensor")
         dev = query.device
         if dev.type != "cuda":
             raise ValueError("accumulate runs on a GPU device; got " + str(dev))
@@ -79,37 +129,22 @@ class CacheEviction:
             raise ValueError(f"query shape {tuple(query.shape)} does not match (*, {self.num_heads}, {self.head_dim})")
         self._state(weights, "weights", torch.float32, dev)
         self._state(positions, "positions", torch.int32, dev, weights)
-        if out is None:
-            out = weights
-        else:
-            self._state(out, "out", torch.float32, dev, weights)
+        self._state(out, "out", torch.float32, dev, weights)
         B = self._batch(block_table, context_lens, state_rows, weights, dev)
-        if q_start_loc is not None:
-            _require(q_start_loc, "q_start_loc", (torch.int32,), 1, dev)
-            if q_start_loc.shape[0] != B + 1:
-                raise ValueError("q_start_loc must have batch+1 entries")
-            if max_q_len is None:
-                max_q_len = int((q_start_loc[1:] - q_start_loc[:-1]).max().item()) if B else 1
-        else:
-            if total_q != B:
-                raise ValueError("query rows must equal the batch size without q_start_loc")
-            max_q_len = 1
         if row_positions is not None:
             _require(row_positions, "row_positions", (torch.int64,), 1, dev)
             if row_positions.shape[0] != total_q:
                 raise ValueError("row_positions must have one entry per row")
-        params = _lib.AttnWeightsParams(
-            self.block_size, h, d, self.num_kv_heads, B, total_q, block_table.shape[1], key_cache.shape[0],
-            _DTYPES[query.dtype], 1 if causal else 0, float(scale) if scale else 0.0, int(max_q_len), weights.shape[0],
-            weights.shape[2])
-        ctx = _lib.context(dev.index or 0)
-        ctx.set_stream(_lib.current_stream(dev.index or 0))
-        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-        _lib.check(_lib.lib().kyro_attn_weights(
-            ctx.handle, ctypes.byref(params), query.data_ptr(), ptr(q_start_loc), ptr(row_positions),
-            key_cache.data_ptr(), block_table.data_ptr(), context_lens.data_ptr(), ptr(state_rows),
-            weights.data_ptr(), out.data_ptr(), positions.data_ptr()))
-        return out
+        if q_start_loc is None:
+            if total_q != B:
+                raise ValueError("query rows must equal the batch size without q_start_loc")
+            return 1
+        _require(q_start_loc, "q_start_loc", (torch.int32,), 1, dev)
+        if q_start_loc.shape[0] != B + 1:
+            raise ValueError("q_start_loc must have batch+1 entries")
+        if max_q_len is None:
+            max_q_len = int((q_start_loc[1:] - q_start_loc[:-1]).max().item()) if B else 1
+        return int(max_q_len)
 
     def accumulate(self, query, key_cache, block_table, context_lens, weights, positions, *, q_start_loc=None,
                    max_q_len=None, row_positions=None, state_rows=None, causal=True, scale=None, out=None):
@@ -129,6 +164,52 @@ class CacheEviction:
     def evict_async(self, key_cache, value_cache, block_table, context_lens, weights, positions, *, budget, sink=4,
                     recent=0, state_rows=None, out=None):
         """Queues the work on torch's current stream and returns the new context lengths; see :meth:`evict`."""
+        # One expression for a call whose tensors are as they should be; _evict_require names what is not.
+        hkv, bs, d = self.num_kv_heads, self.block_size, self.head_dim
+        out_weights, out_positions = (weights, positions) if out is None else out
+        try:
+            idx, dtype = key_cache.get_device(), key_cache.dtype
+            B, width = block_table.shape
+            cache, state = key_cache.shape, weights.shape
+            nb = cache[0]
+            plain = (idx >= 0 and dtype in _DTYPES and cache == (nb, hkv, bs, d) and key_cache.is_contiguous()
+                     and value_cache.shape == cache and value_cache.dtype == dtype and value_cache.is_contiguous()
+                     and value_cache.get_device() == idx and len(state) == 3 and state[1] == hkv
+                     and weights.dtype == torch.float32 and out_weights.dtype == torch.float32
+                     and positions.dtype == torch.int32 and out_positions.dtype == torch.int32
+                     and out_weights.shape == state and positions.shape == state and out_positions.shape == state
+                     and weights.is_contiguous() and out_weights.is_contiguous() and positions.is_contiguous()
+                     and out_positions.is_contiguous() and weights.get_device() == idx
+                     and out_weights.get_device() == idx and positions.get_device() == idx
+                     and out_positions.get_device() == idx and block_table.dtype == torch.int64
+                     and block_table.is_contiguous() and block_table.get_device() == idx
+                     and context_lens.dtype == torch.int64 and context_lens.shape == (B,)
+                     and context_lens.is_contiguous() and context_lens.get_device() == idx
+                     and (state[0] >= B if state_rows is None else
+                          state_rows.dtype == torch.int32 and state_rows.shape == (B,) and state_rows.is_contiguous()
+                          and state_rows.get_device() == idx))
+        except (AttributeError, ValueError, IndexError):  # not a tensor, or not of the right rank
+            plain = False
+        if not plain:
+            self._evict_require(key_cache, value_cache, block_table, context_lens, weights, positions, out_weights,
+                                out_positions, state_rows)
+            idx, dtype, nb = key_cache.get_device(), key_cache.dtype, key_cache.shape[0]
+            (B, width), state = block_table.shape, weights.shape
+        lens = torch.empty_like(context_lens)
+        params = _lib.pack_kv_evict(bs, hkv, d, B, width, nb, _DTYPES[dtype], budget, sink, recent, state[0], state[2])
+        ctx = _lib.context(idx)
+        ctx.set_stream(_lib.current_stream(idx))
+        _lib.check(_lib.lib().kyro_kv_evict(
+            ctx.handle, params, key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
+            context_lens.data_ptr(), None if state_rows is None else state_rows.data_ptr(), weights.data_ptr(),
+            positions.data_ptr(), out_weights.data_ptr(), out_positions.data_ptr(), lens.data_ptr()))
+        return lens
+
+    def _evict_require(self, key_cache, value_cache, block_table, context_lens, weights, positions, out_weights,
+                       out_positions, state_rows):
+        """Raises what is wrong with evict's tensors."""
+        if not isinstance(key_cache, torch.Tensor):
+            raise TypeError("key_cache must be a torch.Tensor")
         dev = key_cache.device
         if dev.type != "cuda":
             raise ValueError("evict runs on a GPU device; got " + str(dev))
@@ -138,22 +219,9 @@ class CacheEviction:
             raise ValueError("key_cache and value_cache shapes differ")
         self._state(weights, "weights", torch.float32, dev)
         self._state(positions, "positions", torch.int32, dev, weights)
-        out_weights, out_positions = (weights, positions) if out is None else out
-        if out is not None:
-            self._state(out_weights, "out[0]", torch.float32, dev, weights)
-            self._state(out_positions, "out[1]", torch.int32, dev, weights)
-        B = self._batch(block_table, context_lens, state_rows, weights, dev)
-        lens = torch.empty_like(context_lens)
-        params = _lib.KvEvictParams(
-            self.block_size, self.num_kv_heads, self.head_dim, B, block_table.shape[1], key_cache.shape[0],
-            _DTYPES[key_cache.dtype], int(budget), int(sink), int(recent), weights.shape[0], weights.shape[2])
-        ctx = _lib.context(dev.index or 0)
-        ctx.set_stream(_lib.current_stream(dev.index or 0))
-        _lib.check(_lib.lib().kyro_kv_evict(
-            ctx.handle, ctypes.byref(params), key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
-            context_lens.data_ptr(), state_rows.data_ptr() if state_rows is not None else None, weights.data_ptr(),
-            positions.data_ptr(), out_weights.data_ptr(), out_positions.data_ptr(), lens.data_ptr()))
-        return lens
+        self._state(out_weights, "out[0]", torch.float32, dev, weights)
+        self._state(out_positions, "out[1]", torch.int32, dev, weights)
+        self._batch(block_table, context_lens, state_rows, weights, dev)
 
     def evict(self, key_cache, value_cache, block_table, context_lens, weights, positions, *, budget, sink=4, recent=0,
               state_rows=None, out=None):

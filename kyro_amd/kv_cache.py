@@ -66,7 +66,7 @@ def _rows(t, name, dtype, shape, device):
     st = t.stride()
     if (d > 1 and st[2] != 1) or (h > 1 and st[1] != d):
         raise ValueError(f"{name}'s heads must be dense: strides (any, {d}, 1), got {st}")
-    return st[0] if n > 1 else h * d  # torch gives a single row any stride
+    return st[0]
 
 
 class PagedKVCache:
@@ -126,6 +126,86 @@ class PagedKVCache:
                          sin=None, positions=None, q_weight=None, k_weight=None, norm_eps=None, weight_offset=0.0,
                          interleaved=False, q_start_loc=None, out=None):
         """Queues the pass on torch's current stream and returns the query; see :meth:`append_qkv`."""
+        # One expression for a call whose tensors are as they should be; _qkv_require names what is not.
+        hkv, bs, d = self.num_kv_heads, self.block_size, self.head_dim
+        try:
+            idx, src, dst = query.get_device(), query.dtype, key_cache.dtype
+            total_q, heads, _ = query.shape
+            B, width = block_table.shape
+            kv, cache, rows = key.shape, key_cache.shape, total_q
+            (q_stride, qh, q1), (k_stride, kh, k1), (v_stride, vh, v1) = query.stride(), key.stride(), value.stride()
+            nb = cache[0]
+            plain = (idx >= 0 and src in _DTYPES and dst in _DTYPES and key.dtype == src and value.dtype == src
+                     and query.shape[2] == d and kv == (rows, hkv, d) and value.shape == kv and rows > 0
+                     and q1 == 1 and k1 == 1 and v1 == 1 and qh == d and kh == d and vh == d
+                     and key.get_device() == idx and value.get_device() == idx
+                     and cache == (nb, hkv, bs, d) and value_cache.shape == cache and value_cache.dtype == dst
+                     and key_cache.is_contiguous() and value_cache.is_contiguous()
+                     and key_cache.get_device() == idx and value_cache.get_device() == idx
+                     and block_table.dtype == torch.int64 and block_table.is_contiguous()
+                     and block_table.get_device() == idx and context_lens.dtype == torch.int64
+                     and context_lens.shape == (B,) and context_lens.is_contiguous() and context_lens.get_device() == idx
+                     and (rows == B if q_start_loc is None else
+                          q_start_loc.dtype == torch.int32 and q_start_loc.shape == (B + 1,)
+                          and q_start_loc.is_contiguous() and q_start_loc.get_device() == idx)
+                     and (positions is None or (positions.dtype == torch.int64 and positions.shape == (rows,)
+                                                and positions.is_contiguous() and positions.get_device() == idx)))
+        except (AttributeError, ValueError, IndexError):  # not a tensor, or not of the right rank
+            plain = False
+        if not plain:
+            q_stride, k_stride, v_stride = self._qkv_require(query, key, value, key_cache, value_cache, block_table,
+                                                             context_lens, q_start_loc, positions)
+            idx, src, dst = query.get_device(), query.dtype, key_cache.dtype
+            (total_q, heads, _), (B, width), nb = query.shape, block_table.shape, key_cache.shape[0]
+        if total_q == 1:  # torch gives a single row any stride
+            q_stride = k_stride = v_stride = 0
+        dev = query.device
+        rotary = max_position = 0
+        if (cos is None) != (sin is None):
+            raise ValueError("cos and sin come together")
+        if cos is not None:
+            _require(cos, "cos", (torch.float32,), 2, dev)
+            _require(sin, "sin", (torch.float32,), 2, dev)
+            if cos.shape != sin.shape:
+                raise ValueError("cos and sin must have the same shape")
+            max_position, rotary = cos.shape
+            rotary *= 2
+        weight_dtype = src
+        if (q_weight is None) != (k_weight is None):
+            raise ValueError("q_weight and k_weight come together")
+        if q_weight is not None:
+            if norm_eps is None:
+                raise ValueError("norm weights need norm_eps")
+            weight_dtype = q_weight.dtype
+            _require(q_weight, "q_weight", (torch.float32, torch.bfloat16), 1, dev)
+            _require(k_weight, "k_weight", (weight_dtype,), 1, dev)
+            if q_weight.shape[0] != d or k_weight.shape[0] != d:
+                raise ValueError(f"norm weights must have {d} entries")
+        if out is None:
+            out = torch.empty((total_q, heads, d), dtype=dst, device=dev)
+        else:
+            _require(out, "out", (dst,), 3, dev)
+            if out.shape != query.shape:
+                raise ValueError("out has the wrong shape")
+        params = _lib.pack_qkv_append(bs, heads, hkv, d, B, total_q, width, nb, _DTYPES[src], _DTYPES[dst], rotary,
+                                      1 if interleaved else 0, max_position, 0 if norm_eps is None else 1,
+                                      _DTYPES[weight_dtype], 0.0 if norm_eps is None else norm_eps, weight_offset,
+                                      q_stride, k_stride, v_stride)
+        ctx = _lib.context(idx)
+        ctx.set_stream(_lib.current_stream(idx))
+        _lib.check(_lib.lib().kyro_qkv_append(
+            ctx.handle, params, query.data_ptr(), key.data_ptr(), value.data_ptr(),
+            None if q_start_loc is None else q_start_loc.data_ptr(), None if positions is None else positions.data_ptr(),
+            block_table.data_ptr(), context_lens.data_ptr(), None if cos is None else cos.data_ptr(),
+            None if sin is None else sin.data_ptr(), None if q_weight is None else q_weight.data_ptr(),
+            None if k_weight is None else k_weight.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+            out.data_ptr()))
+        return out
+
+    def _qkv_require(self, query, key, value, key_cache, value_cache, block_table, context_lens, q_start_loc, positions):
+        """Raises what is wrong with append_qkv's tensors; (query, key, value) row strides where nothing is."""
+        if not isinstance(query, torch.Tensor):
+            raise TypeError("query must be a torch.Tensor")
         dev = query.device
         if dev.type != "cuda":
             raise ValueError("append_qkv runs on a GPU device; got " + str(dev))
@@ -137,16 +217,15 @@ class PagedKVCache:
         hkv, bs = self.num_kv_heads, self.block_size
         if d != self.head_dim:
             raise ValueError(f"query heads have {d} elements, expected {self.head_dim}")
-        q_stride = _rows(query, "query", src, (total_q, heads, d), dev)
-        k_stride = _rows(key, "key", src, (total_q, hkv, d), dev)
-        v_stride = _rows(value, "value", src, (total_q, hkv, d), dev)
+        strides = (_rows(query, "query", src, (total_q, heads, d), dev), _rows(key, "key", src, (total_q, hkv, d), dev),
+                   _rows(value, "value", src, (total_q, hkv, d), dev))
         _require(key_cache, "key_cache", (torch.float32, torch.bfloat16), 4, dev)
         _require(value_cache, "value_cache", (key_cache.dtype,), 4, dev)
         _require(block_table, "block_table", (torch.int64,), 2, dev)
         _require(context_lens, "context_lens", (torch.int64,), 1, dev)
-        nb = key_cache.shape[0]
-        if key_cache.shape != (nb, hkv, bs, d) or value_cache.shape != (nb, hkv, bs, d):
-            raise ValueError(f"caches must be {(nb, hkv, bs, d)}")
+        want = (key_cache.shape[0], hkv, bs, d)
+        if tuple(key_cache.shape) != want or tuple(value_cache.shape) != want:
+            raise ValueError(f"caches must be {want}")
         B = context_lens.shape[0]
         if block_table.shape[0] != B:
             raise ValueError("block_table and context_lens disagree on the batch size")
@@ -160,45 +239,7 @@ class PagedKVCache:
             _require(positions, "positions", (torch.int64,), 1, dev)
             if positions.shape[0] != total_q:
                 raise ValueError("positions must have one entry per row")
-        rotary = max_position = 0
-        if (cos is None) != (sin is None):
-            raise ValueError("cos and sin come together")
-        if cos is not None:
-            _require(cos, "cos", (torch.float32,), 2, dev)
-            _require(sin, "sin", (torch.float32,), 2, dev)
-            if cos.shape != sin.shape:
-                raise ValueError("cos and sin must have the same shape")
-            max_position, rotary = cos.shape[0], 2 * cos.shape[1]
-        weight_dtype = src
-        if (q_weight is None) != (k_weight is None):
-            raise ValueError("q_weight and k_weight come together")
-        if q_weight is not None:
-            if norm_eps is None:
-                raise ValueError("norm weights need norm_eps")
-            weight_dtype = q_weight.dtype
-            _require(q_weight, "q_weight", (torch.float32, torch.bfloat16), 1, dev)
-            _require(k_weight, "k_weight", (weight_dtype,), 1, dev)
-            if q_weight.shape[0] != d or k_weight.shape[0] != d:
-                raise ValueError(f"norm weights must have {d} entries")
-        if out is None:
-            out = torch.empty((total_q, heads, d), dtype=key_cache.dtype, device=dev)
-        else:
-            _require(out, "out", (key_cache.dtype,), 3, dev)
-            if out.shape != query.shape:
-                raise ValueError("out has the wrong shape")
-        params = _lib.QkvAppendParams(bs, heads, hkv, d, B, total_q, block_table.shape[1], nb, _DTYPES[src],
-                                      _DTYPES[key_cache.dtype], rotary, 1 if interleaved else 0, max_position,
-                                      0 if norm_eps is None else 1, _DTYPES[weight_dtype],
-                                      0.0 if norm_eps is None else float(norm_eps), float(weight_offset), q_stride,
-                                      k_stride, v_stride)
-        ctx = _lib.context(dev.index or 0)
-        ctx.set_stream(_lib.current_stream(dev.index or 0))
-        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-        _lib.check(_lib.lib().kyro_qkv_append(
-            ctx.handle, ctypes.byref(params), query.data_ptr(), key.data_ptr(), value.data_ptr(), ptr(q_start_loc),
-            ptr(positions), block_table.data_ptr(), context_lens.data_ptr(), ptr(cos), ptr(sin), ptr(q_weight),
-            ptr(k_weight), key_cache.data_ptr(), value_cache.data_ptr(), out.data_ptr()))
-        return out
+        return strides
 
     def append_qkv(self, query, key, value, key_cache, value_cache, block_table, context_lens, *, cos=None, sin=None,
                    positions=None, q_weight=None, k_weight=None, norm_eps=None, weight_offset=0.0, interleaved=False,
