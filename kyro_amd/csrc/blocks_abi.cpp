@@ -178,10 +178,14 @@ int evict_setup(const kyro_kv_evict_params* p, kyro::EvictArgs& a, size_t& bytes
     a.sink = p->sink;
     a.recent = p->recent;
     a.max_moves = (int)std::max<int64_t>(0, std::min<int64_t>(a.budget, a.cap - a.budget));
-    a.lds_keys = (int)std::min<int64_t>(a.cap, kyro::kEvictLdsKeys);
-    // About 4096 workgroups in all for the copies, each with at least 1024 vectors where the most tokens move.
+    // A selecting workgroup copies what it moves (64 sequences of 8 heads, 256 moves of 512 bytes: 43 us; 16 + 32 in
+    // two kernels), except where few of them would copy much each (64 of them, 900 moves: 42 us, 21 + 11 in two):
+    // then about 4096 workgroups share the moves, each with at least 1024 vectors where the most tokens move.
     const int64_t units = std::max<int64_t>(1, (int64_t)a.B * a.Hkv);
-    a.move_wgs = (int)std::max<int64_t>(1, std::min<int64_t>((4096 + units - 1) / units, ((int64_t)a.max_moves * a.row_vecs + 1023) / 1024));
+    const bool own = units >= 128 || (int64_t)a.max_moves * a.row_vecs <= 8192;
+    a.own_moves = own ? kyro::kEvictOwnMoves : 0;
+    const int64_t left = std::max<int64_t>(0, (int64_t)a.max_moves - a.own_moves) * a.row_vecs;
+    a.move_wgs = (int)std::max<int64_t>(1, std::min<int64_t>((4096 + units - 1) / units, (left + 1023) / 1024));
     bytes = align_up((size_t)a.B * a.Hkv * sizeof(int), 256) +
             align_up((size_t)a.B * a.Hkv * 2 * a.max_moves * sizeof(int32_t), 256);
     return KYRO_OK;

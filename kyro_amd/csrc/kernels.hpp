@@ -390,7 +390,7 @@ hipError_t launch_attn_weights(const AttnWeightsArgs& a, hipStream_t stream);
 void launch_attn_weights_f32(const AttnWeightsArgs& a, hipStream_t stream);
 
 // Eviction by accumulated weight.
-constexpr int kEvictLdsKeys = 12288;  // keys the selection keeps in LDS (48 KiB: two workgroups a CU)
+constexpr int kEvictOwnMoves = 1024;  // moves that a selecting workgroup may make itself
 struct EvictArgs {
     uint4* kc;
     uint4* vc;
@@ -407,7 +407,8 @@ struct EvictArgs {
     int* err;
     int64_t cap;
     int B, Hkv, bs, max_blocks, num_blocks, num_state_rows, max_tokens, row_vecs;
-    int budget, sink, recent, max_moves, lds_keys, move_wgs;
+    int budget, sink, recent, max_moves;
+    int own_moves, move_wgs;    // moves that a selecting workgroup makes itself; workgroups for the list's others
 };
 
 hipError_t launch_kv_evict(const EvictArgs& a, hipStream_t stream);

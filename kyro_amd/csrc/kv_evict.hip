@@ -8,11 +8,13 @@
 // no order among themselves and what is moved is only what has to be: a budget of 2048 with 256 tokens over
 // it moves at most 256 of them, where closing the gaps in order would move most of 2048.
 //
-// evict_select_kernel: one workgroup a (sequence, kv head). Selection reads 8 bytes a token once; the keys
-// stay in LDS (up to kLdsKeys of them) for the three passes over 11, 11 and 10 bits. The first digit holds
-// the sign, the exponent and two bits of the mantissa, so weights that fall over many octaves spread over
-// its bins. Lists of holes and movers go to scratch. evict_move_kernel: copies K and V rows, 16 bytes a lane.
-// What bounds the pair: latency of the passes for few tokens, HBM for many.
+// evict_select_kernel: one workgroup a (sequence, kv head). Weights and positions are read once, 8 bytes a
+// token, and the keys stay in registers, thread i holding slots i, i + 1024, .., for the three passes over
+// 11, 11 and 10 bits. The first digit holds the sign, the exponent and two bits of the mantissa, so weights
+// that fall over many octaves spread over its bins. Ballots give each token its rank in slot order; the
+// workgroup then copies its own K and V rows, up to kOwnMoves of them. evict_move_kernel: the rest, by
+// many workgroups, where a call may have that many. Contexts past the registers read their keys again.
+// What bounds it: latency (a dozen barriers, some five dependent loads) for few tokens, HBM for many moves.
 #include "common.hpp"
 #include "kernels.hpp"
 
@@ -21,217 +23,349 @@ namespace {
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / 64;
-constexpr int kBins = 2048;
+constexpr int kBins = 2 * kSelThreads;
 constexpr int kMoveThreads = 256;
+constexpr int kMaxHeld = 64;   // keys a thread holds at most
+constexpr int kOwnMoves = kEvictOwnMoves;
 
 // Order-preserving bits: a < b as floats <=> rank(a) < rank(b); -0 ranks as +0, NaN as -infinity.
 __device__ __forceinline__ uint32_t rank_bits(float w) {
     uint32_t u = __float_as_uint(w);
-    if ((u & 0x7fffffffu) > 0x7f800000u) u = 0xff800000u;
-    if (u == 0x80000000u) u = 0;
+    u = (u & 0x7fffffffu) > 0x7f800000u ? 0xff800000u : u;
+    u = u == 0x80000000u ? 0u : u;
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-// Maximum over the workgroup; every thread gets it. red: one int per wave.
+struct Shared {
+    int hist[kBins];
+    int red[kSelWaves];
+    int red2[kSelWaves];
+    int found[2];
+    int bad;
+    // Tokens of one kind in each group of 64 slots, then how many there are before it.
+    int count[2][kMaxHeld * kSelWaves];
+    int hole[kOwnMoves], mover[kOwnMoves];  // the first of each list
+    int4 move[kOwnMoves];                   // (block, slot) to, (block, slot) from
+};
+
+// Maximum over the workgroup; every thread gets it.
 __device__ __forceinline__ int block_max(int v, int* red) {
     for (int m = 32; m; m >>= 1) v = max(v, __shfl_xor(v, m, 64));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     v = red[0];
+#pragma unroll
     for (int i = 1; i < kSelWaves; ++i) v = max(v, red[i]);
-    __syncthreads();
     return v;
 }
 
-// Is the sequence to be worked on? Latches what is wrong with it. Uniform over the workgroup.
-__device__ bool evict_valid(const EvictArgs& a, int b, int64_t n, int64_t* row, int* bad_any) {
+// Exclusive sum over the workgroup's threads; *total gets the whole. red: of its own for each call in a row.
+__device__ __forceinline__ int block_scan(int v, int* red, int* total) {
+    const int incl = wave_incl_scan_i(v), wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 63) red[wave] = incl;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < kSelWaves; ++i) {
+        const int x = red[i];
+        before += i < wave ? x : 0;
+        all += x;
+    }
+    *total = all;
+    return before + incl - v;
+}
+
+// Notes what is wrong with the sequence's block ids (n of its tokens are known to fit); read behind a barrier.
+__device__ __forceinline__ void check_blocks(const EvictArgs& a, int b, int n, Shared& sh) {
     int bad = 0;
-    *row = b;
-    if (a.state_rows) {
-        const int r = a.state_rows[b];
-        *row = r;
-        if (r < 0 || r >= a.num_state_rows) bad = ERR_STATE_ROW;
-        for (int i = threadIdx.x; i < a.B; i += blockDim.x)
-            if (i != b && a.state_rows[i] == r) bad = ERR_STATE_ROW;
+    for (int i = threadIdx.x; i < (n + a.bs - 1) / a.bs; i += kSelThreads) {
+        const int64_t id = a.table[(size_t)b * a.max_blocks + i];
+        if (id < 0 || id >= a.num_blocks) bad = ERR_BLOCK_ID;
     }
-    if (n < 0 || n > a.cap) {
-        bad |= ERR_CTX_LEN;
-    } else {
-        const int64_t blocks = (n + a.bs - 1) / a.bs;
-        for (int64_t i = threadIdx.x; i < blocks; i += blockDim.x) {
-            const int64_t id = a.table[(size_t)b * a.max_blocks + i];
-            if (id < 0 || id >= a.num_blocks) bad |= ERR_BLOCK_ID;
-        }
-    }
-    if (bad) atomicOr(bad_any, bad);  // LDS
-    __syncthreads();
-    const int all = *bad_any;
-    if (all && threadIdx.x == 0) latch_error(a.err, all);
-    return all == 0;
+    if (bad) atomicOr(&sh.bad, bad);
 }
 
-// The bin that holds the `want`-th largest of the histogram (want >= 1), and how many are in the bins
-// above it. One wave scans; every thread gets the answer through out[2].
-__device__ __forceinline__ void find_bin(const int* hist, int want, int* out) {
-    if (threadIdx.x < 64) {
-        const int lane = threadIdx.x;
-        constexpr int per = kBins / 64;
-        // Lane 0 holds the largest bins.
-        int mine = 0;
-        for (int i = 0; i < per; ++i) mine += hist[kBins - 1 - lane * per - i];
-        const int incl = wave_incl_scan_i(mine);
-        const unsigned long long reach = __ballot(incl >= want);
-        const int first = __ffsll((unsigned long long)reach) - 1;
-        if (lane == first) {
-            int above = incl - mine, bin = kBins - 1 - lane * per;
-            while (above + hist[bin] < want) above += hist[bin--];
-            out[0] = bin;
-            out[1] = above;
-        }
-    }
-    __syncthreads();
+// One (sequence, kv head)'s arrays.
+struct Unit {
+    const float* w;
+    const int32_t* pos;
+    float* ow;
+    int32_t* op;
+    int n, budget, sink, from;  // positions above `from` are protected
+    int32_t* holes;  // the lists' entries from own_moves on
+    int32_t* movers;
+    __device__ __forceinline__ void protect(int newest, int recent) { from = (int)max((int64_t)newest - recent, (int64_t)INT32_MIN); }
+    __device__ __forceinline__ uint32_t key(int p, float x) const { return ((p < sink) | (p > from)) ? 0xffffffffu : rank_bits(x); }
+};
+
+// Entry i of a list: the first ones in LDS, those that the other kernel reads in memory.
+__device__ __forceinline__ void list(const EvictArgs& a, int* first, int32_t* rest, int i, int t) {
+    if (i < kOwnMoves) first[i] = t;
+    if (i >= a.own_moves) rest[i] = t;
 }
 
-__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
-    extern __shared__ uint32_t lds_keys[];  // a.lds_keys entries
-    __shared__ int hist[kBins];
-    __shared__ int red[3 * kSelWaves];
-    __shared__ int found[2];
-    __shared__ int bad_any;
-    const int b = blockIdx.x / a.Hkv, h = blockIdx.x % a.Hkv;
+// Marks the kept tokens and lists holes and movers; R keys a thread (R = 0: any number, read again). Returns
+// the number of moves, or -1 (before anything is written) for a sequence with a bad block.
+template <int R>
+__device__ __forceinline__ int select(const EvictArgs& a, int b, Unit u, Shared& sh) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t n64 = a.ctx_lens[b];
-    if (tid == 0) bad_any = 0;
-    __syncthreads();
-    int64_t row;
-    const bool ok = evict_valid(a, b, n64, &row, &bad_any);
-    if (tid == 0) {
-        a.num_moves[blockIdx.x] = 0;
-        if (h == 0) a.out_ctx_lens[b] = ok && n64 > a.budget ? a.budget : n64;
-    }
-    if (!ok) return;
-    const int n = (int)n64, budget = a.budget;
-    const size_t base = ((size_t)row * a.Hkv + h) * a.max_tokens;
-    const float* w = a.weights + base;
-    const int32_t* pos = a.positions + base;
-    float* ow = a.out_weights + base;
-    int32_t* op = a.out_positions + base;
-    const bool copy = ow != w, copy_pos = op != pos;
-    if (n <= budget) {
-        for (int t = tid; t < n; t += kSelThreads) {
-            if (copy) ow[t] = w[t];
-            if (copy_pos) op[t] = pos[t];
-        }
-        return;
-    }
-
+    constexpr int kHeld = R ? R : 1;
+    uint32_t key[kHeld];
+    const int rounds = R ? R : (u.n + kSelThreads - 1) / kSelThreads;
     int newest = INT32_MIN;
-    for (int t = tid; t < n; t += kSelThreads) newest = max(newest, pos[t]);
-    newest = block_max(newest, red);
-    const int64_t from = (int64_t)newest - a.recent;  // positions above it are protected
-    const bool in_lds = n <= a.lds_keys;
-    const auto key_of = [&](int t) -> uint32_t {
-        const int p = pos[t];
-        return p < a.sink || (int64_t)p > from ? 0xffffffffu : rank_bits(w[t]);
+    if constexpr (R > 0 && R <= 16) {
+        int p[kHeld];
+        float x[kHeld];
+#pragma unroll
+        for (int r = 0; r < kHeld; ++r) {
+            const int t = r * kSelThreads + tid;
+            p[r] = t < u.n ? u.pos[t] : INT32_MIN;
+            x[r] = t < u.n ? u.w[t] : 0.f;
+        }
+        check_blocks(a, b, u.n, sh);  // while they are under way
+#pragma unroll
+        for (int r = 0; r < kHeld; ++r) newest = max(newest, p[r]);
+        newest = block_max(newest, sh.red);
+        u.protect(newest, a.recent);
+#pragma unroll
+        for (int r = 0; r < kHeld; ++r) key[r] = u.key(p[r], x[r]);
+    } else {
+        check_blocks(a, b, u.n, sh);
+#pragma unroll 8
+        for (int r = 0; r < rounds; ++r) {
+            const int t = r * kSelThreads + tid;
+            newest = max(newest, t < u.n ? u.pos[t] : INT32_MIN);
+        }
+        newest = block_max(newest, sh.red);
+        u.protect(newest, a.recent);
+        if constexpr (R > 0) {  // positions again, from L2: held beside the keys they would not fit
+#pragma unroll
+            for (int r = 0; r < kHeld; ++r) {
+                const int t = min(r * kSelThreads + tid, u.n - 1);
+                key[r] = u.key(u.pos[t], u.w[t]);
+            }
+        }
+    }
+    if (sh.bad) return -1;  // block_max had a barrier
+    const auto key_at = [&](int r) -> uint32_t {
+        if constexpr (R > 0) return key[r];
+        const int t = r * kSelThreads + tid;
+        return t < u.n ? u.key(u.pos[t], u.w[t]) : 0u;
     };
 
     // The budget-th largest key, digit by digit from the top; `want` counts within the keys that share the
-    // digits found so far.
-    uint32_t prefix = 0;
-    int want = budget;
+    // digits found so far. Thread i owns the bins 2 i and 2 i + 1 from the largest down, and leaves them empty.
+    uint32_t T = 0;
+    int want = u.budget;
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, above = pass == 0 ? 32 : pass == 1 ? 21 : 10;
         const uint32_t mask = pass == 2 ? 1023u : 2047u;
-        for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
-        __syncthreads();
-        for (int t = tid; t < n; t += kSelThreads) {
-            uint32_t k;
-            if (pass == 0 || !in_lds) {
-                k = key_of(t);
-                if (in_lds) lds_keys[t] = k;
-            } else {
-                k = lds_keys[t];
-            }
-            const bool same = pass == 0 || (k >> (pass == 1 ? 21 : 10)) == prefix;
-            if (same) atomicAdd(&hist[(k >> shift) & mask], 1);
+        const auto count = [&](uint32_t k, int t) {
+            if (t < u.n && (pass == 0 || (k >> above) == T)) atomicAdd(&sh.hist[(k >> shift) & mask], 1);
+        };
+        if constexpr (R > 0) {
+#pragma unroll
+            for (int r = 0; r < kHeld; ++r) count(key[r], r * kSelThreads + tid);
+        } else {
+            for (int r = 0; r < rounds; ++r) count(key_at(r), r * kSelThreads + tid);
         }
         __syncthreads();
-        find_bin(hist, want, found);
-        prefix = (prefix << (pass == 2 ? 10 : 11)) | (uint32_t)found[0];
-        want -= found[1];
+        const int hi = kBins - 1 - 2 * tid;
+        const int c0 = sh.hist[hi], c1 = sh.hist[hi - 1];
+        sh.hist[hi] = sh.hist[hi - 1] = 0;
+        int total;
+        const int before = block_scan(c0 + c1, pass == 1 ? sh.red2 : sh.red, &total);
+        if (before < want && want <= before + c0 + c1) {
+            const bool first = want <= before + c0;
+            sh.found[0] = first ? hi : hi - 1;
+            sh.found[1] = first ? before : before + c0;
+        }
         __syncthreads();
+        T = (T << (pass == 2 ? 10 : 11)) | (uint32_t)sh.found[0];
+        want -= sh.found[1];
     }
-    const uint32_t T = prefix;  // `want` of the keys equal to T stay, those of the lowest slots
+    // `want` of the keys equal to T stay, those of the lowest slots.
 
-    // Slot order from here on: wave i owns slots [i seg, (i + 1) seg). Equal keys before each wave's first.
-    const int seg = ((n + kSelThreads - 1) / kSelThreads) * 64;
-    const int t0 = min(n, wave * seg), t1 = min(n, t0 + seg);
-    int eq = 0;
-    for (int t = t0; t < t1; t += 64) {
-        const int at = t + lane;
-        const uint32_t k = at < t1 ? (in_lds ? lds_keys[at] : key_of(at)) : 0u;
-        eq += __popcll(__ballot(at < t1 && k == T));
-    }
-    if (lane == 0) red[wave] = eq;
-    __syncthreads();
-    int eq_before = 0;
-    for (int i = 0; i < wave; ++i) eq_before += red[i];
-    // Twice over the wave's slots: holes and movers counted, then listed behind those of the waves before.
     const unsigned long long below = lane == 0 ? 0ull : (~0ull >> (64 - lane));
-    int holes = 0, movers = 0, hole_at = 0, mover_at = 0;
-    int32_t* hole_list = a.moves + (size_t)blockIdx.x * 2 * a.max_moves;
-    int32_t* mover_list = hole_list + a.max_moves;
-#pragma unroll 1
-    for (int pass = 0; pass < 2; ++pass) {
-        int seen = eq_before;
-        for (int t = t0; t < t1; t += 64) {
-            const int at = t + lane;
-            const bool in = at < t1;
-            const uint32_t k = in ? (in_lds ? lds_keys[at] : key_of(at)) : 0u;
-            const unsigned long long ties = __ballot(in && k == T);
-            const bool keep = in && (k > T || (k == T && seen + __popcll(ties & below) < want));
-            seen += __popcll(ties);
-            const unsigned long long hb = __ballot(in && !keep && at < budget), mb = __ballot(keep && at >= budget);
-            if (pass == 0) {
-                holes += __popcll(hb);
-                movers += __popcll(mb);
-            } else {
-                if (in && !keep && at < budget) hole_list[hole_at + __popcll(hb & below)] = at;
-                if (keep && at >= budget) mover_list[mover_at + __popcll(mb & below)] = at;
-                hole_at += __popcll(hb);
-                mover_at += __popcll(mb);
-                if (keep && at < budget) {
-                    if (copy) ow[at] = w[at];
-                    if (copy_pos) op[at] = pos[at];
-                }
-            }
+    // Turns the counts of `rounds` x kSelWaves groups, in slot order, into how many come before each.
+    const auto scan_counts = [&](int* count, int* red) -> int {
+        int carry = 0;
+        if constexpr (R > 0) {  // at most kSelThreads groups
+            const int groups = kHeld * kSelWaves;
+            const int v = tid < groups ? count[tid] : 0;
+            int total;
+            const int before = block_scan(v, red, &total);
+            if (tid < groups) count[tid] = before;
+            carry = total;
         }
-        if (pass == 0) {
-            __syncthreads();  // red's tie counts have been read
+        __syncthreads();
+        return carry;
+    };
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int r = 0; r < kHeld; ++r) {
+            const bool in = r * kSelThreads + tid < u.n;
+            const int c = __popcll(__ballot(in && key[r] == T));
+            if (lane == 0) sh.count[0][r * kSelWaves + wave] = c;
+        }
+        __syncthreads();
+        scan_counts(sh.count[0], sh.red2);
+        unsigned long long kept = 0;  // bit r: this thread's r-th token stays
+#pragma unroll
+        for (int r = 0; r < kHeld; ++r) {
+            const int t = r * kSelThreads + tid;
+            const bool in = t < u.n;
+            const unsigned long long ties = __ballot(in && key[r] == T);
+            const int rank = sh.count[0][r * kSelWaves + wave] + __popcll(ties & below);
+            const bool keep = in && (key[r] > T || (key[r] == T && rank < want));
+            kept |= (unsigned long long)keep << r;
+        }
+        __syncthreads();  // the ties' ranks have been read
+#pragma unroll
+        for (int r = 0; r < kHeld; ++r) {
+            const int t = r * kSelThreads + tid;
+            const bool keep = (kept >> r) & 1;
+            const int holes = __popcll(__ballot(!keep && t < u.budget)), movers = __popcll(__ballot(keep && t >= u.budget));
             if (lane == 0) {
-                red[kSelWaves + wave] = holes;
-                red[2 * kSelWaves + wave] = movers;
-            }
-            __syncthreads();
-            for (int i = 0; i < wave; ++i) {
-                hole_at += red[kSelWaves + i];
-                mover_at += red[2 * kSelWaves + i];
+                sh.count[0][r * kSelWaves + wave] = holes;
+                sh.count[1][r * kSelWaves + wave] = movers;
             }
         }
+        __syncthreads();
+        const int moves = scan_counts(sh.count[0], sh.red);
+        scan_counts(sh.count[1], sh.red2);
+#pragma unroll
+        for (int r = 0; r < kHeld; ++r) {
+            const int t = r * kSelThreads + tid;
+            const bool keep = (kept >> r) & 1, hole = !keep && t < u.budget, mover = keep && t >= u.budget;
+            const unsigned long long hb = __ballot(hole), mb = __ballot(mover);
+            if (hole) list(a, sh.hole, u.holes, sh.count[0][r * kSelWaves + wave] + __popcll(hb & below), t);
+            if (mover) list(a, sh.mover, u.movers, sh.count[1][r * kSelWaves + wave] + __popcll(mb & below), t);
+            if (keep && !mover) {
+                if (u.ow != u.w) u.ow[t] = u.w[t];
+                if (u.op != u.pos) u.op[t] = u.pos[t];
+            }
+        }
+        return moves;
+    } else {
+        // Round by round, each with its own ranks: ties before, holes before, movers before.
+        int ties_before = 0, holes_before = 0, movers_before = 0;
+        for (int r = 0; r < rounds; ++r) {
+            const int t = r * kSelThreads + tid;
+            const bool in = t < u.n;
+            const uint32_t k = key_at(r);
+            int total;
+            __syncthreads();  // the round before has read its sums
+            const int rank = ties_before + block_scan(in && k == T, sh.red, &total);
+            ties_before += total;
+            const bool keep = in && (k > T || (k == T && rank < want));
+            const bool hole = in && !keep && t < u.budget, mover = keep && t >= u.budget;
+            const int at = block_scan(hole | (mover << 16), sh.red2, &total);
+            if (hole) list(a, sh.hole, u.holes, holes_before + (at & 0xffff), t);
+            if (mover) list(a, sh.mover, u.movers, movers_before + (at >> 16), t);
+            holes_before += total & 0xffff;
+            movers_before += total >> 16;
+            if (keep && !mover) {
+                if (u.ow != u.w) u.ow[t] = u.w[t];
+                if (u.op != u.pos) u.op[t] = u.pos[t];
+            }
+        }
+        return holes_before;
     }
-    __syncthreads();  // the lists are whole
-    int total = 0;
-    for (int i = 0; i < kSelWaves; ++i) total += red[kSelWaves + i];
-    for (int i = tid; i < total; i += kSelThreads) {
-        const int to = hole_list[i], src = mover_list[i];
-        ow[to] = w[src];
-        op[to] = pos[src];
-    }
-    if (tid == 0) a.num_moves[blockIdx.x] = total;
 }
 
-// K and V rows of the listed moves; a.move_wgs neighbouring workgroups share one (sequence, kv head)'s list.
+// HELD: most keys a thread holds (4, 16, 64), which sets the kernel's registers; with 4, two workgroups share
+// a CU (64 x 2304 tokens of 8 heads: 50 us with one, 43 with two).
+template <int HELD>
+__global__ __launch_bounds__(kSelThreads, HELD == 4 ? 8 : 4) void evict_select_kernel(EvictArgs a) {
+    __shared__ Shared sh;
+    const int b = blockIdx.x / a.Hkv, h = blockIdx.x % a.Hkv;
+    const int tid = threadIdx.x;
+    const int64_t n64 = a.ctx_lens[b];
+    const int64_t row = a.state_rows ? a.state_rows[b] : b;
+    if (tid == 0) sh.bad = 0;
+    for (int i = tid; i < kBins; i += kSelThreads) sh.hist[i] = 0;
+    if (tid == 0) {
+        a.num_moves[blockIdx.x] = 0;
+        if (h == 0) a.out_ctx_lens[b] = n64 > a.budget && n64 <= a.cap ? a.budget : n64;
+    }
+    int bad = n64 < 0 || n64 > a.cap ? ERR_CTX_LEN : 0;
+    if (a.state_rows) {
+        bad |= row < 0 || row >= a.num_state_rows ? ERR_STATE_ROW : 0;
+        int twice = 0;
+        for (int i = tid; i < a.B; i += kSelThreads)
+            if (i != b && a.state_rows[i] == row) twice = 1;
+        if (__syncthreads_or(twice)) bad |= ERR_STATE_ROW;
+    }
+    if (bad) {
+        if (tid == 0) {
+            latch_error(a.err, bad);
+            if (h == 0) a.out_ctx_lens[b] = n64;
+        }
+        return;
+    }
+    const size_t base = ((size_t)row * a.Hkv + h) * a.max_tokens;
+    Unit u = {a.weights + base, a.positions + base, a.out_weights + base, a.out_positions + base, (int)n64, a.budget, a.sink, 0,
+              a.moves + (size_t)blockIdx.x * 2 * a.max_moves, a.moves + ((size_t)blockIdx.x * 2 + 1) * a.max_moves};
+    if (u.n <= u.budget) {
+        for (int t = tid; t < u.n; t += kSelThreads) {
+            if (u.ow != u.w) u.ow[t] = u.w[t];
+            if (u.op != u.pos) u.op[t] = u.pos[t];
+        }
+        return;
+    }
+    __syncthreads();
+    const int rounds = (u.n + kSelThreads - 1) / kSelThreads;
+    int moves;
+    if (rounds <= 1) moves = select<1>(a, b, u, sh);
+    else if (rounds <= 4) moves = select<4>(a, b, u, sh);
+    else if (HELD >= 16 && rounds <= 16) moves = select<HELD >= 16 ? 16 : 1>(a, b, u, sh);
+    else if (HELD >= 64 && rounds <= 32) moves = select<HELD >= 64 ? 32 : 1>(a, b, u, sh);
+    else if (HELD >= 64 && rounds <= 64) moves = select<HELD >= 64 ? 64 : 1>(a, b, u, sh);
+    else moves = select<0>(a, b, u, sh);
+    if (moves < 0) {
+        if (tid == 0) {
+            latch_error(a.err, sh.bad);
+            if (h == 0) a.out_ctx_lens[b] = n64;
+        }
+        return;
+    }
+    __syncthreads();  // the lists are whole
+    const int64_t* table = a.table + (size_t)b * a.max_blocks;
+    const int own = min(moves, a.own_moves);
+    for (int i = tid; i < moves; i += kSelThreads) {
+        const int to = i < kOwnMoves ? sh.hole[i] : u.holes[i], src = i < kOwnMoves ? sh.mover[i] : u.movers[i];
+        if (i < own) {
+            const int p = to / a.bs, q = src / a.bs;
+            sh.move[i] = make_int4((int)table[p], to - p * a.bs, (int)table[q], src - q * a.bs);
+        }
+        const float x = u.w[src];
+        const int p = u.pos[src];
+        u.ow[to] = x;
+        u.op[to] = p;
+    }
+    __syncthreads();
+    const int vecs = own * a.row_vecs;
+    const size_t head = (size_t)h * a.bs;
+    for (int v = tid; v < vecs; v += kSelThreads) {
+        const int i = v / a.row_vecs, part = v - i * a.row_vecs;
+        const int4 m = sh.move[i];
+        const size_t dst = ((size_t)m.x * a.Hkv * a.bs + head + m.y) * a.row_vecs + part;
+        const size_t from = ((size_t)m.z * a.Hkv * a.bs + head + m.w) * a.row_vecs + part;
+        const uint4 k = a.kc[from], x = a.vc[from];
+        a.kc[dst] = k;
+        a.vc[dst] = x;
+    }
+    if (tid == 0) a.num_moves[blockIdx.x] = moves;
+}
+
+// K and V rows of the moves that the selection has left; a.move_wgs neighbouring workgroups share one
+// (sequence, kv head)'s list.
+__device__ __forceinline__ size_t row_of(const EvictArgs& a, const int64_t* table, int h, int t) {
+    const int page = t / a.bs;
+    return (((size_t)table[page] * a.Hkv + h) * a.bs + (t - page * a.bs)) * a.row_vecs;
+}
 __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
     const int unit = blockIdx.x / a.move_wgs, part_wg = blockIdx.x % a.move_wgs, b = unit / a.Hkv, h = unit % a.Hkv;
     const int moves = a.num_moves[unit];
@@ -239,14 +373,13 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
     const int32_t* mover_list = hole_list + a.max_moves;
     const int64_t* table = a.table + (size_t)b * a.max_blocks;
     const int64_t work = (int64_t)moves * a.row_vecs;
-    for (int64_t v = (int64_t)part_wg * kMoveThreads + threadIdx.x; v < work; v += (int64_t)a.move_wgs * kMoveThreads) {
-        const int i = (int)(v / a.row_vecs), part = (int)(v % a.row_vecs);
-        const int to = hole_list[i], src = mover_list[i];
-        const size_t dst = (((size_t)table[to / a.bs] * a.Hkv + h) * a.bs + to % a.bs) * a.row_vecs + part;
-        const size_t from = (((size_t)table[src / a.bs] * a.Hkv + h) * a.bs + src % a.bs) * a.row_vecs + part;
-        const uint4 k = a.kc[from], x = a.vc[from];
-        a.kc[dst] = k;
-        a.vc[dst] = x;
+    for (int64_t v = (int64_t)a.own_moves * a.row_vecs + (int64_t)part_wg * kMoveThreads + threadIdx.x; v < work;
+         v += (int64_t)a.move_wgs * kMoveThreads) {
+        const int i = (int)(v / a.row_vecs), part = (int)(v - (int64_t)i * a.row_vecs);
+        const size_t to = row_of(a, table, h, hole_list[i]) + part, src = row_of(a, table, h, mover_list[i]) + part;
+        const uint4 k = a.kc[src], x = a.vc[src];
+        a.kc[to] = k;
+        a.vc[to] = x;
     }
 }
 
@@ -254,14 +387,12 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
 
 hipError_t launch_kv_evict(const EvictArgs& a, hipStream_t stream) {
     if (a.B == 0) return hipSuccess;
-    const size_t lds = (size_t)a.lds_keys * sizeof(uint32_t);
-    evict_select_kernel<<<a.B * a.Hkv, kSelThreads, lds, stream>>>(a);
-    if (hipError_t e = hipGetLastError()) return e;
-    if (a.max_moves > 0) {
-        evict_move_kernel<<<a.B * a.Hkv * a.move_wgs, kMoveThreads, 0, stream>>>(a);
-        return hipGetLastError();
-    }
-    return hipSuccess;
+    const int units = a.B * a.Hkv;
+    if (a.cap <= 4 * kSelThreads) evict_select_kernel<4><<<units, kSelThreads, 0, stream>>>(a);
+    else if (a.cap <= 16 * kSelThreads) evict_select_kernel<16><<<units, kSelThreads, 0, stream>>>(a);
+    else evict_select_kernel<64><<<units, kSelThreads, 0, stream>>>(a);
+    if (a.max_moves > a.own_moves) evict_move_kernel<<<units * a.move_wgs, kMoveThreads, 0, stream>>>(a);
+    return hipGetLastError();
 }
 
 }  // namespace kyro
