@@ -340,6 +340,7 @@ struct QkvAppendArgs {
     int rotary, interleaved, max_position, norm, weight_bf16;
     int src_bf16, dst_bf16;
     float eps, weight_offset;
+    float inv_dim;           // 1 / D
     // Set by qkv_append_setup: elements of a lane's chunk, units of two paired chunks (rotated in
     // halves), log2 of the lanes of a head row, waves of a packed row.
     int chunk, pairs, lp_shift, waves_per_row;

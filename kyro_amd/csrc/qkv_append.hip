@@ -69,20 +69,13 @@ struct Chunk {
     }
 };
 
-// Round to nearest even with the canonical NaN 0x7FC0, as the plain append stores.
-__device__ __forceinline__ uint32_t bf16_bits(float f) {
-    const uint32_t u = __float_as_uint(f);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return 0x7fc0u;
-    return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
-}
-
 template <bool BF16, int E>
 __device__ __forceinline__ void store_chunk(void* base, size_t off, const float* f) {
     if constexpr (BF16) {
         uint16_t* p = reinterpret_cast<uint16_t*>(base) + off;
         uint32_t w[E / 2];
 #pragma unroll
-        for (int i = 0; i < E / 2; ++i) w[i] = bf16_bits(f[2 * i]) | (bf16_bits(f[2 * i + 1]) << 16);
+        for (int i = 0; i < E / 2; ++i) w[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
         if constexpr (E == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
         else if constexpr (E == 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
         else *reinterpret_cast<uint32_t*>(p) = w[0];
@@ -102,21 +95,16 @@ __device__ __forceinline__ void store_chunk(void* base, size_t off, const float*
 template <int E>
 __device__ __forceinline__ void load_weights(const void* w, int bf16, float offset, int d, float* out) {
     if (bf16) {
-        const uint16_t* p = reinterpret_cast<const uint16_t*>(w) + d;
+        Chunk<true, E> c;
+        c.load(w, d);
+        c.widen();
 #pragma unroll
-        for (int i = 0; i < E; i += 2) {
-            const uint32_t u = *reinterpret_cast<const uint32_t*>(p + i);
-            out[i] = bf16_lo(u) + offset;
-            out[i + 1] = bf16_hi(u) + offset;
-        }
+        for (int i = 0; i < E; ++i) out[i] = c.f[i] + offset;
     } else {
-        const float* p = reinterpret_cast<const float*>(w) + d;
+        Chunk<false, E> c;
+        c.load(w, d);
 #pragma unroll
-        for (int i = 0; i < E; i += 2) {
-            const float2 u = *reinterpret_cast<const float2*>(p + i);
-            out[i] = u.x + offset;
-            out[i + 1] = u.y + offset;
-        }
+        for (int i = 0; i < E; ++i) out[i] = c.f[i] + offset;
     }
 }
 
@@ -138,17 +126,16 @@ __device__ __forceinline__ int find_sequence(const int32_t* start, int B, int r)
 template <bool SRC_BF16, bool DST_BF16, int E>
 __global__ __launch_bounds__(kThreads) void qkv_append_kernel(QkvAppendArgs a) {
     const int lane = threadIdx.x & 63;
-    const int64_t wave =
-        __builtin_amdgcn_readfirstlane((int)(blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6)));
+    const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6)));
     if (wave == 0 && a.q_start) {  // one wave looks the whole layout over
         for (int i = lane; i <= a.B; i += 64) {
             const int s = a.q_start[i];
             if (s < 0 || s > a.total_q || (i < a.B && a.q_start[i + 1] < s)) latch_error(a.err, ERR_Q_LAYOUT);
         }
     }
-    const int r = (int)(wave / a.waves_per_row);
+    const int r = wave / a.waves_per_row;
     if (r >= a.total_q) return;
-    const int head = (int)(wave % a.waves_per_row) * (64 >> a.lp_shift) + (lane >> a.lp_shift);
+    const int head = (wave - r * a.waves_per_row) * (64 >> a.lp_shift) + (lane >> a.lp_shift);
     const int unit = lane & ((1 << a.lp_shift) - 1);
     const int D = a.D;
     // The lane's two chunks (element offsets): unit i < pairs holds i and i + R / 2, the others two
@@ -187,9 +174,10 @@ __global__ __launch_bounds__(kThreads) void qkv_append_kernel(QkvAppendArgs a) {
         if (lane == 0) latch_error(a.err, ERR_CTX_LEN);
         return;
     }
-    const int64_t slot = ctx - (r1 - r0) + (r - r0);
+    const int slot = (int)(ctx - (r1 - r0) + (r - r0));  // below max_blocks * bs, which fits
+    const int page = slot / a.bs;
     const int64_t pos = a.positions ? a.positions[r] : slot;
-    const int64_t blk = a.table[(size_t)b * a.max_blocks + (size_t)(slot / a.bs)];
+    const int64_t blk = a.table[(size_t)b * a.max_blocks + page];
     const bool bad_pos = a.rotary > 0 && (pos < 0 || pos >= a.max_position);
     const bool bad_blk = blk < 0 || blk >= a.num_blocks;
     if (bad_pos || bad_blk) {
@@ -206,8 +194,7 @@ __global__ __launch_bounds__(kThreads) void qkv_append_kernel(QkvAppendArgs a) {
         for (int i = 0; i < E; ++i) ss += x0.f[i] * x0.f[i] + x1.f[i] * x1.f[i];
         for (int m = 1; m < (1 << a.lp_shift); m <<= 1) ss += shfl_xor_f(ss, m);
         if (qk) {
-            // An IEEE square root and division: one of each for 2 E elements.
-            const float rstd = 1.f / sqrtf(ss / (float)D + a.eps);
+            const float rstd = __builtin_amdgcn_rsqf(ss * a.inv_dim + a.eps);
             float w0[E], w1[E];
 #pragma unroll
             for (int i = 0; i < E; ++i) w0[i] = w1[i] = 1.f;
@@ -259,7 +246,7 @@ __global__ __launch_bounds__(kThreads) void qkv_append_kernel(QkvAppendArgs a) {
     if (!mine) return;
     void* dst = is_q ? a.out_query : is_k ? a.kc : a.vc;
     const size_t to = is_q ? ((size_t)r * a.H + h) * D
-                           : (((size_t)blk * a.Hkv + h) * a.bs + (size_t)(slot % a.bs)) * D;
+                           : (((size_t)blk * a.Hkv + h) * a.bs + (size_t)(slot - page * a.bs)) * D;
     if constexpr (SRC_BF16 && DST_BF16) {
         if (!qk) {
 #pragma unroll

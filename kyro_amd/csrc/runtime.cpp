@@ -1158,6 +1158,8 @@ int kyro_qkv_append(kyro_ctx ctx, const kyro_qkv_append_params* p, const void* q
         if (p->block_size <= 0 || p->num_heads <= 0 || p->num_kv_heads <= 0 || p->head_dim <= 0 || p->batch_size < 0 ||
             p->total_q < 0 || p->max_blocks_per_seq <= 0 || p->num_blocks <= 0)
             return fail(KYRO_EINVAL, "qkv_append: sizes must be positive (batch_size, total_q >= 0)");
+        if ((int64_t)p->max_blocks_per_seq * p->block_size > INT32_MAX)
+            return fail(KYRO_EUNSUPPORTED, "qkv_append: a sequence of more than 2^31 slots");
         if (p->num_heads % p->num_kv_heads != 0)
             return fail(KYRO_EINVAL, "qkv_append: num_heads %d is not a multiple of num_kv_heads %d", p->num_heads,
                         p->num_kv_heads);
@@ -1238,6 +1240,7 @@ int kyro_qkv_append(kyro_ctx ctx, const kyro_qkv_append_params* p, const void* q
         a.dst_bf16 = p->cache_dtype == KYRO_BF16;
         a.eps = p->eps;
         a.weight_offset = p->weight_offset;
+        a.inv_dim = 1.f / (float)p->head_dim;
         if (!kyro::qkv_append_setup(a))
             return fail(KYRO_EUNSUPPORTED, "qkv_append: total_q x heads, or head_dim %d with rotary_dim %d, is more than one launch carries",
                         p->head_dim, p->rotary_dim);
