@@ -38,11 +38,17 @@ struct Frag<true> {
     bf16x8 x;
     template <bool FULL>
     __device__ __forceinline__ void load(const void* base, size_t row, int i, bool last, int D, int lane) {
-        const int at = last && i % 2 == 0 ? 32 * i + 8 * (lane >> 4) : 64 * (i / 2) + 16 * (lane >> 4) + 8 * (i % 2);
+        const int at = piece(i, last, 0, lane);
         const uint16_t* p = reinterpret_cast<const uint16_t*>(base) + row;
         uint4 u = *reinterpret_cast<const uint4*>(p + (FULL || at < D ? at : 0));
         if (!FULL && at >= D) u = make_uint4(0, 0, 0, 0);
         x = __builtin_bit_cast(bf16x8, u);
+    }
+    __device__ __forceinline__ void get(const uint4 (&p)[1][64], int lane) { x = __builtin_bit_cast(bf16x8, p[0][lane]); }
+    __device__ __forceinline__ void put(uint4 (&p)[1][64], int lane) const { p[0][lane] = __builtin_bit_cast(uint4, x); }
+    // Element of the row that piece p of part i starts with.
+    static __device__ __forceinline__ int piece(int i, bool last, int, int lane) {
+        return last && i % 2 == 0 ? 32 * i + 8 * (lane >> 4) : 64 * (i / 2) + 16 * (lane >> 4) + 8 * (i % 2);
     }
     __device__ __forceinline__ void zero() { x = __builtin_bit_cast(bf16x8, make_uint4(0, 0, 0, 0)); }
     static __device__ __forceinline__ f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
@@ -57,11 +63,20 @@ struct Frag<false> {
         const float* p = reinterpret_cast<const float*>(base) + row;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int at = 32 * part + 8 * (lane >> 4) + 4 * i;
+            const int at = piece(part, false, i, lane);
             x[i] = *reinterpret_cast<const f32x4*>(p + (FULL || at < D ? at : 0));
             if (!FULL && at >= D) x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
     }
+    __device__ __forceinline__ void get(const uint4 (&p)[2][64], int lane) {
+        x[0] = __builtin_bit_cast(f32x4, p[0][lane]);
+        x[1] = __builtin_bit_cast(f32x4, p[1][lane]);
+    }
+    __device__ __forceinline__ void put(uint4 (&p)[2][64], int lane) const {
+        p[0][lane] = __builtin_bit_cast(uint4, x[0]);
+        p[1][lane] = __builtin_bit_cast(uint4, x[1]);
+    }
+    static __device__ __forceinline__ int piece(int i, bool, int p, int lane) { return 32 * i + 8 * (lane >> 4) + 4 * p; }
     __device__ __forceinline__ void zero() { x[0] = x[1] = f32x4{0.f, 0.f, 0.f, 0.f}; }
     static __device__ __forceinline__ f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
 #pragma unroll
@@ -200,6 +215,20 @@ __device__ __forceinline__ void add_scores(float& m, float& l, const float (&x)[
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) sum += fast_exp2(x[i] - ref);
+    l = l * fast_exp2(m - ref) + sum;
+    m = top;
+}
+
+// The same for N products that are scores once scaled (scale >= 0).
+template <int N>
+__device__ __forceinline__ void add_products(float& m, float& l, const float (&x)[N], float scale) {
+    float most = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) most = fmaxf(most, x[i]);
+    const float top = fmaxf(m, most * scale), ref = top == kNegInf ? 0.f : top;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum += fast_exp2(x[i] * scale - ref);
     l = l * fast_exp2(m - ref) + sum;
     m = top;
 }
@@ -539,9 +568,18 @@ __global__ __launch_bounds__(kThreads) void kept_sum_kernel(AttnWeightsArgs a) {
 //   stats  stationary: query rows;  streamed: a chunk's keys.    Item: (sequence, chunk, kv head, row group)
 //   sum    stationary: keys;        streamed: the query rows.    Item: (sequence, run of tokens, kv head, part
 //          of the rows); with several parts (few tokens, many rows) their sums are joined by join_kernel
-// A streamed tile is worked on without a branch: whether any of its scores is hidden is decided once for the
-// wave, since a branch per 16 x 16 scores kept the products of one from running beside the exponentials of
-// another (stats 150 -> 141 us, sum 122 -> 107 us on 2 x 512 rows at 8192 tokens, 32/8 heads of 128).
+// Whether any score of a streamed tile is hidden is decided once for the wave, and the tile is worked on
+// without a branch: a branch per 16 x 16 scores kept their products and exponentials apart. On 2 x 512 rows at
+// 8192 tokens, 32/8 heads of 128 (2 x 69 GFLOP), stats take 127 us and sum 101 us, 540 and 680 TFLOP/s where a
+// large library product reaches 1245. With a quarter of the products sum takes 79 us, without the exponentials
+// 90 us, without both 62 us: what is left is the tiles' way through LDS and the barriers.
+template <bool BF16, int FRAGS, int N>
+struct Staged {
+    uint4 x[FRAGS][BF16 ? 1 : 2][64];  // operand f's 16-byte pieces, one a lane
+    float lse[N];  // sum: of the streamed rows
+    int last[N];   // sum: the last token each streamed row sees; stats: -1 for no token
+    int gap;       // stats: some token of the tile is not there
+};
 template <bool BF16, int STEPS>
 constexpr int many_tiles() { return BF16 || STEPS <= 4 ? 4 : 2; }
 template <bool BF16, int STEPS>
@@ -552,10 +590,8 @@ __global__ __launch_bounds__(kThreads) void many_kernel(AttnWeightsArgs a) {
     constexpr int NT = many_tiles<BF16, STEPS>(), kTile = many_streamed<BF16, STEPS>();
     constexpr int kSub = kTile / 16, kHold = kWaves * NT * 16;
     constexpr int kLoads = (kSub * STEPS + kWaves - 1) / kWaves;  // operands of a tile, for each wave
-    __shared__ Frag<BF16> tile[2][kSub * STEPS][64];
-    __shared__ float lse[2][kTile];  // sum: of the streamed rows
-    __shared__ int last[2][kTile];   // sum: the last token each streamed row sees; stats: -1 for no token
-    __shared__ int gap[2];           // stats: some token of the tile is not there
+    // Two arrays, not one of two: what is loaded into one is then known not to touch the other.
+    __shared__ Staged<BF16, kSub * STEPS, kTile> tile0, tile1;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int col = lane & 15, quad = lane >> 4;
     const auto items_of = [&](int ctx, int n) {
@@ -617,11 +653,14 @@ __global__ __launch_bounds__(kThreads) void many_kernel(AttnWeightsArgs a) {
             from = chunk * a.chunk;
             to = min(min(s.ctx, from + a.chunk), last_seen(a, s, min(rows, row0 + kHold) - 1) + 1);
         }
-        Frag<BF16> buf[kLoads];
+        // A tile's vectors: whole rows straight into LDS (FULL), where they land while the tile before is worked on,
+        // others by way of the registers, which put zeros behind their last element. Vectors that are not there
+        // repeat element 0 or the last row: their scores are hidden.
+        constexpr int kHeld = FULL ? 1 : kLoads;
+        Frag<BF16> buf[kHeld];
         float buf_lse = 0.f;
         int buf_last = 0;
         int64_t blk[kLoads], blk_last = 0;  // stats: the block ids of the tile to be fetched next
-        // A tile's vectors on their way into the registers, and from there into LDS.
         const auto ids = [&](int v0) {
             if constexpr (!SUM) {
 #pragma unroll
@@ -633,13 +672,13 @@ __global__ __launch_bounds__(kThreads) void many_kernel(AttnWeightsArgs a) {
                 if (threadIdx.x < kTile) blk_last = v < to ? block_of(a, s.b, v) : 0;
             }
         };
-        const auto fetch = [&](int v0) {
+        const auto fetch = [&](Staged<BF16, kSub * STEPS, kTile>& into, int v0) {
             int64_t off[kLoads];
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
                 const int v = v0 + (i * kWaves + wave) / STEPS * 16 + col;
-                off[i] = -1;
-                if (v < to) off[i] = SUM ? (int64_t)query_row(a, s, h, v) * a.D : key_offset(a, blk[i], h, v);
+                if constexpr (SUM) off[i] = (int64_t)query_row(a, s, h, min(v, to - 1)) * a.D;
+                else off[i] = v < to ? max((int64_t)0, key_offset(a, blk[i], h, v)) : 0;
             }
             if (threadIdx.x < kTile) {
                 const int v = v0 + threadIdx.x;
@@ -651,27 +690,44 @@ __global__ __launch_bounds__(kThreads) void many_kernel(AttnWeightsArgs a) {
                 }
             }
             ids(v0 + kTile);
+            constexpr int kSize = BF16 ? 2 : 4;
+            const char* base = reinterpret_cast<const char*>(SUM ? a.q : a.k);
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
                 const int f = i * kWaves + wave;
-                if (off[i] >= 0 && f < kSub * STEPS) buf[i].template load<FULL>(SUM ? a.q : a.k, (size_t)off[i], f % STEPS, f % STEPS == STEPS - 1, a.D, lane);
-                else buf[i].zero();
-            }
-        };
-        const auto stage = [&](int at) {
+                if (kSub * STEPS % kWaves != 0 && f >= kSub * STEPS) break;
+                if constexpr (FULL) {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const int f = i * kWaves + wave;
-                if (kSub * STEPS % kWaves == 0 || f < kSub * STEPS) tile[at][f][lane] = buf[i];
-            }
-            if (threadIdx.x < kTile) {
-                lse[at][threadIdx.x] = buf_lse;
-                last[at][threadIdx.x] = buf_last;
-                if (!SUM) {
-                    const bool any = __ballot(buf_last < 0) != 0;
-                    if (threadIdx.x == 0) gap[at] = any;
+                    for (int p = 0; p < (BF16 ? 1 : 2); ++p) {
+                        const size_t at = (size_t)off[i] + Frag<BF16>::piece(f % STEPS, f % STEPS == STEPS - 1, p, lane);
+                        __builtin_amdgcn_global_load_lds(
+                            (const __attribute__((address_space(1))) void*)(base + at * kSize),
+                            (__attribute__((address_space(3))) void*)&into.x[f][p][0], 16, 0, 0);
+                    }
+                } else {
+                    buf[i].template load<FULL>(base, (size_t)off[i], f % STEPS, f % STEPS == STEPS - 1, a.D, lane);
                 }
             }
+        };
+        // Ends a fetch: after the barrier behind it the tile may be read.
+        const auto stage = [&](Staged<BF16, kSub * STEPS, kTile>& into) {
+            if constexpr (!FULL) {
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    const int f = i * kWaves + wave;
+                    if (kSub * STEPS % kWaves == 0 || f < kSub * STEPS) buf[i].put(into.x[f], lane);
+                }
+            }
+            if (threadIdx.x < kTile) {
+                into.lse[threadIdx.x] = buf_lse;
+                into.last[threadIdx.x] = buf_last;
+                if (!SUM) {
+                    const bool any = __ballot(buf_last < 0) != 0;
+                    if (threadIdx.x == 0) into.gap = any;
+                }
+            }
+            if constexpr (FULL) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's loads have landed
+            __syncthreads();
         };
         float m[NT], l[NT];  // stats: running maximum and sum; sum: l is the token's weight
 #pragma unroll
@@ -682,70 +738,91 @@ __global__ __launch_bounds__(kThreads) void many_kernel(AttnWeightsArgs a) {
         __syncthreads();  // the item before has read its tiles
         if (from < to) {
             ids(from);
-            fetch(from);
-            stage(0);
+            fetch(tile0, from);
+            stage(tile0);
         }
-        __syncthreads();
         const bool mine = hold0 < (SUM ? s.ctx : rows);
         const int whole = SUM ? 0 : last_seen(a, s, min(hold0, rows - 1));  // seen by all of the wave's rows
-        // A streamed tile. EDGE: some of its scores are hidden.
-        const auto work = [&](auto edge, int v0, int at) {
-            constexpr bool EDGE = decltype(edge)::value;
+        // A streamed tile, two 16-vector parts at a time. EDGE: some of its scores are hidden.
+        const auto product = [&](f32x4 (&c)[2][NT], const Staged<BF16, kSub * STEPS, kTile>& in, int sub) {
 #pragma unroll
-            for (int sub = 0; sub < kSub; ++sub) {
-                f32x4 c[NT];
+            for (int j = 0; j < 2; ++j) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) c[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int nt = 0; nt < NT; ++nt) c[j][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < STEPS; ++i) {
-                    const Frag<BF16> y = tile[at][sub * STEPS + i][lane];
+                    Frag<BF16> y;
+                    y.get(in.x[(sub + j) * STEPS + i], lane);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) c[nt] = Frag<BF16>::mma(y, x[nt][i], c[nt]);
-                }
-                float set[4];
-                int see[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (SUM) set[i] = lse[at][sub * 16 + quad * 4 + i];
-                    if (EDGE) see[i] = last[at][sub * 16 + quad * 4 + i];
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float p[4];
-                    if constexpr (SUM) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            p[i] = fast_exp2(c[nt][i] * a.scale_log2 - set[i]);
-                            if (EDGE) p[i] = hold0 + nt * 16 + col > see[i] ? 0.f : p[i];
-                        }
-                        l[nt] += (p[0] + p[1]) + (p[2] + p[3]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            p[i] = c[nt][i] * a.scale_log2;
-                            if (EDGE) {
-                                const bool hidden = (see[i] < 0) | (v0 + sub * 16 + quad * 4 + i > limit[nt]);
-                                p[i] = hidden ? kNegInf : p[i];
-                            }
-                        }
-                        add_scores<4>(m[nt], l[nt], p);
-                    }
+                    for (int nt = 0; nt < NT; ++nt) c[j][nt] = Frag<BF16>::mma(y, x[nt][i], c[j][nt]);
                 }
             }
         };
-        int at = 0;
-        for (int v0 = from; v0 < to; v0 += kTile, at ^= 1) {
-            const bool more = v0 + kTile < to;
-            if (more) fetch(v0 + kTile);
-            if (mine) {
-                // sum: the wave's last token against what the tile's first row sees.
-                const bool edge = SUM ? hold0 + NT * 16 - 1 > __builtin_amdgcn_readfirstlane(last[at][0])
-                                      : v0 + kTile - 1 > whole || __builtin_amdgcn_readfirstlane(gap[at]) != 0;
-                if (edge) work(std::true_type{}, v0, at);
-                else work(std::false_type{}, v0, at);
+        const auto scores = [&](auto edge, const f32x4 (&c)[2][NT], const Staged<BF16, kSub * STEPS, kTile>& in, int sub,
+                                int v0) {
+            constexpr bool EDGE = decltype(edge)::value;
+            float set[2][4];
+            int see[2][4];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (SUM) set[j][i] = in.lse[(sub + j) * 16 + quad * 4 + i];
+                    if (EDGE) see[j][i] = in.last[(sub + j) * 16 + quad * 4 + i];
+                }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                if constexpr (SUM) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float p[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            p[i] = fast_exp2(c[j][nt][i] * a.scale_log2 - set[j][i]);
+                            if (EDGE) p[i] = hold0 + nt * 16 + col > see[j][i] ? 0.f : p[i];
+                        }
+                        l[nt] += (p[0] + p[1]) + (p[2] + p[3]);
+                    }
+                } else {
+                    float p[8];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            p[4 * j + i] = c[j][nt][i];
+                            if (EDGE) {
+                                const bool hidden = (see[j][i] < 0) | (v0 + (sub + j) * 16 + quad * 4 + i > limit[nt]);
+                                p[4 * j + i] = hidden ? kNegInf : p[4 * j + i];
+                            }
+                        }
+                    add_products<8>(m[nt], l[nt], p, a.scale_log2);
+                }
             }
-            if (more) stage(at ^ 1);
-            __syncthreads();
+        };
+        const auto work = [&](auto edge, const Staged<BF16, kSub * STEPS, kTile>& in, int v0) {
+#pragma unroll
+            for (int sub = 0; sub < kSub; sub += 2) {
+                f32x4 c[2][NT];
+                product(c, in, sub);
+                scores(edge, c, in, sub, v0);
+            }
+        };
+        // sum: the wave's last token against what the tile's first row sees.
+        const auto turn = [&](Staged<BF16, kSub * STEPS, kTile>& in, Staged<BF16, kSub * STEPS, kTile>& next, int v0) {
+            const bool more = v0 + kTile < to;
+            if (more) fetch(next, v0 + kTile);
+            if (mine) {
+                const bool edge = v0 + kTile > to ||
+                                  (SUM ? hold0 + NT * 16 - 1 > __builtin_amdgcn_readfirstlane(in.last[0])
+                                       : v0 + kTile - 1 > whole || __builtin_amdgcn_readfirstlane(in.gap) != 0);
+                if (edge) work(std::true_type{}, in, v0);
+                else work(std::false_type{}, in, v0);
+            }
+            if (more) stage(next);
+        };
+        for (int v0 = from; v0 < to; v0 += 2 * kTile) {
+            turn(tile0, tile1, v0);
+            if (v0 + kTile < to) turn(tile1, tile0, v0 + kTile);
         }
         if constexpr (SUM) {
             const size_t base = ((size_t)row * a.Hkv + h) * a.max_tokens;

@@ -129,6 +129,23 @@ def test_long_context(gpu):
     check_weights(case(gpu, rows=[1, 3], old=[70001, 33], H=4, hkv=1, D=64, seed=3))
 
 
+def test_more_scores_than_are_kept(gpu):
+    """16 rows of 64 kv heads at 70000 tokens: 286 MB of scores, of which 256 MiB are kept between the passes."""
+    check_weights(case(gpu, rows=[1], old=[69999], H=1024, hkv=64, D=8, seed=5))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_prompts_beside_decode_steps(gpu, dtype):
+    """Sequences of many rows and of few in one call, each with its own kernels."""
+    check_weights(case(gpu, rows=[1, 200, 9, 0, 1, 65], old=[900, 40, 333, 7, 0, 64], D=128, H=8, hkv=2, dtype=dtype, seed=6))
+
+
+def test_many_rows_over_few_tokens(gpu):
+    """The rows of a sum split into parts, joined in their order."""
+    check_weights(case(gpu, rows=[700], old=[3], D=128, H=8, hkv=1, seed=7))
+    check_weights(case(gpu, rows=[900, 2], old=[0, 100], D=80, H=4, hkv=1, dtype=F32, seed=8))
+
+
 def test_not_causal_scale_out_and_row_positions(gpu):
     c = case(gpu, rows=[4, 1, 30], old=[10, 0, 99], seed=4)
     c["row_positions"] = torch.randint(0, 5000, (35,), device=gpu)
