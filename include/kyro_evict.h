@@ -18,6 +18,9 @@
  * of a call may not name the same row. After an eviction a token's slot differs between kv heads and is
  * no longer its position: rows appended from then on are rotated by positions of their own
  * (kyro_qkv_append's positions). Entries behind a sequence's tokens are not read or written.
+ *
+ * Both calls take scratch from the context's arena, as attention does: captured into HIP graphs, the calls of one
+ * context run in order, one replay after the other.
  */
 #ifndef KYRO_EVICT_H
 #define KYRO_EVICT_H
@@ -56,7 +59,8 @@ typedef struct kyro_attn_weights_params {
  *                            softmax_t(scale * query[j][g] . key[t]) over the tokens row j sees
  * The new tokens are the sequence's last q_len, which the step has appended: their entries start at 0
  * whatever they held (a rejected draft's), and positions[r][h][t] becomes row_positions[row] (NULL: t). A
- * row that sees no token adds nothing. Sums and softmax are held in 32 bits; results do not depend on the
+ * row that sees no token (of a context shorter than its rows, or empty as in a padded batch) adds nothing.
+ * Sums and softmax are held in 32 bits; results do not depend on the
  * order of execution. out_weights may be weights itself; otherwise they do not overlap.
  *   query [total_q, H, D] dtype, q_start_loc, key_cache, block_table, context_lens: as for
  *     kyro_paged_attention_mq, after kyro_paged_kv_append or kyro_qkv_append has written the rows

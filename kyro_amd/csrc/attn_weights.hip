@@ -123,10 +123,10 @@ struct Walk {
                 const int64_t c = a.ctx_lens[b];
                 int bad = 0;
                 if (r0 < 0 || r1 < r0 || r1 > a.total_q || r1 - r0 > a.max_q_len) bad |= ERR_Q_LAYOUT;
-                else if (c < r1 - r0 || c > a.cap) bad |= ERR_CTX_LEN;
+                else if (c < 0 || c > a.cap) bad |= ERR_CTX_LEN;
                 if (bad) {
                     latch_error(a.err, bad);
-                } else if (r1 > r0) {
+                } else if (r1 > r0 && c > 0) {
                     q0 = r0;
                     n = r1 - r0;
                     ctx = (int)c;

@@ -122,8 +122,8 @@ int weights_setup(const kyro_attn_weights_params* p, bool has_q_start, int num_c
     // Chunks as long as they may be while there are a few for each CU: a chunk costs its start (a walk to its
     // sequence, its queries, its first keys), the last ones leave CUs idle. 8 x 2048 and 16 x 1024 tokens a CU
     // measured best on the two cases above.
-    int64_t chunk = many ? 256 : 64;
-    while (chunk < (keep ? 1024 : 2048) && items(2 * chunk) >= (keep ? 8 : 4) * num_cus) chunk *= 2;
+    int64_t chunk = many && a.bf16 ? 128 : 64;
+    while (chunk < (keep ? 1024 : 2048) && items(2 * chunk) >= (keep ? 8 : many ? 2 : 4) * num_cus) chunk *= 2;
     while (part_bytes(chunk) > ((size_t)64 << 20) && chunk < a.cap) chunk *= 2;
     a.chunk = (int)chunk;
     // 64 sequences' items are counted in 32 bits.
@@ -137,9 +137,9 @@ int weights_setup(const kyro_attn_weights_params* p, bool has_q_start, int num_c
     a.few_grid = (int)std::min(most, a.few_items_most);
     a.many_stat_grid = many ? (int)std::min(most, items(chunk)) : 0;
     // Few runs of tokens for the CUs (short contexts of many rows): the rows are split, into parts of at least
-    // 256, until there are two workgroups a CU.
+    // 128 (f32 products take eight times as long: 64), until there are two workgroups a CU.
     const int64_t runs = a.B * ((a.cap + hold - 1) / hold) * a.Hkv;
-    a.row_parts = many ? (int)std::max<int64_t>(1, std::min<int64_t>((2 * num_cus + runs - 1) / runs, rows / 256)) : 1;
+    a.row_parts = many ? (int)std::max<int64_t>(1, std::min<int64_t>((2 * num_cus + runs - 1) / runs, rows / (a.bf16 ? 128 : 64))) : 1;
     a.run_tokens = (a.cap + hold - 1) / hold * hold;
     a.many_sum_grid = many ? (int)std::min(most, runs * a.row_parts) : 0;
     bytes = align_up(part_bytes(chunk), 256) + (many ? align_up((size_t)a.total_q * a.H * sizeof(float), 256) : 0);

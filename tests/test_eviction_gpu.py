@@ -59,6 +59,8 @@ def plain_weights(c, causal=True, scale=None):
         if n == 0:
             continue
         tok = torch.arange(n_ctx, device=q.device)
+        if n_ctx == 0:
+            continue
         last = n_ctx - n + torch.arange(n, device=q.device) if causal else torch.full((n,), n_ctx - 1, device=q.device)
         for h in range(hkv):
             k = c["key_cache"][c["block_table"][b], h].reshape(-1, D)[:n_ctx].double()
@@ -67,14 +69,15 @@ def plain_weights(c, causal=True, scale=None):
                 x = q[starts[b]:starts[b + 1], g]
                 s = (x @ k.T * scale).masked_fill(tok > last[:, None], -float("inf"))
                 size = ((x.abs() @ k.abs().T) * abs(scale)).amax(1)
-                p = torch.softmax(s, -1)
+                p = torch.softmax(s, -1).nan_to_num()  # a row that sees nothing adds nothing
                 new += p.sum(0)
                 err += (p * (2 * (D + 4) * size + 128 + n * (H // hkv))[:, None]).sum(0) * U
-            w[st, h, : n_ctx - n] += new[: n_ctx - n]
-            w[st, h, n_ctx - n:n_ctx] = new[n_ctx - n:]
+            old = max(0, n_ctx - n)
+            w[st, h, :old] += new[:old]
+            w[st, h, old:n_ctx] = new[old:]
             tol[st, h, :n_ctx] = err + 2 * U * w[st, h, :n_ctx].abs() + 1e-37
-            at = c["row_positions"][starts[b]:starts[b + 1]] if c.get("row_positions") is not None else tok[n_ctx - n:]
-            pos[st, h, n_ctx - n:n_ctx] = at.int()
+            at = c["row_positions"][starts[b]:starts[b + 1]][old - (n_ctx - n):] if c.get("row_positions") is not None else tok[old:]
+            pos[st, h, old:n_ctx] = at.int()
     return w, pos, tol
 
 
@@ -161,6 +164,30 @@ def test_entries_behind_the_tokens_and_other_rows_stay(gpu):
     check_weights(c)  # compares the whole state
 
 
+@pytest.mark.parametrize("rows", [(1, 1, 4, 6), (1, 130, 4, 300)])
+def test_padded_batches_and_contexts_shorter_than_their_rows(gpu, rows):
+    """Empty contexts with a row each, as a padded batch has them, and rows that see no token."""
+    c = case(gpu, rows=rows, old=[0, 30, 60, 0], seed=9)
+    c["context_lens"] = torch.tensor([0, 30 + rows[1], 2, rows[3] - 3], device=gpu)
+    c["row_positions"] = torch.randint(0, 5000, (sum(rows),), device=gpu)
+    check_weights(c)
+    assert (c["weights"][0] <= 1).all()
+
+
+def test_unseen_numbers_reach_nothing_from_prompts(gpu):
+    """The same for the kernels of many rows: a row of NaN reaches the tokens it sees and no others."""
+    c = case(gpu, rows=[200, 90], old=[50, 7], D=128, H=2, hkv=2, extra_rows=5)
+    c["query"][290:] = float("nan")
+    for b, n in enumerate([250, 97]):
+        t = torch.arange(n, 16 * c["block_table"].shape[1], device=gpu)
+        c["key_cache"][c["block_table"][b, t // 16], :, t % 16] = float("nan")
+    check_weights(c)
+    c["query"][250, 1] = float("nan")  # the second sequence's row 50: sees tokens 0 to 57
+    out = kyro_amd.CacheEviction(16, 2, 128, 2).accumulate(**c)
+    assert out[1, 1, :58].isnan().all() and out[1, 1, 58:].isfinite().all()
+    assert out[0].isfinite().all() and out[1, 0].isfinite().all()
+
+
 def test_one_row_without_q_start(gpu):
     c = case(gpu, rows=[1, 1, 1], old=[5, 0, 300])
     d = {k: v.clone() for k, v in c.items() if k != "q_start_loc"}
@@ -206,7 +233,7 @@ def test_bad_sequences_are_reported_and_left_out(gpu):
         c = case(gpu, rows=[2, 3, 1, 5], old=[20, 5, 7, 9], state_rows=[0, 1, 2, 3], max_tokens=40, width=4)
         bad = [1]
         if what == "context":
-            c["context_lens"][1] = 2
+            c["context_lens"][1] = -1
         elif what == "cap":
             c["context_lens"][1] = 41
         elif what == "layout":
