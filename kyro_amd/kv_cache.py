@@ -159,32 +159,32 @@ class PagedKVCache:
             (total_q, heads, _), (B, width), nb = query.shape, block_table.shape, key_cache.shape[0]
         if total_q == 1:  # torch gives a single row any stride
             q_stride = k_stride = v_stride = 0
-        dev = query.device
         rotary = max_position = 0
-        if (cos is None) != (sin is None):
-            raise ValueError("cos and sin come together")
-        if cos is not None:
-            _require(cos, "cos", (torch.float32,), 2, dev)
-            _require(sin, "sin", (torch.float32,), 2, dev)
-            if cos.shape != sin.shape:
-                raise ValueError("cos and sin must have the same shape")
-            max_position, rotary = cos.shape
-            rotary *= 2
         weight_dtype = src
-        if (q_weight is None) != (k_weight is None):
-            raise ValueError("q_weight and k_weight come together")
-        if q_weight is not None:
-            if norm_eps is None:
-                raise ValueError("norm weights need norm_eps")
-            weight_dtype = q_weight.dtype
-            _require(q_weight, "q_weight", (torch.float32, torch.bfloat16), 1, dev)
-            _require(k_weight, "k_weight", (weight_dtype,), 1, dev)
-            if q_weight.shape[0] != d or k_weight.shape[0] != d:
-                raise ValueError(f"norm weights must have {d} entries")
+        try:
+            if cos is not None:
+                max_position, half = turn = cos.shape
+                rotary = 2 * half
+                plain = (cos.dtype == torch.float32 and sin.dtype == torch.float32 and sin.shape == turn
+                         and cos.is_contiguous() and sin.is_contiguous() and cos.get_device() == idx
+                         and sin.get_device() == idx)
+            else:
+                plain = sin is None
+            if q_weight is not None:
+                weight_dtype = q_weight.dtype
+                plain = (plain and norm_eps is not None and weight_dtype in _DTYPES and k_weight.dtype == weight_dtype
+                         and q_weight.shape == (d,) and k_weight.shape == (d,) and q_weight.is_contiguous()
+                         and k_weight.is_contiguous() and q_weight.get_device() == idx and k_weight.get_device() == idx)
+            else:
+                plain = plain and k_weight is None
+        except (AttributeError, ValueError):
+            plain = False
+        if not plain:
+            self._turn_require(query.device, cos, sin, q_weight, k_weight, norm_eps)
         if out is None:
-            out = torch.empty((total_q, heads, d), dtype=dst, device=dev)
+            out = query.new_empty((total_q, heads, d), dtype=dst)
         else:
-            _require(out, "out", (dst,), 3, dev)
+            _require(out, "out", (dst,), 3, query.device)
             if out.shape != query.shape:
                 raise ValueError("out has the wrong shape")
         params = _lib.pack_qkv_append(bs, heads, hkv, d, B, total_q, width, nb, _DTYPES[src], _DTYPES[dst], rotary,
@@ -201,6 +201,25 @@ class PagedKVCache:
             None if k_weight is None else k_weight.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
             out.data_ptr()))
         return out
+
+    def _turn_require(self, dev, cos, sin, q_weight, k_weight, norm_eps):
+        """Raises what is wrong with append_qkv's tables and weights."""
+        if (cos is None) != (sin is None):
+            raise ValueError("cos and sin come together")
+        if cos is not None:
+            _require(cos, "cos", (torch.float32,), 2, dev)
+            _require(sin, "sin", (torch.float32,), 2, dev)
+            if cos.shape != sin.shape:
+                raise ValueError("cos and sin must have the same shape")
+        if (q_weight is None) != (k_weight is None):
+            raise ValueError("q_weight and k_weight come together")
+        if q_weight is not None:
+            if norm_eps is None:
+                raise ValueError("norm weights need norm_eps")
+            _require(q_weight, "q_weight", (torch.float32, torch.bfloat16), 1, dev)
+            _require(k_weight, "k_weight", (q_weight.dtype,), 1, dev)
+            if q_weight.shape[0] != self.head_dim or k_weight.shape[0] != self.head_dim:
+                raise ValueError(f"norm weights must have {self.head_dim} entries")
 
     def _qkv_require(self, query, key, value, key_cache, value_cache, block_table, context_lens, q_start_loc, positions):
         """Raises what is wrong with append_qkv's tensors; (query, key, value) row strides where nothing is."""
