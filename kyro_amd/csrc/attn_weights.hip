@@ -501,10 +501,10 @@ __global__ __launch_bounds__(kThreads) void few_sum_kernel(AttnWeightsArgs a) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) p[i][u] = fast_exp2(c[i] * a.scale_log2 - to[nt][i]);
                 }
-                if (t0 + 16 * U - 1 > whole) {
+                if (t0 + 16 * U - 1 > whole || rows < NT * 16) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int last = last_seen(a, s, nt * 16 + quad * 4 + i);
+                        const int r = nt * 16 + quad * 4 + i, last = r < rows ? last_seen(a, s, r) : -1;
 #pragma unroll
                         for (int u = 0; u < U; ++u) p[i][u] = t0 + 16 * u + col > last ? 0.f : p[i][u];
                     }
@@ -548,11 +548,11 @@ __global__ __launch_bounds__(kThreads) void kept_sum_kernel(AttnWeightsArgs a) {
             for (int r = 0; r < a.kept_rows; r += 4) {
                 const float4 v = x[(size_t)(r / 4) * a.chunk];
                 // What a row does not see was kept as -infinity, and adds nothing to it even where the row
-                // has a NaN.
-                const float p0 = v.x == kNegInf ? 0.f : fast_exp2(v.x - lse[r]);
-                const float p1 = v.y == kNegInf ? 0.f : fast_exp2(v.y - lse[r + 1]);
-                const float p2 = v.z == kNegInf ? 0.f : fast_exp2(v.z - lse[r + 2]);
-                const float p3 = v.w == kNegInf ? 0.f : fast_exp2(v.w - lse[r + 3]);
+                // has a NaN. What fills up the last rows (lse infinity) adds nothing even where the token has one.
+                const float p0 = ((v.x == kNegInf) | (lse[r] == -kNegInf)) ? 0.f : fast_exp2(v.x - lse[r]);
+                const float p1 = ((v.y == kNegInf) | (lse[r + 1] == -kNegInf)) ? 0.f : fast_exp2(v.y - lse[r + 1]);
+                const float p2 = ((v.z == kNegInf) | (lse[r + 2] == -kNegInf)) ? 0.f : fast_exp2(v.z - lse[r + 2]);
+                const float p3 = ((v.w == kNegInf) | (lse[r + 3] == -kNegInf)) ? 0.f : fast_exp2(v.w - lse[r + 3]);
                 sum += (p0 + p1) + (p2 + p3);
             }
             store_weight(a, s, base, t, w + sum);

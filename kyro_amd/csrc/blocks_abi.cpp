@@ -98,6 +98,8 @@ int weights_setup(const kyro_attn_weights_params* p, bool has_q_start, int num_c
     a.cap = token_cap(a.max_blocks, a.bs, a.max_tokens);
     const double scale = p->scale != 0.f ? (double)p->scale : 1.0 / std::sqrt((double)a.D);
     a.scale_log2 = (float)(scale * 1.4426950408889634);
+    if (!std::isnormal(a.scale_log2))
+        return fail(KYRO_EINVAL, "attn_weights: scale %g is too small or too large for 32 bits", (double)p->scale);
     if (a.B == 0 || a.total_q == 0) return KYRO_OK;
     const int64_t rows = (int64_t)std::min(a.max_q_len, a.total_q) * a.group;
     const double block_elems = (double)a.Hkv * a.bs * a.D;

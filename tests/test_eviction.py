@@ -46,7 +46,8 @@ def test_good_calls_only_lack_their_context():
     (dict(block_size=0), "EINVAL", "sizes"), (dict(max_tokens=0), "EINVAL", "sizes"), (dict(max_q_len=-1), "EINVAL", "sizes"),
     (dict(num_heads=7), "EINVAL", "num_kv_heads"), (dict(head_dim=68), "EUNSUPPORTED", "head_dim 68"),
     (dict(head_dim=264), "EUNSUPPORTED", "head_dim 264"), (dict(dtype=3), "EINVAL", "dtype"),
-    (dict(scale=math.nan), "EINVAL", "scale"), (dict(scale=-0.5), "EINVAL", "scale"), (dict(total_q=5), "EINVAL", "batch_size"),
+    (dict(scale=math.nan), "EINVAL", "scale"), (dict(scale=-0.5), "EINVAL", "scale"),
+    (dict(scale=1e-44), "EINVAL", "scale"), (dict(scale=3e38), "EINVAL", "scale"), (dict(total_q=5), "EINVAL", "batch_size"),
     (dict(query=None), "EINVAL", "null device pointer"), (dict(positions=None), "EINVAL", "null device pointer"),
     (dict(key_cache=(2 << 20) + 8), "EINVAL", "16-byte"), (dict(num_state_rows=1), "EINVAL", "state row"),
     (dict(out_weights=(5 << 20) + 4), "EINVAL", "overlaps"),

@@ -188,6 +188,20 @@ def test_unseen_numbers_reach_nothing_from_prompts(gpu):
     assert out[0].isfinite().all() and out[1, 0].isfinite().all()
 
 
+@pytest.mark.parametrize("n,hkv", [(3, 2), (3, 8), (7, 2), (7, 8), (20, 2), (100, 2), (70, 8)])
+def test_a_score_of_minus_infinity_is_a_weight_of_zero(gpu, n, hkv):
+    """Every row scores one token -infinity. The zeros that fill up the operands of the products would make it
+    NaN (0 * infinity): they are no rows."""
+    c = case(gpu, rows=[n], old=[50], H=8, hkv=hkv, D=64, seed=n)
+    c["query"][..., 0] = -1
+    c["key_cache"][c["block_table"][0, 0], :, 5, 0] = float("inf")
+    c["weights"].zero_()
+    out = kyro_amd.CacheEviction(16, 8, 64, hkv).accumulate(**c)
+    assert (out[0, :, 5] == 0).all() and out.isfinite().all()
+    # each row of a kv head's 8 / hkv heads shares out a weight of 1, within 2^-24 x (the bound of plain_weights) of it
+    assert ((out[0].double().sum(-1) / (n * 8 // hkv) - 1).abs() < 1e-4).all()
+
+
 def test_one_row_without_q_start(gpu):
     c = case(gpu, rows=[1, 1, 1], old=[5, 0, 300])
     d = {k: v.clone() for k, v in c.items() if k != "q_start_loc"}
