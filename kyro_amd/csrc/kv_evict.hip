@@ -118,9 +118,10 @@ __device__ __forceinline__ int select(const EvictArgs& a, int b, Unit u, Shared&
         float x[kHeld];
 #pragma unroll
         for (int r = 0; r < kHeld; ++r) {
-            const int t = r * kSelThreads + tid;
-            p[r] = t < u.n ? u.pos[t] : INT32_MIN;
-            x[r] = t < u.n ? u.w[t] : 0.f;
+            // Behind the last token it again: a load that is always made waits for nothing.
+            const int t = min(r * kSelThreads + tid, u.n - 1);
+            p[r] = u.pos[t];
+            x[r] = u.w[t];
         }
         check_blocks(a, b, u.n, sh);  // while they are under way
 #pragma unroll
@@ -131,10 +132,9 @@ __device__ __forceinline__ int select(const EvictArgs& a, int b, Unit u, Shared&
         for (int r = 0; r < kHeld; ++r) key[r] = u.key(p[r], x[r]);
     } else {
         check_blocks(a, b, u.n, sh);
-#pragma unroll 8
+#pragma unroll 16
         for (int r = 0; r < rounds; ++r) {
-            const int t = r * kSelThreads + tid;
-            newest = max(newest, t < u.n ? u.pos[t] : INT32_MIN);
+            newest = max(newest, u.pos[min(r * kSelThreads + tid, u.n - 1)]);
         }
         newest = block_max(newest, sh.red);
         u.protect(newest, a.recent);
@@ -143,6 +143,8 @@ __device__ __forceinline__ int select(const EvictArgs& a, int b, Unit u, Shared&
             for (int r = 0; r < kHeld; ++r) {
                 const int t = min(r * kSelThreads + tid, u.n - 1);
                 key[r] = u.key(u.pos[t], u.w[t]);
+                // A part at a time: else all the loads come first, and spill.
+                if (r % (R == 32 ? 16 : 8) == (R == 32 ? 15 : 7)) __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
@@ -242,9 +244,26 @@ __device__ __forceinline__ int select(const EvictArgs& a, int b, Unit u, Shared&
             const unsigned long long hb = __ballot(hole), mb = __ballot(mover);
             if (hole) list(a, sh.hole, u.holes, sh.count[0][r * kSelWaves + wave] + __popcll(hb & below), t);
             if (mover) list(a, sh.mover, u.movers, sh.count[1][r * kSelWaves + wave] + __popcll(mb & below), t);
-            if (keep && !mover) {
-                if (u.ow != u.w) u.ow[t] = u.w[t];
-                if (u.op != u.pos) u.op[t] = u.pos[t];
+        }
+        if ((u.ow != u.w) | (u.op != u.pos)) {  // out of place: what stays where it is, four loads at a time
+#pragma unroll 1
+            for (int r0 = 0; r0 < kHeld && r0 * kSelThreads < u.budget; r0 += 4) {
+                float x[4];
+                int p[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int t = min((r0 + j) * kSelThreads + tid, u.n - 1);
+                    x[j] = u.w[t];
+                    p[j] = u.pos[t];
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int t = (r0 + j) * kSelThreads + tid;
+                    if (t < u.budget && ((kept >> (r0 + j)) & 1)) {
+                        if (u.ow != u.w) u.ow[t] = x[j];
+                        if (u.op != u.pos) u.op[t] = p[j];
+                    }
+                }
             }
         }
         return moves;
@@ -275,7 +294,7 @@ __device__ __forceinline__ int select(const EvictArgs& a, int b, Unit u, Shared&
     }
 }
 
-// HELD: most keys a thread holds (4, 16, 64), which sets the kernel's registers; with 4, two workgroups share
+// HELD: most keys a thread holds (4, 16, 32, 64), which sets the kernel's registers; with 4, two workgroups share
 // a CU (64 x 2304 tokens of 8 heads: 50 us with one, 43 with two).
 template <int HELD>
 __global__ __launch_bounds__(kSelThreads, HELD == 4 ? 8 : 4) void evict_select_kernel(EvictArgs a) {
@@ -321,7 +340,7 @@ __global__ __launch_bounds__(kSelThreads, HELD == 4 ? 8 : 4) void evict_select_k
     if (rounds <= 1) moves = select<1>(a, b, u, sh);
     else if (rounds <= 4) moves = select<4>(a, b, u, sh);
     else if (HELD >= 16 && rounds <= 16) moves = select<HELD >= 16 ? 16 : 1>(a, b, u, sh);
-    else if (HELD >= 64 && rounds <= 32) moves = select<HELD >= 64 ? 32 : 1>(a, b, u, sh);
+    else if (HELD >= 32 && rounds <= 32) moves = select<HELD >= 32 ? 32 : 1>(a, b, u, sh);
     else if (HELD >= 64 && rounds <= 64) moves = select<HELD >= 64 ? 64 : 1>(a, b, u, sh);
     else moves = select<0>(a, b, u, sh);
     if (moves < 0) {
@@ -390,6 +409,7 @@ hipError_t launch_kv_evict(const EvictArgs& a, hipStream_t stream) {
     const int units = a.B * a.Hkv;
     if (a.cap <= 4 * kSelThreads) evict_select_kernel<4><<<units, kSelThreads, 0, stream>>>(a);
     else if (a.cap <= 16 * kSelThreads) evict_select_kernel<16><<<units, kSelThreads, 0, stream>>>(a);
+    else if (a.cap <= 32 * kSelThreads) evict_select_kernel<32><<<units, kSelThreads, 0, stream>>>(a);
     else evict_select_kernel<64><<<units, kSelThreads, 0, stream>>>(a);
     if (a.max_moves > a.own_moves) evict_move_kernel<<<units * a.move_wgs, kMoveThreads, 0, stream>>>(a);
     return hipGetLastError();
