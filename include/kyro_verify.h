@@ -388,7 +388,7 @@ typedef struct kyro_qkv_append_params {
     int32_t max_position;        /* rows of cos / sin */
     int32_t norm;                /* 1: root-mean-square norm of each query and key head before the rotation */
     int32_t weight_dtype;        /* kyro_dtype of q_weight / k_weight */
-    float eps;                   /* added to the mean square */
+    float eps;                   /* added to the mean square; at least 2^-126 */
     float weight_offset;         /* added to the weights (1 for models that store w - 1) */
     int64_t query_stride;        /* elements from one row of query to the next (0 => H * D); a */
     int64_t key_stride;          /* multiple of 8. Slices of one projection's [total_q, (H + 2 Hkv) * D] */
@@ -403,8 +403,8 @@ typedef struct kyro_qkv_append_params {
  *     (w = 1 without weights); then with angle row t = positions[row] (NULL: t = p) of cos and sin,
  *     (x_i, x_i') <- (x_i cos[t][i] - x_i' sin[t][i], x_i' cos[t][i] + x_i sin[t][i]) for i < R/2;
  *   out_query [total_q, H, D] gets the queries, the caches' slots the keys and the values.
- * In 32 bits, rounded once to cache_dtype (to nearest even); values keep their bits where src_dtype
- * is cache_dtype.
+ * In 32 bits (the sum of squares too: a head's must stay below 3.4e38), rounded once to cache_dtype (to
+ * nearest even); values keep their bits where src_dtype is cache_dtype.
  *   query [total_q, H, D], key, value [total_q, Hkv, D]   src_dtype, rows at their strides, heads dense
  *   q_start_loc, block_table, context_lens, caches         as for kyro_paged_kv_append
  *   positions [total_q] int64 or NULL: needed where a token's position is not its slot, as after

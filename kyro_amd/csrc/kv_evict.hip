@@ -9,8 +9,8 @@
 // it moves at most 256 of them, where closing the gaps in order would move most of 2048.
 //
 // evict_select_kernel: one workgroup a (sequence, kv head). Weights and positions are read once, 8 bytes a
-// token, and the keys stay in registers, thread i holding slots i, i + 1024, .., for the three passes over
-// 11, 11 and 10 bits. The first digit holds the sign, the exponent and two bits of the mantissa, so weights
+// token (the positions a second time past 16 keys a thread), and the keys stay in registers, thread i holding
+// slots i, i + 1024, .., for the three passes over 11, 11 and 10 bits. The first digit holds the sign, the exponent and two bits of the mantissa, so weights
 // that fall over many octaves spread over its bins. Ballots give each token its rank in slot order; the
 // workgroup then copies its own K and V rows, up to kOwnMoves of them. evict_move_kernel: the rest, by
 // many workgroups, where a call may have that many. Contexts past the registers read their keys again.

@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -1176,8 +1177,9 @@ int kyro_qkv_append(kyro_ctx ctx, const kyro_qkv_append_params* p, const void* q
             return fail(KYRO_EINVAL, "qkv_append: unknown dtype");
         if (p->rotary_dim > 0 && (!cos || !sin || p->max_position <= 0))
             return fail(KYRO_EINVAL, "qkv_append: rotary_dim > 0 needs cos, sin and max_position > 0");
-        if (p->norm != 0 && (!(p->eps >= 0.f) || !std::isfinite(p->eps) || !std::isfinite(p->weight_offset)))
-            return fail(KYRO_EINVAL, "qkv_append: eps must be finite and >= 0, weight_offset finite");
+        // The kernel's reciprocal root takes no subnormals, which a smaller eps would let through.
+        if (p->norm != 0 && (!(p->eps >= FLT_MIN) || !std::isfinite(p->eps) || !std::isfinite(p->weight_offset)))
+            return fail(KYRO_EINVAL, "qkv_append: eps must be finite and >= 2^-126, weight_offset finite");
         if ((p->norm == 0 && (q_weight || k_weight)) || (!q_weight != !k_weight))
             return fail(KYRO_EINVAL, "qkv_append: norm weights come together, and with norm set");
         if (!q_start_loc && p->total_q != p->batch_size)

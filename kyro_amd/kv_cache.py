@@ -272,8 +272,8 @@ class PagedKVCache:
         first ``2 * cos.shape[1]`` elements of each query and key head, element i with i + half of them, or
         neighbours with ``interleaved``; without them nothing turns. ``positions`` (int64 [total_q]) are the
         tables' rows; by default a row's slot in its sequence, which it no longer is after
-        :meth:`kyro_amd.CacheEviction.evict`. ``norm_eps`` asks for the root-mean-square norm of each query
-        and key head, scaled by ``q_weight`` / ``k_weight`` (+ ``weight_offset``) where given. The call
+        :meth:`kyro_amd.CacheEviction.evict`. ``norm_eps`` (> 0) asks for the root-mean-square norm of each
+        query and key head, scaled by ``q_weight`` / ``k_weight`` (+ ``weight_offset``) where given. The call
         synchronises, so a bad block id, context length or position raises KyroError here."""
         out = self.append_qkv_async(query, key, value, key_cache, value_cache, block_table, context_lens, cos=cos,
                                     sin=sin, positions=positions, q_weight=q_weight, k_weight=k_weight,

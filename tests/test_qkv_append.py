@@ -43,7 +43,8 @@ def test_a_good_call_only_lacks_its_context():
     (dict(rotary_dim=31), "EINVAL", "rotary_dim"), (dict(rotary_dim=62), "EUNSUPPORTED", "multiple of 4"),
     (dict(src_dtype=2), "EINVAL", "dtype"), (dict(cache_dtype=5), "EINVAL", "dtype"), (dict(weight_dtype=-1), "EINVAL", "dtype"),
     (dict(cos=None), "EINVAL", "cos"), (dict(max_position=0), "EINVAL", "max_position"),
-    (dict(eps=-1.0), "EINVAL", "eps"), (dict(eps=math.nan), "EINVAL", "eps"), (dict(weight_offset=math.inf), "EINVAL", "offset"),
+    (dict(eps=-1.0), "EINVAL", "eps"), (dict(eps=0.0), "EINVAL", "eps"), (dict(eps=1e-39), "EINVAL", "eps"),
+    (dict(eps=math.nan), "EINVAL", "eps"), (dict(weight_offset=math.inf), "EINVAL", "offset"),
     (dict(norm=0), "EINVAL", "norm weights"), (dict(k_weight=None), "EINVAL", "norm weights"),
     (dict(total_q=3), "EINVAL", "batch_size"), (dict(query_stride=500), "EINVAL", "strides"),
     (dict(key_stride=132), "EINVAL", "strides"), (dict(value_stride=-128), "EINVAL", "strides"),
