@@ -66,6 +66,8 @@ def _rows(t, name, dtype, shape, device):
     st = t.stride()
     if (d > 1 and st[2] != 1) or (h > 1 and st[1] != d):
         raise ValueError(f"{name}'s heads must be dense: strides (any, {d}, 1), got {st}")
+    if n > 1 and st[0] < h * d:  # an expanded tensor's 0 would stand for dense rows in the library
+        raise ValueError(f"{name}'s rows must not share memory: a row stride of at least {h * d}, got {st[0]}")
     return st[0]
 
 
@@ -138,6 +140,7 @@ class PagedKVCache:
             plain = (idx >= 0 and src in _DTYPES and dst in _DTYPES and key.dtype == src and value.dtype == src
                      and query.shape[2] == d and kv == (rows, hkv, d) and value.shape == kv and rows > 0
                      and q1 == 1 and k1 == 1 and v1 == 1 and qh == d and kh == d and vh == d
+                     and q_stride >= heads * d and k_stride >= hkv * d and v_stride >= hkv * d
                      and key.get_device() == idx and value.get_device() == idx
                      and cache == (nb, hkv, bs, d) and value_cache.shape == cache and value_cache.dtype == dst
                      and key_cache.is_contiguous() and value_cache.is_contiguous()
@@ -268,12 +271,13 @@ class PagedKVCache:
         may be ``query`` itself where that is contiguous and of the caches' dtype).
 
         ``query`` [total_q, H, D], ``key`` and ``value`` [total_q, Hkv, D] are the projections' rows; they may
-        be slices of one [total_q, H + 2 Hkv, D] output. ``cos`` and ``sin`` (:func:`rope_tables`) turn the
-        first ``2 * cos.shape[1]`` elements of each query and key head, element i with i + half of them, or
-        neighbours with ``interleaved``; without them nothing turns. ``positions`` (int64 [total_q]) are the
-        tables' rows; by default a row's slot in its sequence, which it no longer is after
-        :meth:`kyro_amd.CacheEviction.evict`. ``norm_eps`` (> 0) asks for the root-mean-square norm of each
-        query and key head, scaled by ``q_weight`` / ``k_weight`` (+ ``weight_offset``) where given. The call
+        be slices of one [total_q, H + 2 Hkv, D] output, but no expanded tensors, whose rows share memory.
+        ``cos`` and ``sin`` (:func:`rope_tables`) turn the first ``2 * cos.shape[1]`` elements of each query
+        and key head, element i with i + half of them, or neighbours with ``interleaved``; without them nothing
+        turns. ``positions`` (int64 [total_q]) are the tables' rows; by default a row's slot in its sequence,
+        which it no longer is after :meth:`kyro_amd.CacheEviction.evict`. ``norm_eps`` (> 0) asks for the
+        root-mean-square norm of each query and key head, scaled by ``q_weight`` / ``k_weight``
+        (+ ``weight_offset``) where given. The call
         synchronises, so a bad block id, context length or position raises KyroError here."""
         out = self.append_qkv_async(query, key, value, key_cache, value_cache, block_table, context_lens, cos=cos,
                                     sin=sin, positions=positions, q_weight=q_weight, k_weight=k_weight,

@@ -87,3 +87,86 @@ def test_rope_tables_own_frequencies_and_refusals():
                 dict(max_position=4, rotary_dim=4, inv_freq=[1.0])):
         with pytest.raises(ValueError):
             kyro_amd.rope_tables(**bad)
+
+
+# ------------------------------------------------------------------------------------ the Python entry's own checks
+
+class OnGpu(torch.Tensor):
+    """A host tensor that says it is on a GPU: the library behind the checks is a stub here."""
+
+    def get_device(self):
+        return 0
+
+    @property
+    def device(self):
+        return torch.device("cuda", 0)
+
+    @property
+    def is_cuda(self):
+        return True
+
+
+class Recorder:
+    """Stands for the library and a context: keeps the parameters of a call that passes the checks."""
+
+    handle, params = None, None
+
+    def set_stream(self, stream):
+        pass
+
+    def kyro_qkv_append(self, handle, params, *pointers):
+        self.params = _lib.QkvAppendParams.from_buffer_copy(params)
+        return _lib.KYRO_OK
+
+
+@pytest.fixture
+def recorder(monkeypatch):
+    r = Recorder()
+    monkeypatch.setattr(_lib, "lib", lambda: r)
+    monkeypatch.setattr(_lib, "context", lambda idx: r)
+    monkeypatch.setattr(_lib, "current_stream", lambda idx: 0)
+    return r
+
+
+def python_call(rows=5, heads=8, **change):
+    """append_qkv_async of one sequence's rows with host tensors in place of the GPU's."""
+    t = dict(query=torch.zeros(rows, heads, 64), key=torch.zeros(rows, 2, 64), value=torch.zeros(rows, 2, 64),
+             key_cache=torch.zeros(9, 2, 16, 64), value_cache=torch.zeros(9, 2, 16, 64),
+             block_table=torch.zeros(1, 4, dtype=torch.int64), context_lens=torch.full((1,), rows),
+             q_start_loc=torch.tensor([0, rows], dtype=torch.int32), out=torch.zeros(rows, heads, 64))
+    t.update(change)
+    return kyro_amd.PagedKVCache(16, 2, 64).append_qkv_async(**{k: v.as_subclass(OnGpu) for k, v in t.items()})
+
+
+@pytest.mark.parametrize("name,heads", [("query", 8), ("key", 2), ("value", 2)])
+def test_rows_that_share_memory_are_refused(recorder, name, heads):
+    """The library reads a stride of 0 as that of dense rows: rows of an expanded tensor would be read behind it."""
+    for bad in (torch.zeros(1, heads, 64).expand(5, heads, 64), torch.zeros(heads + 4, 64).as_strided((5, heads, 64), (64, 64, 1))):
+        with pytest.raises(ValueError, match=f"{name}'s rows"):
+            python_call(**{name: bad})
+    assert recorder.params is None
+    # With one query head as well, where torch leaves the head stride open.
+    if name == "query":
+        with pytest.raises(ValueError, match="query's rows"):
+            kv = kyro_amd.PagedKVCache(16, 1, 64)
+            one = {k: torch.zeros(5, 1, 64).as_subclass(OnGpu) for k in ("key", "value", "out")}
+            caches = {k: torch.zeros(9, 1, 16, 64).as_subclass(OnGpu) for k in ("key_cache", "value_cache")}
+            kv.append_qkv_async(torch.zeros(1, 1, 64).expand(5, 1, 64).as_subclass(OnGpu), **one, **caches,
+                                block_table=torch.zeros(1, 4, dtype=torch.int64).as_subclass(OnGpu),
+                                context_lens=torch.full((1,), 5).as_subclass(OnGpu),
+                                q_start_loc=torch.tensor([0, 5], dtype=torch.int32).as_subclass(OnGpu))
+
+
+def test_row_strides_that_reach_the_library(recorder):
+    packed = torch.zeros(5, 12, 64)
+    python_call(query=packed[:, :8], key=packed[:, 8:10], value=packed[:, 10:])
+    p = recorder.params
+    assert (p.query_stride, p.key_stride, p.value_stride) == (768, 768, 768)
+    python_call()
+    p = recorder.params
+    assert (p.query_stride, p.key_stride, p.value_stride) == (512, 128, 128)
+    # One row has no next one: any stride is as good as the dense one.
+    python_call(rows=1, query=torch.zeros(1, 8, 64).as_strided((1, 8, 64), (0, 64, 1)), key=torch.zeros(2, 64).expand(1, 2, 64))
+    p = recorder.params
+    for stride, heads in ((p.query_stride, 8), (p.key_stride, 2), (p.value_stride, 2)):
+        assert stride in (0, heads * 64)
