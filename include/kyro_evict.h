@@ -53,13 +53,14 @@ typedef struct kyro_attn_weights_params {
 } kyro_attn_weights_params;
 
 /*
- * For every sequence b with rows, kv head h and cached token t < context_lens[b]:
+ * For every sequence b, kv head h and cached token t < context_lens[b]:
  *   out_weights[r][h][t] = (t is new ? 0 : weights[r][h][t])
  *                          + sum over the sequence's rows j and the query heads g of kv head h of
  *                            softmax_t(scale * query[j][g] . key[t]) over the tokens row j sees
  * The new tokens are the sequence's last q_len, which the step has appended: their entries start at 0
  * whatever they held (a rejected draft's), and positions[r][h][t] becomes row_positions[row] (NULL: t). A
- * row that sees no token (of a context shorter than its rows, or empty as in a padded batch) adds nothing.
+ * row that sees no token (of a context shorter than its rows, or empty as in a padded batch) adds nothing. A
+ * sequence without rows keeps its weights and positions: out_weights gets its weights as they are.
  * Sums and softmax are held in 32 bits; results do not depend on the
  * order of execution. out_weights may be weights itself; otherwise they do not overlap.
  *   query [total_q, H, D] dtype, q_start_loc, key_cache, block_table, context_lens: as for

@@ -256,6 +256,29 @@ __device__ __forceinline__ void store_weight(const AttnWeightsArgs& a, const Seq
     if (t >= old) a.positions[base + t] = a.row_pos ? (int32_t)a.row_pos[s.q0 + t - old] : t;
 }
 
+// Where the weights go elsewhere, a sequence that has no rows in the step takes its own along. The workgroups of
+// the kernel that calls it share a sequence's tokens where they are more than the sequences; at its end, so that
+// the work items' loads wait for nothing of this.
+__device__ __forceinline__ void copy_idle(const AttnWeightsArgs& a) {
+    const int parts = max(1u, gridDim.x / (unsigned)a.B);
+    for (unsigned item = blockIdx.x; item < (unsigned)parts * a.B; item += gridDim.x) {
+        const int part = (int)(item / (unsigned)a.B), b = (int)item - part * a.B;
+        const int r0 = a.q_start[b];
+        if (r0 != a.q_start[b + 1]) continue;
+        const int64_t ctx = a.ctx_lens[b];
+        const int bad = r0 < 0 || r0 > a.total_q ? ERR_Q_LAYOUT : ctx < 0 || ctx > a.cap ? ERR_CTX_LEN : 0;
+        if (bad && threadIdx.x == 0) latch_error(a.err, bad);
+        if (bad || ctx == 0) continue;
+        const int64_t row = state_row(a, b);
+        if (row < 0) continue;
+        const int64_t per = (ctx + parts - 1) / parts, from = part * per, to = min(ctx, from + per);
+        for (int h = 0; h < a.Hkv; ++h) {
+            const size_t base = ((size_t)row * a.Hkv + h) * a.max_tokens;
+            for (int64_t t = from + threadIdx.x; t < to; t += kThreads) a.out_w[base + t] = a.w[base + t];
+        }
+    }
+}
+
 // m + log2 l of a kv head's first N rows (a power of two, at most kThreads), merged over the chunks.
 template <int N>
 __device__ __forceinline__ void merge_chunks(const AttnWeightsArgs& a, const Sequence& s, int h, int parts, float2* partial,
@@ -522,6 +545,7 @@ __global__ __launch_bounds__(kThreads) void few_sum_kernel(AttnWeightsArgs a) {
             }
         }
     }
+    if (a.idle == kIdleFewSum) copy_idle(a);
 }
 
 // The sums of items whose scores were kept: a thread has a token.
@@ -558,6 +582,7 @@ __global__ __launch_bounds__(kThreads) void kept_sum_kernel(AttnWeightsArgs a) {
             store_weight(a, s, base, t, w + sum);
         }
     }
+    if (a.idle == kIdleKeptSum) copy_idle(a);
 }
 
 // ------------------------------------------------------------------- many rows (prompts)
@@ -872,9 +897,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttnWeightsArgs a) {
 }
 
 // The rows' statistics merged over their chunks, one thread a (row, head).
-__global__ __launch_bounds__(kThreads) void merge_kernel(AttnWeightsArgs a) {
-    const int64_t all = (int64_t)a.total_q * a.H, i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= all) return;
+__device__ __forceinline__ void merge_row(const AttnWeightsArgs& a, int64_t i, int64_t all) {
     const int r = (int)(i / a.H);
     // The row's sequence tells how many chunks there are; a row of none, or of one left out, has no
     // statistics.
@@ -898,6 +921,11 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(AttnWeightsArgs a) {
         merge(m, l, x.x, x.y);
     }
     a.lse[i] = log_sum(m, l);
+}
+__global__ __launch_bounds__(kThreads) void merge_kernel(AttnWeightsArgs a) {
+    const int64_t all = (int64_t)a.total_q * a.H, i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i < all) merge_row(a, i, all);
+    if (a.idle == kIdleMerge) copy_idle(a);
 }
 
 template <bool BF16, int STEPS, bool FULL>
@@ -952,9 +980,14 @@ int attn_weights_few_rows(bool bf16, int D) { return bf16 || D <= 128 ? 64 : 32;
 int attn_weights_many_hold(bool bf16, int D) { return bf16 || D <= 128 ? 256 : 128; }
 
 hipError_t launch_attn_weights(const AttnWeightsArgs& a, hipStream_t stream) {
-    if (a.B == 0 || a.total_q == 0) return hipSuccess;
-    if (a.bf16) launch_type<true>(a, stream);
-    else launch_attn_weights_f32(a, stream);
+    if (a.B == 0) return hipSuccess;
+    if (a.total_q == 0) {  // no row: the merge of none, which takes the sequences' weights along
+        if (a.idle) merge_kernel<<<(unsigned)(a.B < 256 ? 256 : 2048), kThreads, 0, stream>>>(a);
+    } else if (a.bf16) {
+        launch_type<true>(a, stream);
+    } else {
+        launch_attn_weights_f32(a, stream);
+    }
     return hipGetLastError();
 }
 #endif

@@ -469,8 +469,9 @@ int kyro_attn_weights(kyro_ctx ctx, const kyro_attn_weights_params* p, const voi
         kyro::AttnWeightsArgs a{};
         size_t bytes = 0;
         if (int rc = weights_setup(p, q_start_loc != nullptr, ctx ? ctx->num_cus : 256, a, bytes)) return rc;
-        if (a.B == 0 || a.total_q == 0) return check_ctx(ctx);
-        if (!query || !key_cache || !block_table || !context_lens || !weights || !out_weights || !positions)
+        // Without rows nothing is gained; weights that go elsewhere are taken along.
+        if (a.B == 0 || (a.total_q == 0 && weights == out_weights)) return check_ctx(ctx);
+        if ((!query && a.total_q) || !key_cache || !block_table || !context_lens || !weights || !out_weights || !positions)
             return fail(KYRO_EINVAL, "attn_weights: null device pointer");
         if ((at(query) | at(key_cache)) % 16 != 0)
             return fail(KYRO_EINVAL, "attn_weights: query and key_cache must be 16-byte aligned");
@@ -492,15 +493,21 @@ int kyro_attn_weights(kyro_ctx ctx, const kyro_attn_weights_params* p, const voi
         DeviceGuard dg(ctx->device);
         KYRO_HIP(dg.status);
         if (int rc = ensure_arena(ctx, bytes)) return rc;
-        char* base = static_cast<char*>(ctx->arena);
-        a.part = reinterpret_cast<float2*>(base);
-        base += align_up((size_t)((a.cap + a.chunk - 1) / a.chunk) * a.total_q * a.H * sizeof(float2), 256);
-        if (a.many_stat_grid) {
-            a.lse = reinterpret_cast<float*>(base);
-            base += align_up((size_t)a.total_q * a.H * sizeof(float), 256);
+        if (a.total_q > 0) {
+            char* base = static_cast<char*>(ctx->arena);
+            a.part = reinterpret_cast<float2*>(base);
+            base += align_up((size_t)((a.cap + a.chunk - 1) / a.chunk) * a.total_q * a.H * sizeof(float2), 256);
+            if (a.many_stat_grid) {
+                a.lse = reinterpret_cast<float*>(base);
+                base += align_up((size_t)a.total_q * a.H * sizeof(float), 256);
+            }
+            // A call has either parts of sums or kept scores.
+            a.row_sums = a.kept = reinterpret_cast<float*>(base);
         }
-        // A call has either parts of sums or kept scores.
-        a.row_sums = a.kept = reinterpret_cast<float*>(base);
+        if (weights != out_weights && q_start_loc)
+            a.idle = a.many_stat_grid || a.total_q == 0 ? kyro::kIdleMerge
+                     : a.kept_items                     ? kyro::kIdleKeptSum
+                                                        : kyro::kIdleFewSum;
         a.err = ctx->err;
         KYRO_HIP(kyro::launch_attn_weights(a, ctx->stream));
         return KYRO_OK;

@@ -351,6 +351,9 @@ bool qkv_append_setup(QkvAppendArgs& a);
 hipError_t launch_qkv_append(const QkvAppendArgs& a, hipStream_t stream);
 
 // Accumulated attention weight per cached token.
+// The kernel that copies the weights of sequences without rows, where they go elsewhere: one of those that a call
+// launches anyway.
+enum IdleCopy : int { kIdleNone, kIdleFewSum, kIdleKeptSum, kIdleMerge };
 struct AttnWeightsArgs {
     const void* q;              // [total_q, H, D]
     const int32_t* q_start;     // [B+1] or nullptr
@@ -381,6 +384,7 @@ struct AttnWeightsArgs {
     float* row_sums;            // [row_parts, B, Hkv, run_tokens]: the parts' sums, where there are several
     int64_t few_items_most;     // work items of the few-row kernels where every context is as long as it may be
     int64_t kept_items;         // items whose scores have room; 0: scores are not kept
+    int idle;                   // IdleCopy
 };
 
 // Rows a kv head up to which a sequence can go to the few-row kernels.

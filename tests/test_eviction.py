@@ -175,3 +175,13 @@ def test_make_private_random_streams():
         if rng.integers(0, 2):
             bm.take_copies()
         bm.check()
+
+
+def test_no_rows_at_all_still_take_weights_elsewhere():
+    """A call without rows is one to make where the weights go elsewhere, and needs its pointers then."""
+    none = dict(total_q=0, q_start_loc=8 << 20, query=None)
+    for change in (none, dict(none, out_weights=15 << 20), dict(none, weights=None, out_weights=None)):
+        rc, msg = weigh(**change)
+        assert rc == _lib.KYRO_EINVAL and "null kyro_ctx" in msg, (change, msg)
+    rc, msg = weigh(**dict(none, out_weights=15 << 20, block_table=None))
+    assert rc == _lib.KYRO_EINVAL and "null device pointer" in msg

@@ -616,3 +616,61 @@ def test_a_run_of_steps_under_a_budget(gpu):
     assert cut >= 10
     bm.free(2)
     bm.check()
+
+
+# ------------------------------------------------------------------------------------ weights that go elsewhere
+
+@pytest.mark.parametrize("what,rows,old,more", [
+    # 8 / 2 heads: 4 rows of a kv head for each of a sequence.
+    ("scores kept", (1, 0, 4, 0), (70, 33, 300, 0), {}),
+    ("scores computed again", (1, 0, 9, 0), (70, 33, 300, 16), {}),
+    ("f32, scores computed again", (0, 12, 0), (1, 900, 64), dict(dtype=F32)),
+    ("rows through LDS", (100, 0, 100), (70, 33, 300), {}),
+    ("both forms", (100, 0, 1, 0, 7), (70, 333, 300, 5, 0), {}),
+    ("rows in parts", (0, 700, 0), (3, 3, 3), dict(D=128, hkv=1)),
+    ("f32 rows in parts", (400, 0), (3, 90), dict(D=80, hkv=1, dtype=F32)),
+    ("a long sequence without rows", (0, 1), (5000, 20), {}),
+    ("no rows at all", (0, 0, 0), (17, 0, 400), {})])
+def test_weights_go_elsewhere_whole(gpu, what, rows, old, more):
+    """Entries of every sequence's tokens, also of one without rows, come from `weights`; what is behind them
+    in `out`, and state rows of no sequence, stay as they are."""
+    n = len(rows)
+    c = case(gpu, rows=rows, old=old, state_rows=[(2 * b + 1) % (2 * n + 1) for b in range(n)], num_state=2 * n + 1,
+             width=-(-(max(old) + max(rows)) // 16) + 3, seed=n, **more)
+    before, pos = c["weights"].clone(), c["positions"].clone()
+    want, want_pos, tol = plain_weights(c)
+    out = torch.full_like(before, 7.0)
+    kyro_amd.CacheEviction(16, 8, c["query"].shape[2], c["key_cache"].shape[1]).accumulate(**c, out=out)
+    held = torch.zeros_like(out, dtype=torch.bool)
+    for b in range(n):
+        held[(2 * b + 1) % (2 * n + 1), :, :old[b] + rows[b]] = True
+    assert (out[~held] == 7).all() and torch.equal(c["weights"], before) and torch.equal(c["positions"], want_pos)
+    assert ((out.double() - want).abs() <= tol)[held].all()
+    for b in range(n):
+        if rows[b] == 0:
+            r = (2 * b + 1) % (2 * n + 1)
+            assert torch.equal(out[r, :, :old[b]], before[r, :, :old[b]]) and torch.equal(c["positions"][r], pos[r])
+
+
+def test_bad_sequences_without_rows_are_reported_and_left_out(gpu):
+    for what, match in (("context", "context length"), ("cap", "context length"), ("row", "state row"), ("twice", "state row")):
+        for rows in ((0, 2, 0), (0, 0, 0)):
+            c = case(gpu, rows=rows, old=[20, 7, 9], state_rows=[0, 1, 2], max_tokens=40, width=4)
+            if what in ("context", "cap"):
+                c["context_lens"][0] = -1 if what == "context" else 41
+            else:
+                c["state_rows"][0] = 3 if what == "row" else 2
+            out = torch.full_like(c["weights"], 7.0)
+            with pytest.raises(kyro_amd.KyroError, match=match):
+                kyro_amd.CacheEviction(16, 8, 64, 2).accumulate(**c, max_q_len=2, out=out)
+            assert (out[0] == 7).all()
+            assert (out[2] == 7).all() if what == "twice" else torch.equal(out[2, :, :9], c["weights"][2, :, :9])
+            kyro_amd.sync()
+
+
+def test_padded_batch_without_rows_needs_no_state_row(gpu):
+    """Empty sequences of no rows have nothing to take along: their state rows are not looked at."""
+    c = case(gpu, rows=[3, 0, 0], old=[20, 0, 0], state_rows=[1, -1, -1], num_state=2)
+    out = torch.full_like(c["weights"], 7.0)
+    kyro_amd.CacheEviction(16, 8, 64, 2).accumulate(**c, out=out)
+    assert (out[0] == 7).all() and (out[1, :, :23] != 7).all()
