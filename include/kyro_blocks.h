@@ -77,7 +77,8 @@ int kyro_bm_allocate_with_prefix(kyro_bm bm, uint64_t request_id, const uint32_t
 int kyro_bm_allocate(kyro_bm bm, uint64_t request_id, int64_t num_tokens);
 /* Room for n more tokens of a request (a decode token, the k + 1 rows of a verify step). */
 int kyro_bm_append_slots(kyro_bm bm, uint64_t request_id, int64_t n);
-/* Shrinks a request to num_tokens (>= its prompt length), releasing blocks no longer needed. */
+/* Shrinks a request to num_tokens (>= its prompt length), releasing blocks no longer needed. A cut inside a
+ * block that others share, where the request's next tokens would be written, is KYRO_EINVAL. */
 int kyro_bm_truncate(kyro_bm bm, uint64_t request_id, int64_t num_tokens);
 /* Before a request's cached tokens are moved (kyro_kv_evict): replaces every block that the prefix cache or
  * another request shares by one of its own, with a pending copy (kyro_bm_take_copies), and forgets the
@@ -85,6 +86,9 @@ int kyro_bm_truncate(kyro_bm bm, uint64_t request_id, int64_t num_tokens);
  * kyro_bm_truncate may cut below it. KYRO_ENOSPACE when the free pool (after evicting cache leaves) cannot
  * hold the copies; the request is unchanged then. */
 int kyro_bm_make_private(kyro_bm bm, uint64_t request_id);
+/* The same for the blocks of the request's first num_tokens tokens alone: the slots that an eviction to that
+ * budget writes. Those behind stay shared, are only read by it, and go with kyro_bm_truncate. */
+int kyro_bm_make_private_front(kyro_bm bm, uint64_t request_id, int64_t num_tokens);
 /* Ends a request. cache_prompt != 0 hands its prompt blocks to the prefix cache (their K/V must
  * have been written); 0 releases them. */
 int kyro_bm_free(kyro_bm bm, uint64_t request_id, int32_t cache_prompt);

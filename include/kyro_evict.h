@@ -108,7 +108,7 @@ typedef struct kyro_kv_evict_params {
  *     the caches' slots >= budget are not written
  *   context_lens, out_context_lens [B] int64, not overlapping
  * A block that holds any of a sequence's first `budget` slots must be in no other table and twice in none
- * (kyro_bm_make_private sees to it). Afterwards the blocks behind the budget may be released
+ * (kyro_bm_make_private_front of the budget sees to it). Afterwards the blocks behind the budget may be released
  * (kyro_bm_truncate). Caches are on 16-byte boundaries. A bad block id, context length or state row latches
  * KYRO_EINVAL for the next kyro_sync, and that sequence is left as it is.
  */

@@ -45,7 +45,7 @@
 extern "C" {
 #endif
 
-#define KYRO_ABI_VERSION 10
+#define KYRO_ABI_VERSION 11
 
 typedef enum kyro_status {
     KYRO_OK = 0,

@@ -120,7 +120,7 @@ pack_qkv_append = packer(QkvAppendParams)
 pack_attn_weights = packer(AttnWeightsParams)
 pack_kv_evict = packer(KvEvictParams)
 
-ABI_VERSION = 10  # KYRO_ABI_VERSION of include/kyro_verify.h
+ABI_VERSION = 11  # KYRO_ABI_VERSION of include/kyro_verify.h
 
 _lib = None
 _lib_lock = threading.Lock()
@@ -169,6 +169,7 @@ _SIGNATURES = {
     "kyro_bm_append_slots": ([_P, ctypes.c_uint64, ctypes.c_int64], ctypes.c_int),
     "kyro_bm_truncate": ([_P, ctypes.c_uint64, ctypes.c_int64], ctypes.c_int),
     "kyro_bm_make_private": ([_P, ctypes.c_uint64], ctypes.c_int),
+    "kyro_bm_make_private_front": ([_P, ctypes.c_uint64, ctypes.c_int64], ctypes.c_int),
     "kyro_bm_free": ([_P, ctypes.c_uint64, ctypes.c_int32], ctypes.c_int),
     "kyro_bm_request_blocks": ([_P, ctypes.c_uint64, _P, ctypes.c_int64, _P, _P], ctypes.c_int),
     "kyro_bm_take_copies": ([_P, _P, _P, ctypes.c_int64, _P], ctypes.c_int),

@@ -152,11 +152,17 @@ class BlockManager:
     def truncate(self, request_id: int, num_tokens: int) -> None:
         _lib.check(_lib.lib().kyro_bm_truncate(self._h, int(request_id), int(num_tokens)))
 
-    def make_private(self, request_id: int) -> bool:
+    def make_private(self, request_id: int, num_tokens: Optional[int] = None) -> bool:
         """Before :meth:`kyro_amd.CacheEviction.evict`: the request gets blocks of its own for those it
         shares (:meth:`take_copies` has the copies to queue) and its prompt is no longer handed to the prefix
-        cache, nor a floor for :meth:`truncate`. False, and nothing changes, when no blocks are left."""
-        rc = _lib.lib().kyro_bm_make_private(self._h, int(request_id))
+        cache, nor a floor for :meth:`truncate`. With ``num_tokens``, the eviction's budget, only the blocks of
+        so many tokens, which are the ones it writes; those behind stay shared until :meth:`truncate` cuts them
+        off. False, and the request is unchanged, when no blocks are left."""
+        lib = _lib.lib()
+        if num_tokens is None:
+            rc = lib.kyro_bm_make_private(self._h, int(request_id))
+        else:
+            rc = lib.kyro_bm_make_private_front(self._h, int(request_id), int(num_tokens))
         if rc == _lib.KYRO_ENOSPACE:
             return False
         _lib.check(rc)

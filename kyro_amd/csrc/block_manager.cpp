@@ -245,13 +245,15 @@ int BlockManager::append_slots(uint64_t rid, int64_t n) {
 }
 
 // Drops rows after num_tokens (rejected drafts), releasing blocks no longer covered. The prompt
-// is never cut: its last block may be shared with the cache.
+// is never cut: its last block may be shared with the cache. A request made private has no prompt, but
+// may share blocks behind its front ones: the next row must not be written into one of them.
 int BlockManager::truncate(uint64_t rid, int64_t num_tokens) {
     auto it = table_.find(rid);
     if (it == table_.end()) return EINVAL_;
     Request& r = it->second;
     const int64_t floor_len = r.has_prompt ? (int64_t)r.prompt.size() : 0;
     if (num_tokens < floor_len || num_tokens > r.num_tokens) return EINVAL_;
+    if (!r.has_prompt && num_tokens % bs_ != 0 && ref_[(size_t)r.blocks[(size_t)(num_tokens / bs_)]] > 1) return EINVAL_;
     const int64_t keep = blocks_for(num_tokens, bs_);
     while ((int64_t)r.blocks.size() > keep) {
         release(r.blocks.back());
@@ -261,25 +263,27 @@ int BlockManager::truncate(uint64_t rid, int64_t num_tokens) {
     return OK;
 }
 
-// A request whose cached tokens are about to be moved (eviction) owns its blocks alone: every one that
-// another holder shares is replaced by a fresh block and a pending copy. Its blocks no longer hold its
-// prompt in order, so the prompt is forgotten: it is not handed to the prefix cache when the request ends,
-// and truncate may cut below it. Evicting cache leaves to make room can only lower reference counts, so
-// the blocks are looked at again after it.
-int BlockManager::make_private(uint64_t rid) {
+// A request whose cached tokens are about to be moved (eviction) owns the blocks of its first num_tokens
+// tokens alone, the ones that are written: every one of them that another holder shares is replaced by a fresh
+// block and a pending copy. Its blocks no longer hold its prompt in order, so the prompt is forgotten: it is
+// not handed to the prefix cache when the request ends, and truncate may cut below it. Evicting cache leaves
+// to make room can only lower reference counts, so the blocks are looked at again after it.
+int BlockManager::make_private(uint64_t rid, int64_t num_tokens) {
     auto it = table_.find(rid);
-    if (it == table_.end()) return EINVAL_;
+    if (it == table_.end() || num_tokens < 0) return EINVAL_;
     Request& r = it->second;
+    const size_t front = (size_t)blocks_for(std::min(num_tokens, r.num_tokens), bs_);
     int64_t need = 0;
-    for (int64_t b : r.blocks) need += ref_[(size_t)b] > 1;
+    for (size_t i = 0; i < front; ++i) need += ref_[(size_t)r.blocks[i]] > 1;
     if (!reserve(need)) return ENOSPACE;
-    for (int64_t& b : r.blocks) {
+    for (size_t i = 0; i < front; ++i) {
+        const int64_t b = r.blocks[i];
         if (ref_[(size_t)b] <= 1) continue;
         const int64_t fresh = free_.back();
         free_.pop_back();
         ref_[(size_t)fresh] = 1;
         copies_.push_back({b, fresh});  // the request's reference on b is the copy's from here on
-        b = fresh;
+        r.blocks[i] = fresh;
     }
     r.prompt.clear();
     r.has_prompt = false;

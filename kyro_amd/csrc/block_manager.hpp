@@ -88,7 +88,7 @@ class BlockManager {
     int allocate(uint64_t rid, int64_t num_tokens);
     int append_slots(uint64_t rid, int64_t n);
     int truncate(uint64_t rid, int64_t num_tokens);
-    int make_private(uint64_t rid);
+    int make_private(uint64_t rid, int64_t num_tokens);
     int free(uint64_t rid, bool cache_prompt);
 
     const Request* find(uint64_t rid) const;

@@ -302,7 +302,14 @@ int kyro_bm_truncate(kyro_bm bm, uint64_t request_id, int64_t num_tokens) {
 int kyro_bm_make_private(kyro_bm bm, uint64_t request_id) {
     return guarded([&]() -> int {
         if (!bm) return fail(KYRO_EINVAL, "bm_make_private: null handle");
-        return bm_status(bm->m.make_private(request_id), "bm_make_private", request_id);
+        return bm_status(bm->m.make_private(request_id, INT64_MAX), "bm_make_private", request_id);
+    });
+}
+
+int kyro_bm_make_private_front(kyro_bm bm, uint64_t request_id, int64_t num_tokens) {
+    return guarded([&]() -> int {
+        if (!bm) return fail(KYRO_EINVAL, "bm_make_private_front: null handle");
+        return bm_status(bm->m.make_private(request_id, num_tokens), "bm_make_private_front", request_id);
     });
 }
 

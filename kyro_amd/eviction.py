@@ -9,7 +9,7 @@ budget move into the slots of the ones that go, so caches, block tables and cont
     state = ev.new_state(rows, max_tokens, device)               # weights, positions, beside each layer's cache
     kv.append_qkv(..., positions=positions)                      # rows rotated by their own positions
     ev.accumulate(query, key_cache, block_table, context_lens, *state, row_positions=positions)
-    bm.make_private(rid); copy_blocks(key_cache, value_cache, bm.take_copies())
+    bm.make_private(rid, 2048); copy_blocks(key_cache, value_cache, bm.take_copies())
     context_lens = ev.evict(key_cache, value_cache, block_table, context_lens, *state, budget=2048)
     bm.truncate(rid, 2048)
 """
@@ -230,8 +230,9 @@ class CacheEviction:
         positions, and of the others those of the most weight (ties: the lower slot). Kept tokens in slots >=
         budget move, in ascending order, into the slots of the ones that go; all others stay where they are. K, V,
         weight and position move together. ``out`` (weights, positions) receives the kept entries instead of the
-        inputs. A sequence's blocks must be its own: :meth:`kyro_amd.BlockManager.make_private`. The call
-        synchronises, so errors the device detects raise KyroError here."""
+        inputs. The blocks of a sequence's first ``budget`` slots must be its own:
+        :meth:`kyro_amd.BlockManager.make_private`. The call synchronises, so errors the device detects raise
+        KyroError here."""
         lens = self.evict_async(key_cache, value_cache, block_table, context_lens, weights, positions, budget=budget,
                                 sink=sink, recent=recent, state_rows=state_rows, out=out)
         _lib.context(key_cache.device.index or 0).sync()

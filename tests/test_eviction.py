@@ -185,3 +185,109 @@ def test_no_rows_at_all_still_take_weights_elsewhere():
         assert rc == _lib.KYRO_EINVAL and "null kyro_ctx" in msg, (change, msg)
     rc, msg = weigh(**dict(none, out_weights=15 << 20, block_table=None))
     assert rc == _lib.KYRO_EINVAL and "null device pointer" in msg
+
+
+# ------------------------------------------------------------------------------------ the front blocks alone
+
+def shared_prompt(bm, tokens):
+    """A request whose whole prompt is shared with the prefix cache."""
+    bm.allocate_with_prefix(1, list(range(tokens)))
+    bm.free(1)
+    assert bm.allocate_with_prefix(2, list(range(tokens)))[1] == tokens
+
+
+def test_make_private_of_the_front_fits_where_the_whole_does_not():
+    """24 shared tokens cut to 6: two blocks are rewritten, and two are free. The four behind are only read, and
+    their references go with the cut."""
+    for front in (False, True):
+        bm = BlockManager(4, 18)
+        shared_prompt(bm, 24)
+        assert bm.allocate(3, 40) is not None and bm.num_free_blocks == 2
+        bm.allocate_with_prefix(4, list(range(24)))
+        before = bm.block_table[2]
+        if not front:
+            assert not bm.make_private(2) and bm.block_table[2] == before
+            continue
+        assert bm.make_private(2, 6)
+        copies, now = bm.take_copies(), bm.block_table[2]
+        assert [s for s, _ in copies] == before[:2] and [d for _, d in copies] == now[:2] and now[2:] == before[2:]
+        bm.check()
+        bm.truncate(2, 6)
+        assert bm.request(2)[1] == 6 and bm.block_table[2] == now[:2] and bm.block_table[4] == before
+        bm.free(2)
+        bm.check()
+        assert bm.num_free_blocks == 2 and bm.num_cached_blocks == 6
+
+
+def test_a_cut_inside_a_shared_block_is_refused():
+    """Rows appended behind such a cut would be written into a block that others read."""
+    bm = BlockManager(4, 30)
+    shared_prompt(bm, 24)
+    assert bm.make_private(2, 6)
+    bm.take_copies()
+    for bad in (9, 10, 23):
+        with pytest.raises(KyroError):
+            bm.truncate(2, bad)
+    bm.truncate(2, 20)  # at a block's end: what follows goes to blocks of its own
+    assert bm.append_slots(2, 3)
+    assert bm.block_table[2][5] not in bm.request(2)[0][:5]
+    bm.check()
+    with pytest.raises(KyroError):
+        bm.truncate(2, 11)
+    bm.truncate(2, 8)
+    bm.truncate(2, 7)
+    bm.check()
+
+
+@pytest.mark.parametrize("tokens", [0, 1, 4, 5, 24, 1000])
+def test_make_private_of_so_many_tokens(tokens):
+    bm = BlockManager(4, 30)
+    shared_prompt(bm, 24)
+    before = bm.block_table[2]
+    n = min(6, -(-tokens // 4))
+    assert bm.make_private(2, tokens)
+    assert [s for s, _ in bm.take_copies()] == before[:n] and bm.block_table[2][n:] == before[n:]
+    assert not set(bm.block_table[2][:n]) & set(before)
+    bm.check()
+    with pytest.raises(KyroError):
+        bm.make_private(2, -1)
+    with pytest.raises(KyroError):
+        bm.make_private(77, 4)
+
+
+def test_make_private_front_random_streams():
+    """No block that a request may write, the front ones and the one its next row goes to, has another holder."""
+    rng = np.random.default_rng(6)
+    bm, live, front = BlockManager(4, 60), {}, {}
+    for step in range(600):
+        what = rng.integers(0, 6)
+        if what <= 1 and len(live) < 8:
+            if bm.allocate_with_prefix(step, [int(x) for x in rng.integers(0, 2, rng.integers(1, 24))]):
+                live[step], front[step] = True, 0
+        elif live:
+            rid = int(rng.choice(list(live)))
+            tokens = bm.request(rid)[1]
+            if what == 2:
+                n = int(rng.integers(0, tokens + 2))
+                if bm.make_private(rid, n):
+                    front[rid] = max(front[rid], n)
+            elif what == 3:
+                bm.append_slots(rid, int(rng.integers(0, 6)))
+            elif what == 4:
+                to = int(rng.integers(0, tokens + 1))
+                try:
+                    bm.truncate(rid, to)
+                    front[rid] = min(front[rid], to)
+                except KyroError:
+                    pass
+            else:
+                bm.free(rid, cache_prompt=bool(rng.integers(0, 2)))
+                del live[rid]
+        if rng.integers(0, 2):
+            bm.take_copies()
+        bm.check()
+        for rid in live:
+            blocks, tokens = bm.request(rid)[:2]
+            written = set(blocks[: -(-front[rid] // 4)]) | (set(blocks[tokens // 4:]) if tokens % 4 else set())
+            others = [b for o in live if o != rid for b in bm.block_table[o]]
+            assert not written & set(others)

@@ -674,3 +674,32 @@ def test_padded_batch_without_rows_needs_no_state_row(gpu):
     out = torch.full_like(c["weights"], 7.0)
     kyro_amd.CacheEviction(16, 8, 64, 2).accumulate(**c, out=out)
     assert (out[0] == 7).all() and (out[1, :, :23] != 7).all()
+
+
+def test_evict_with_only_the_front_private(gpu):
+    """A shared prompt of 50 tokens cut to 13: four of its 13 blocks are copied, the others stay shared and are
+    only read, and what the other holder reads is as it was."""
+    bm = kyro_amd.BlockManager(4, 60)
+    prompt = list(range(50))
+    bm.allocate_with_prefix(1, prompt)
+    bm.free(1)
+    for rid in (2, 3):
+        assert bm.allocate_with_prefix(rid, prompt)[1] == 50
+    c = ecase(gpu, [50], bs=4, seed=3)
+    g = torch.Generator().manual_seed(8)
+    for name in ("key_cache", "value_cache"):
+        c[name] = torch.randn(60, 2, 4, 64, generator=g).to(BF16).to(gpu)
+    kyro_amd.copy_blocks(c["key_cache"], c["value_cache"], bm.take_copies())
+    assert bm.make_private(2, 13)
+    copies = bm.take_copies()
+    assert len(copies) == 4
+    kyro_amd.copy_blocks(c["key_cache"], c["value_cache"], copies)
+    bm.write_tables([2], c["block_table"], c["context_lens"])
+    other = bm.block_table[3]
+    assert bm.block_table[2][4:12] == other[4:12]
+    kyro_amd.sync()
+    before = c["key_cache"][other].clone(), c["value_cache"][other].clone()
+    lens = check_evict(c, 13, 2, 3)
+    assert torch.equal(c["key_cache"][other], before[0]) and torch.equal(c["value_cache"][other], before[1])
+    bm.truncate(2, int(lens))
+    bm.check()
