@@ -166,7 +166,8 @@ int evict_setup(const kyro_kv_evict_params* p, kyro::EvictArgs& a, size_t& bytes
     if (p->budget <= 0 || p->sink < 0 || p->recent < 0 || (int64_t)p->sink + p->recent > p->budget)
         return fail(KYRO_EINVAL, "kv_evict: need budget > 0, sink >= 0, recent >= 0 and sink + recent <= budget");
     a.cap = token_cap(p->max_blocks_per_seq, p->block_size, p->max_tokens);
-    if (a.cap > (1 << 30) || (int64_t)p->batch_size * p->num_kv_heads > (1 << 24))
+    // A grid has fewer than 2^32 threads, and a (sequence, kv head) a workgroup of 1024.
+    if (a.cap > (1 << 30) || (int64_t)p->batch_size * p->num_kv_heads >= (1 << 22))
         return fail(KYRO_EUNSUPPORTED, "kv_evict: more tokens or sequences than one launch carries");
     a.B = p->batch_size;
     a.Hkv = p->num_kv_heads;

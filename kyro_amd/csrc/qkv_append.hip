@@ -290,8 +290,12 @@ bool qkv_append_setup(QkvAppendArgs& a) {
     while ((1 << a.lp_shift) < lanes) ++a.lp_shift;
     if (a.lp_shift > 6) return false;
     const int heads = 64 >> a.lp_shift;
-    a.waves_per_row = (a.H + 2 * a.Hkv + heads - 1) / heads;
-    return (long long)a.total_q * a.waves_per_row <= (long long)INT32_MAX - kThreads;
+    const long long all_heads = (long long)a.H + 2ll * a.Hkv;
+    if (all_heads > INT32_MAX - 64) return false;  // the kernel counts them in 32 bits
+    a.waves_per_row = (int)((all_heads + heads - 1) / heads);
+    // A grid has fewer than 2^32 threads.
+    constexpr long long kMaxBlocks = (1ll << 32) / kThreads - 1;
+    return (long long)a.total_q * a.waves_per_row <= kMaxBlocks * (kThreads / 64);
 }
 
 hipError_t launch_qkv_append(const QkvAppendArgs& a, hipStream_t stream) {

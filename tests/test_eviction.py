@@ -291,3 +291,15 @@ def test_make_private_front_random_streams():
             written = set(blocks[: -(-front[rid] // 4)]) | (set(blocks[tokens // 4:]) if tokens % 4 else set())
             others = [b for o in live if o != rid for b in bm.block_table[o]]
             assert not written & set(others)
+
+
+@pytest.mark.parametrize("batch, heads, fits", [(2**22 - 1, 1, True), (2**22, 1, False), (2**20, 3, True), (2**20, 4, False),
+                                                (3, 2**30, False)])
+def test_sequences_and_heads_that_one_launch_carries(batch, heads, fits):
+    """A grid has fewer than 2^32 threads: at most 2^22 - 1 workgroups of 1024."""
+    rc, msg = evict(batch_size=batch, num_state_rows=batch, num_kv_heads=heads, weights=1 << 40, positions=1 << 50,
+                    out_weights=1 << 40, out_positions=1 << 50, context_lens=1 << 30, out_context_lens=2 << 30)
+    if fits:
+        assert rc == _lib.KYRO_EINVAL and "null kyro_ctx" in msg, msg
+    else:
+        assert rc == _lib.KYRO_EUNSUPPORTED and "one launch" in msg, msg

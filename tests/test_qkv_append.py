@@ -170,3 +170,25 @@ def test_row_strides_that_reach_the_library(recorder):
     p = recorder.params
     for stride, heads in ((p.query_stride, 8), (p.key_stride, 2), (p.value_stride, 2)):
         assert stride in (0, heads * 64)
+
+
+FAR = dict(query=1 << 40, key=2 << 40, value=3 << 40, out_query=4 << 40, q_start_loc=13 << 20)
+
+
+@pytest.mark.parametrize("sizes, fits", [
+    # A grid has fewer than 2^32 threads: at most 2^24 - 1 workgroups of four waves. A wave takes a row of 64 heads
+    # of 8 elements (rotary_dim 0), or one head of 256 on 32 lanes.
+    (dict(num_heads=1, num_kv_heads=1, head_dim=8, total_q=2**26 - 4), True),
+    (dict(num_heads=1, num_kv_heads=1, head_dim=8, total_q=2**26 - 3), False),
+    (dict(num_heads=62, num_kv_heads=1, head_dim=8, total_q=2**26 - 4), True),
+    (dict(num_heads=63, num_kv_heads=1, head_dim=8, total_q=2**25), False),
+    # heads that pass 32 bits when they are added up
+    (dict(num_heads=2**29, num_kv_heads=2**29, head_dim=8, total_q=1), True),
+    (dict(num_heads=2**30, num_kv_heads=2**30, head_dim=8, total_q=1), False),
+    (dict(num_heads=2**31 - 1, num_kv_heads=2**31 - 1, head_dim=8, total_q=1), False)])
+def test_what_one_launch_carries(sizes, fits):
+    rc, msg = call(**FAR, rotary_dim=0, cos=None, sin=None, norm=0, q_weight=None, k_weight=None, **sizes)
+    if fits:
+        assert rc == _lib.KYRO_EINVAL and "null kyro_ctx" in msg, msg
+    else:
+        assert rc == _lib.KYRO_EUNSUPPORTED and "one launch" in msg, msg
