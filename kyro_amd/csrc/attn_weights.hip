@@ -14,6 +14,7 @@
 // element 8 (lane / 16), so keys and queries go from memory straight into them, 16 bytes a lane, whatever
 // the block size; the result has the first operand's index in the lane's four registers and the second's
 // in the lane. The f32 caches take 16x16x4 products on 4-element pieces, the same pieces for both operands.
+#include <cfloat>
 #include <type_traits>
 
 #include "common.hpp"
@@ -423,7 +424,13 @@ __global__ __launch_bounds__(kThreads) void few_stats_kernel(AttnWeightsArgs a) 
                     for (int i = 0; i < STEPS; ++i) c[u] = Frag<BF16>::mma(q[nt][i], keys.k[u][i], c[u]);
                     const bool hide = !keys.ok[u];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i][u] = hide ? kNegInf : c[u][i] * a.scale_log2;
+                    for (int i = 0; i < 4; ++i) {
+                        float v = c[u][i] * a.scale_log2;
+                        // A kept -infinity is a score that is not seen. One that is seen stays apart from it:
+                        // a row that has a NaN gives it one.
+                        if constexpr (KEEP) v = v == kNegInf ? -FLT_MAX : v;
+                        x[i][u] = hide ? kNegInf : v;
+                    }
                 }
                 if (t0 + 16 * U - 1 > whole) {
 #pragma unroll
@@ -452,8 +459,12 @@ __global__ __launch_bounds__(kThreads) void few_stats_kernel(AttnWeightsArgs a) 
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float top = row16_max(m[nt][i]);
-                const float sum = row16_sum(l[nt][i] * (m[nt][i] == kNegInf ? 1.f : fast_exp2(m[nt][i] - top)));
+                float top = row16_max(m[nt][i]);
+                float sum = row16_sum(l[nt][i] * (m[nt][i] == kNegInf ? 1.f : fast_exp2(m[nt][i] - top)));
+                if (KEEP && top == -FLT_MAX) {  // no score above -infinity
+                    top = kNegInf;
+                    sum = sum == sum ? 0.f : sum;
+                }
                 if (col == 0) stat[wave][nt * 16 + quad * 4 + i] = make_float2(top, sum);
             }
         __syncthreads();

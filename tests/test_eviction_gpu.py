@@ -703,3 +703,35 @@ def test_evict_with_only_the_front_private(gpu):
     assert torch.equal(c["key_cache"][other], before[0]) and torch.equal(c["value_cache"][other], before[1])
     bm.truncate(2, int(lens))
     bm.check()
+
+
+@pytest.mark.parametrize("n,hkv", [(3, 8), (3, 2), (7, 2), (9, 2), (100, 2), (70, 8)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_row_of_nan_gives_nan_where_it_scores_minus_infinity(gpu, n, hkv, dtype):
+    """Token 5 scores -infinity and token 7 NaN with every row: the softmax of a row is NaN over all it sees, in
+    every form of the kernels, and a row of numbers beside it is not."""
+    c = case(gpu, rows=[n, n], old=[50, 50], H=8, hkv=hkv, D=64, dtype=dtype, seed=n)
+    c["query"][..., 0] = -1
+    for b in range(2):
+        c["key_cache"][c["block_table"][b, 0], :, 5, 0] = float("inf")
+    c["key_cache"][c["block_table"][1, 0], :, 7, 1] = float("nan")
+    c["key_cache"][c["block_table"][1, (49 + n) // 16], :, (49 + n) % 16, 0] = float("inf")  # seen by the last row
+    c["weights"].zero_()
+    out = kyro_amd.CacheEviction(16, 8, 64, hkv).accumulate(**c)
+    assert out[1, :, :50 + n].isnan().all() and out[0].isfinite().all() and (out[0, :, 5] == 0).all()
+
+
+@pytest.mark.parametrize("n,hkv", [(3, 8), (3, 2), (9, 2), (100, 2)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_row_of_minus_infinities_adds_nothing(gpu, n, hkv, dtype):
+    """As one that sees no token: in every form, and beside a sequence of numbers."""
+    c = case(gpu, rows=[n, n], old=[150, 150], H=8, hkv=hkv, D=64, dtype=dtype, seed=n)
+    c["query"][..., 0] = -1
+    c["key_cache"][c["block_table"][1], ..., 0] = float("inf")
+    before = c["weights"].clone()
+    out = kyro_amd.CacheEviction(16, 8, 64, hkv).accumulate(**c)
+    assert torch.equal(out[1, :, :150], before[1, :, :150]) and (out[1, :, 150:150 + n] == 0).all()
+    # The other's rows share out a weight of 1 each, within 2^-24 x 4000 (plain_weights: 136 |q| |k| / 8 + 128 + 400);
+    # adding it to up to 250 weights below 1 and gains rounds each by half a step of a number below 128, 2^-18.
+    gain = out[0].double().sum(-1) - before[0, :, :150].double().sum(-1) - before[0, :, 150 + n:].double().sum(-1)
+    assert ((gain / (n * 8 // hkv) - 1).abs() < 4000 * U + 250 * 2.0 ** -18 / (n * 8 // hkv)).all()
