@@ -735,3 +735,106 @@ def test_a_row_of_minus_infinities_adds_nothing(gpu, n, hkv, dtype):
     # adding it to up to 250 weights below 1 and gains rounds each by half a step of a number below 128, 2^-18.
     gain = out[0].double().sum(-1) - before[0, :, :150].double().sum(-1) - before[0, :, 150 + n:].double().sum(-1)
     assert ((gain / (n * 8 // hkv) - 1).abs() < 4000 * U + 250 * 2.0 ** -18 / (n * 8 // hkv)).all()
+
+
+# ------------------------------------------------------------------------------------ every form of the kernels
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("D", [8, 32, 40, 64, 72, 96, 112, 128, 160, 192, 200, 256])
+def test_head_dims_of_many_rows(gpu, dtype, D):
+    """Rows through LDS: each number of steps a product has, whole rows and padded ones, in parts of the rows and
+    (with more tokens) without, beside sequences of few rows."""
+    check_weights(case(gpu, rows=[75, 3, 0, 33], old=[130, 300, 9, 0], H=8, hkv=2, D=D, dtype=dtype, seed=D))
+    check_weights(case(gpu, rows=[300], old=[77], H=4, hkv=1, D=D, dtype=dtype, seed=D + 1))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("D", [32, 192])
+@pytest.mark.parametrize("n", [1, 3, 8, 16])
+def test_head_dims_of_few_rows(gpu, dtype, D, n):
+    check_weights(case(gpu, rows=[n, 0, n], old=[90, 5, 400], H=8, hkv=2, D=D, dtype=dtype, seed=D + n))
+
+
+def test_many_rows_that_are_not_split(gpu):
+    """Runs of tokens enough for the CUs: the rows of a sum in one part, in place and elsewhere."""
+    for dtype in (BF16, F32):
+        c = case(gpu, rows=[70, 66], old=[20000, 17000], H=8, hkv=8, D=64, dtype=dtype, seed=2)
+        out = torch.full_like(c["weights"], 7.0)
+        kyro_amd.CacheEviction(16, 8, 64, 8).accumulate(**{**c, "positions": c["positions"].clone()}, out=out)
+        got = check_weights(c)
+        for b, n in enumerate(c["context_lens"].tolist()):
+            assert torch.equal(out[b, :, :n], got[b, :, :n]) and (out[b, :, n:] == 7).all()
+
+
+LIMITS = [1024, 4096, 16384, 32768, 65536]  # tokens up to which a selecting thread holds 1, 4, 16, 32 and 64 keys
+
+
+@pytest.mark.parametrize("n", [m for limit in LIMITS for m in (limit, limit + 1)] + [70001])
+@pytest.mark.parametrize("part", [0.43, 0.999, 0.002])
+@pytest.mark.parametrize("elsewhere", [False, True])
+def test_evict_on_both_sides_of_every_form(gpu, n, part, elsewhere):
+    """Few moves, and more than a selecting workgroup makes itself (1024)."""
+    c = ecase(gpu, [n], hkv=1, D=8, seed=n)
+    out = (torch.full_like(c["weights"], -7.0), torch.full_like(c["positions"], -7)) if elsewhere else None
+    budget = int(n * part) + 1
+    check_evict(c, budget, min(4, budget), min(50, budget - min(4, budget)), out=out)
+
+
+@pytest.mark.parametrize("kind", ["ties", "equal", "odd"])
+@pytest.mark.parametrize("n", [4000, 16000, 30000, 60000, 66000])
+def test_evict_ties_and_odd_weights_of_every_form(gpu, kind, n):
+    check_evict(ecase(gpu, [n], hkv=1, D=8, kind=kind, seed=n), n // 3, 2, 5)
+
+
+@pytest.mark.parametrize("width", [300, 1100, 2100, 4200])
+def test_evict_short_contexts_in_wide_tables(gpu, width):
+    """The table's width chooses the kernel, a context's length the form within it."""
+    check_evict(ecase(gpu, [900, 3000, 40, 4700], D=8, width=width, seed=width), 500, 4, 20)
+
+
+def test_evict_many_caches_of_many_moves(gpu):
+    """From 128 caches on the selecting workgroups make up to 1024 moves, and leave the others."""
+    check_evict(ecase(gpu, [6000, 5000] + [10] * 126, hkv=1, D=8, seed=4), 2600, 4, 20)
+    check_evict(ecase(gpu, [6000, 5000] + [10] * 126, hkv=1, D=8, seed=5, dtype=F32, kind="ties"), 2600, 4, 20)
+
+
+@pytest.mark.parametrize("rows,old", [((200, 150), (64, 500)), ((200, 1, 0, 9), (64, 500, 33, 20)), ((300, 300), (3, 5))])
+def test_graphs_of_prompts_replay_as_eager(gpu, rows, old):
+    """The kernels of many rows, their parts, and few rows beside them, captured and replayed with other inputs."""
+    ev = kyro_amd.CacheEviction(16, 8, 128, 2)
+    c = case(gpu, rows=rows, old=old, D=128, seed=1)
+    out = torch.zeros_like(c["weights"])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ev.accumulate_async(**c, max_q_len=max(rows), out=out)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            ev.accumulate_async(**c, max_q_len=max(rows), out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    for turn in range(4):
+        c["query"].copy_(torch.randn(c["query"].shape, device=gpu))
+        c["key_cache"].copy_(torch.randn(c["key_cache"].shape, device=gpu))
+        c["weights"].uniform_()
+        out.fill_(turn)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = torch.full_like(out, turn)
+        ev.accumulate(**{**c, "positions": c["positions"].clone()}, out=eager)
+        assert torch.equal(out, eager)
+
+
+def test_a_verify_step_weighs_its_accepted_rows(gpu):
+    """Every row of a call weighs, so a step that rejects drafts is weighed once its acceptance is known: with the
+    rows that stay, at the lengths that stay. The same as if the rejected rows had never been."""
+    c = case(gpu, rows=[5, 5, 5], old=[100, 7, 40], seed=11)
+    stay = [3, 5, 1]
+    rows = torch.cat([torch.arange(5 * b, 5 * b + n) for b, n in enumerate(stay)]).to(gpu)
+    c["query"] = c["query"][rows]
+    c["q_start_loc"] = torch.tensor([0, 3, 8, 9], dtype=torch.int32, device=gpu)
+    c["context_lens"] -= torch.tensor([2, 0, 4], device=gpu)
+    before = c["weights"].clone()
+    check_weights(c)
+    for b, n in enumerate((103, 12, 41)):
+        assert torch.equal(c["weights"][b, :, n:], before[b, :, n:])
