@@ -59,10 +59,12 @@ typedef struct kyro_attn_weights_params {
  *                            softmax_t(scale * query[j][g] . key[t]) over the tokens row j sees
  * The new tokens are the sequence's last q_len, which the step has appended: their entries start at 0
  * whatever they held (a rejected draft's), and positions[r][h][t] becomes row_positions[row] (NULL: t). A
- * row that sees no token (of a context shorter than its rows, or empty as in a padded batch) adds nothing. A
- * sequence without rows keeps its weights and positions: out_weights gets its weights as they are.
- * Sums and softmax are held in 32 bits; results do not depend on the
- * order of execution. out_weights may be weights itself; otherwise they do not overlap.
+ * row that sees no token (of a context shorter than its rows, or empty as in a padded batch), or scores each it
+ * sees -infinity, adds nothing. A sequence without rows keeps its weights and positions: out_weights gets its
+ * weights as they are. Every row of the call weighs: after a verify step that may reject drafts, call it once
+ * acceptance is known, with the query rows that stay (and their q_start_loc) and the context lengths that stay,
+ * or older tokens keep the weight that rejected rows gave them. Sums and softmax are held in 32 bits; results do
+ * not depend on the order of execution. out_weights may be weights itself; otherwise they do not overlap.
  *   query [total_q, H, D] dtype, q_start_loc, key_cache, block_table, context_lens: as for
  *     kyro_paged_attention_mq, after kyro_paged_kv_append or kyro_qkv_append has written the rows
  *   row_positions [total_q] int64 or NULL, state_rows [B] int32 or NULL (then B <= num_state_rows)

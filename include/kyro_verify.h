@@ -400,7 +400,8 @@ typedef struct kyro_qkv_append_params {
  * the new rows. For row j of sequence b (rows as for kyro_paged_kv_append, its slot p = context_lens[b]
  * - q_len + j):
  *   queries and keys, each head x: with norm, x <- x * (w + weight_offset) / sqrt(mean(x^2) + eps)
- *     (w = 1 without weights); then with angle row t = positions[row] (NULL: t = p) of cos and sin,
+ *     (without weights x / sqrt(mean(x^2) + eps), whatever weight_offset is); then with angle row
+ *     t = positions[row] (NULL: t = p) of cos and sin,
  *     (x_i, x_i') <- (x_i cos[t][i] - x_i' sin[t][i], x_i' cos[t][i] + x_i sin[t][i]) for i < R/2;
  *   out_query [total_q, H, D] gets the queries, the caches' slots the keys and the values.
  * In 32 bits (the sum of squares too: a head's must stay below 3.4e38), rounded once to cache_dtype (to

@@ -976,7 +976,8 @@ void launch_type(const AttnWeightsArgs& a, hipStream_t stream) {
         case 256: return launch_steps<BF16, 8, true>(a, stream);
         default: break;
     }
-    // Others take the next of three sizes, with zeros behind their last element.
+    // Others take the next of three sizes, with zeros behind their last element: fewer kernels to build, not the
+    // fastest (2 x 512 rows at 8192 tokens, 32/8 heads: 330 us at 136, where 192 takes 264; 198 at 72, 169 at 96).
     if (a.D < 64) return launch_steps<BF16, 2, false>(a, stream);
     if (a.D < 128) return launch_steps<BF16, 4, false>(a, stream);
     launch_steps<BF16, 8, false>(a, stream);

@@ -10,11 +10,14 @@
 //
 // evict_select_kernel: one workgroup a (sequence, kv head). Weights and positions are read once, 8 bytes a
 // token (the positions a second time past 16 keys a thread), and the keys stay in registers, thread i holding
-// slots i, i + 1024, .., for the three passes over 11, 11 and 10 bits. The first digit holds the sign, the exponent and two bits of the mantissa, so weights
-// that fall over many octaves spread over its bins. Ballots give each token its rank in slot order; the
-// workgroup then copies its own K and V rows, up to kOwnMoves of them. evict_move_kernel: the rest, by
-// many workgroups, where a call may have that many. Contexts past the registers read their keys again.
-// What bounds it: latency (a dozen barriers, some five dependent loads) for few tokens, HBM for many moves.
+// slots i, i + 1024, .., for the three passes over 11, 11 and 10 bits (with 64 of them, past 32768 tokens, 151
+// registers are spilled to scratch, and 1 with 32). The first digit holds the sign, the exponent and two bits of
+// the mantissa, so weights that fall over many octaves spread over its bins. Ballots give each token its rank in
+// slot order; the workgroup then copies its own K and V rows, up to kOwnMoves of them. evict_move_kernel: the
+// rest, by many workgroups, where a call may have that many. Contexts past the registers read their keys again.
+// What bounds it: latency (a dozen barriers, some five dependent loads) for few tokens, HBM for many moves, the
+// one CU that selects for a (sequence, kv head) for long contexts (8 heads cut to a fifth: 27606 tokens 58 us,
+// 52160 136 us, 131072, whose keys are read again for every pass, 444 us).
 #include "common.hpp"
 #include "kernels.hpp"
 
@@ -143,7 +146,7 @@ __device__ __forceinline__ int select(const EvictArgs& a, int b, Unit u, Shared&
             for (int r = 0; r < kHeld; ++r) {
                 const int t = min(r * kSelThreads + tid, u.n - 1);
                 key[r] = u.key(u.pos[t], u.w[t]);
-                // A part at a time: else all the loads come first, and spill.
+                // A part at a time, so that not all the loads come first: the keys fill the registers as it is.
                 if (r % (R == 32 ? 16 : 8) == (R == 32 ? 15 : 7)) __builtin_amdgcn_sched_barrier(0);
             }
         }

@@ -152,9 +152,11 @@ class CacheEviction:
         ``query``'s rows (the arguments of :meth:`kyro_amd.PagedAttention.forward`, after the append), summed over
         the rows and over each kv head's query heads, and returns them. The step's own new tokens start from
         zero, and their entries of ``positions`` (int32, like weights) become ``row_positions`` (int64
-        [total_q]; None: the slots). ``state_rows`` (int32 [B]) names the rows of weights and positions that the
-        sequences own; by default sequence b owns row b. ``out`` receives the weights of every sequence's tokens
-        (of one without rows as they are) instead of weights itself; its other entries stay. The call synchronises, so errors the device detects raise KyroError here."""
+        [total_q]; None: the slots). Every row weighs: after a verify step call it once acceptance is known, with
+        the rows and context lengths that stay. ``state_rows`` (int32 [B]) names the rows of weights and positions
+        that the sequences own; by default sequence b owns row b. ``out`` receives the weights of every sequence's
+        tokens (of one without rows as they are) instead of weights itself; its other entries stay. The call
+        synchronises, so errors the device detects raise KyroError here."""
         out = self.accumulate_async(query, key_cache, block_table, context_lens, weights, positions,
                                     q_start_loc=q_start_loc, max_q_len=max_q_len, row_positions=row_positions,
                                     state_rows=state_rows, causal=causal, scale=scale, out=out)
