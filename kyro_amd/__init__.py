@@ -15,6 +15,7 @@ acceptance, and the paged KV write. This package is the Python host mirror of th
         (no counterpart: caches held to a budget by accumulated attention weight)
     BlockManager(block_size, num_gpu_blocks, num_cpu_blocks), RadixCache(max_capacity)
         (src/scheduler/block_manager.rs, src/scheduler/radix_cache.rs) and the device tables
+    RequestTables(...).extend(...) / .keep(...)  the same tables built on the GPU, accepted lengths included
     sample_tokens(...)  (src/worker.rs:141-197 logit processors, then sample_token :267-362)
     NgramTable(corpus, order).draft(...)  (src/speculative.rs:196-256, the Ngram draft strategy)
 """
@@ -24,10 +25,11 @@ from .block_manager import BlockManager, RadixCache, copy_blocks
 from .drafting import NgramTable, context_tails
 from .eviction import CacheEviction
 from .kv_cache import PagedKVCache, rope_tables
+from .request_tables import RequestTables, StepTables
 from .sampling import grammar_mask, penalty_adds, sample_token, sample_tokens, sample_tokens_async
 from .speculative import VerifyResult, verify_drafts, verify_drafts_async
 
-__all__ = ["BlockManager", "CacheEviction", "Context", "KyroError", "NgramTable", "PagedAttention", "PagedKVCache", "RadixCache",
+__all__ = ["BlockManager", "CacheEviction", "Context", "KyroError", "NgramTable", "PagedAttention", "PagedKVCache", "RadixCache", "RequestTables", "StepTables",
            "context_tails",
            "VerifyResult", "context", "copy_blocks", "grammar_mask", "lib", "penalty_adds", "rope_tables", "sample_token",
            "sample_tokens", "sample_tokens_async",

@@ -89,6 +89,12 @@ class KvEvictParams(ctypes.Structure):
         "sink", "recent", "num_state_rows", "max_tokens")]
 
 
+class TablesParams(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "block_size", "batch_size", "max_blocks_per_seq", "num_state_rows", "max_state_blocks", "num_blocks",
+        "pool_capacity", "max_rows", "kept_plus")]
+
+
 class CopyBlocksParams(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("block_size", "num_kv_heads", "head_dim", "num_blocks", "dtype")]
 
@@ -119,8 +125,9 @@ def packer(cls):
 pack_qkv_append = packer(QkvAppendParams)
 pack_attn_weights = packer(AttnWeightsParams)
 pack_kv_evict = packer(KvEvictParams)
+pack_tables = packer(TablesParams)
 
-ABI_VERSION = 11  # KYRO_ABI_VERSION of include/kyro_verify.h
+ABI_VERSION = 12  # KYRO_ABI_VERSION of include/kyro_verify.h
 
 _lib = None
 _lib_lock = threading.Lock()
@@ -185,6 +192,11 @@ _SIGNATURES = {
                                      ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
     "kyro_kv_evict": ([_P, _P] + [_P] * 10, ctypes.c_int),
     "kyro_kv_evict_workspace": ([ctypes.POINTER(KvEvictParams), ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
+    # include/kyro_tables.h
+    "kyro_tables_extend": ([_P, _P] + [_P] * 11, ctypes.c_int),
+    "kyro_tables_keep": ([_P, _P] + [_P] * 9, ctypes.c_int),
+    "kyro_tables_release": ([_P, _P] + [_P] * 5, ctypes.c_int),
+    "kyro_tables_workspace": ([_P, ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
     # include/kyro_sample.h
     "kyro_sample_tokens": ([_P, ctypes.POINTER(SampleParams)] + [_P] * 14, ctypes.c_int),
     "kyro_penalty_adds": ([_P, ctypes.c_int64, ctypes.c_float, ctypes.c_float, ctypes.c_int32, _P, _P,

@@ -16,7 +16,11 @@ enum ErrorBits : int {
     ERR_NO_DRAFT = 32,  // a sampled sequence with drafts but no draft_logits
     ERR_PLAN = 64,      // balanced attention schedule: more partial-state slots than the host sized
     ERR_POSITION = 128, // a row's position outside [0, max_position)
-    ERR_STATE_ROW = 256 // a state row outside [0, num_state_rows), or named by two sequences
+    ERR_STATE_ROW = 256, // a state row outside [0, num_state_rows), or named by two sequences
+    ERR_REQUEST = 512,  // tables: a request's record whose numbers do not fit each other
+    ERR_POOL = 1024,    // tables: pool_count outside [0, pool_capacity], or blocks that would pass it
+    ERR_NO_BLOCKS = 2048, // tables: the pool has too few blocks (KYRO_ENOSPACE)
+    ERR_GROUPS = 4096   // shared attention: group_starts not monotone or out of range, or group_blocks out of range
 };
 
 
@@ -417,6 +421,43 @@ struct EvictArgs {
 };
 
 hipError_t launch_kv_evict(const EvictArgs& a, hipStream_t stream);
+
+// Block tables and slots of a step (tables.hip).
+constexpr int kTablesEntryBytes = 32;
+struct alignas(16) TablesEntry {
+    char bytes[kTablesEntryBytes];
+};
+constexpr int kTablesMaxRows = 131072;  // requests of a state: two bits each in LDS
+// Batches whose tables have up to so many entries and whose rows are up to so many are one launch.
+constexpr int kTablesOneEntries = 16384;
+constexpr int kTablesOneRows = 4096;
+struct TablesArgs {
+    const int32_t* state_rows;  // [B] or nullptr
+    const int32_t* new_rows;    // extend
+    int4* requests;             // [num_rows] {tokens, held, shared, -}
+    int64_t* blocks;            // [num_rows, state_blocks]
+    const int64_t* pool;        // extend
+    int64_t* pool_out;          // keep, release
+    int* pool_count;
+    int64_t* table;             // extend: [B, width]
+    int64_t* ctx_lens;          // [B]: extend's output, keep's input
+    int64_t* out_ctx;           // keep
+    int32_t* q_start;           // [B + 1]: extend's output, keep's input
+    int64_t* positions;         // [max_rows] or nullptr
+    int64_t* slots;
+    const int32_t* kept;        // keep
+    TablesEntry* entries;       // [B] scratch
+    int* err;
+    int64_t table_wgs;
+    int B, num_rows, state_blocks, width, bs, bs_shift, num_blocks, pool_cap, max_rows, kept_plus;
+};
+
+// Workgroups of the launches beside the scan.
+int64_t tables_fill_wgs(const TablesArgs& a, int64_t& table_wgs);
+int64_t tables_free_wgs(const TablesArgs& a);
+hipError_t launch_tables_extend(const TablesArgs& a, hipStream_t stream);
+hipError_t launch_tables_keep(const TablesArgs& a, hipStream_t stream);
+hipError_t launch_tables_release(const TablesArgs& a, hipStream_t stream);
 
 // Whole-block copies within a cache pair (copy-on-write of a prefix block).
 constexpr int kCopyInline = 240;  // block pairs passed in the kernel arguments (2 x 240 x 4 B)

@@ -146,7 +146,11 @@ int sync_and_report(kyro_ctx ctx) {
                "(internal error; no item ran);";
     if (err & kyro::ERR_STATE_ROW) msg += " a state row outside [0, num_state_rows) or named by two sequences;";
     if (err & kyro::ERR_POSITION) msg += " a position outside [0, max_position);";
-    return fail(KYRO_EINVAL, "%s", msg.c_str());
+    if (err & kyro::ERR_REQUEST) msg += " a request's record whose numbers do not fit each other;";
+    if (err & kyro::ERR_POOL) msg += " pool_count outside [0, pool_capacity], or more blocks than the pool holds;";
+    if (err & kyro::ERR_GROUPS) msg += " group_starts not monotone / out of range, or group_blocks out of range;";
+    if (err & kyro::ERR_NO_BLOCKS) msg += " not enough free blocks in the pool;";
+    return fail(err == kyro::ERR_NO_BLOCKS ? KYRO_ENOSPACE : KYRO_EINVAL, "%s", msg.c_str());
 }
 
 }  // namespace
