@@ -251,6 +251,34 @@ int kyro_paged_attention_plan(const kyro_paged_attention_params* params, int num
                               const int64_t* context_lens, const int32_t* q_lens, int32_t* out_splits,
                               kyro_attention_plan* out);
 
+/* ---------------------------------------------------------------- attention over shared prefixes */
+
+/*
+ * kyro_paged_attention_mq for a batch whose sequences come in groups that hold the same first blocks (a system
+ * prompt, a document, the prompt that several samples continue): the groups' common tokens are read and multiplied
+ * once for all rows of a group, not once a sequence. The same arguments and results, but for rounding, and
+ *   group_starts [num_groups + 1] int32: the sequences of group g are [group_starts[g], group_starts[g+1]);
+ *     sequences of no group, and those before the first and behind the last, share nothing
+ *   group_blocks [num_groups] int32: the leading blocks that the tables of all its sequences have in common (0: none).
+ *     The table of its first sequence is read for them: that the others' are the same is the caller's to see to
+ *     (kyro_bm_prefix_groups finds groups so).
+ * Groups are ranges of the batch, so its sequences are to be ordered by prefix. A sequence whose context does not
+ * reach past its group's common tokens with every row (with causal, ctx - q_len + 1 of them) reads its own table
+ * instead, and a group whose common tokens are not worth a pass of their own is computed as if it had none. params
+ * as for kyro_paged_attention_mq, with path and schedule AUTO and num_splits 0. Geometries that the kernel for many
+ * query rows does not take (block sizes that are no multiple of 16, other head dims, caches off a 16-byte boundary)
+ * run as kyro_paged_attention_mq runs them, with the groups unread. Groups out of range or order
+ * latch KYRO_EINVAL for the next kyro_sync, and the sequences are computed without them.
+ */
+int kyro_paged_attention_shared(kyro_ctx ctx, const kyro_paged_attention_params* params, int32_t num_groups,
+                                const void* query, const int32_t* q_start_loc, const void* key_cache,
+                                const void* value_cache, const int64_t* block_table, const int64_t* context_lens,
+                                const int32_t* group_starts, const int32_t* group_blocks, void* out);
+
+/* Scratch bytes such a call takes at most from the context's arena, as kyro_paged_attention_workspace. */
+int kyro_paged_attention_shared_workspace(kyro_ctx ctx, const kyro_paged_attention_params* params, int has_q_start_loc,
+                                          int32_t num_groups, size_t* bytes);
+
 /* ---------------------------------------------------------------- speculative verify */
 
 typedef struct kyro_spec_verify_params {

@@ -153,6 +153,9 @@ _SIGNATURES = {
                                         ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
     "kyro_paged_attention_plan": ([ctypes.POINTER(PagedAttentionParams), ctypes.c_int, ctypes.c_int, _P, _P, _P,
                                    ctypes.POINTER(AttentionPlan)], ctypes.c_int),
+    "kyro_paged_attention_shared": ([_P, ctypes.POINTER(PagedAttentionParams), ctypes.c_int32] + [_P] * 9, ctypes.c_int),
+    "kyro_paged_attention_shared_workspace": ([_P, ctypes.POINTER(PagedAttentionParams), ctypes.c_int, ctypes.c_int32,
+                                               ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
     "kyro_spec_verify": ([_P, ctypes.POINTER(SpecVerifyParams)] + [_P] * 11, ctypes.c_int),
     "kyro_spec_verify_noalloc": ([_P, ctypes.POINTER(SpecVerifyParams)] + [_P] * 11, ctypes.c_int),
     "kyro_spec_verify_workspace": ([ctypes.POINTER(SpecVerifyParams), ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),

@@ -241,6 +241,7 @@ struct PrefillArgs {
     int tile_tokens;  // prefill_tile_tokens
     int slots;        // workgroups the device runs at once
     int split_cost;   // tiles a workgroup computes in the time that parking and merging one part takes
+    int tail_waves;   // shared attention: wave slots of a part of a sequence's own tokens
 };
 
 // Without a list: tiles of a part of a sequence's row groups, from the sequence's own context, which the
@@ -254,6 +255,24 @@ __host__ __device__ inline int prefill_part_tiles(const PrefillArgs& p, int ctx)
 }
 
 hipError_t launch_attention_prefill(const PrefillArgs& p, hipStream_t stream);
+
+// Attention for sequences that share prefixes (shared_attention.hip): the many-row kernel over a list that has
+// each group's common tokens once, against the rows of the whole group, and each sequence's own tokens.
+constexpr int kSharedAll = 1 << 30;  // in an entry's tiles: common tokens, which every row sees
+struct SharedArgs {
+    PrefillArgs f;                  // list {b, q0, q_len, ctx}, {first row, first tile, tiles | kSharedAll, wave slot or -1};
+                                    // comb {q0, q_len, first row, its row in the group}, {own wave slot, own parts,
+                                    // common wave slot, common parts}
+    const int32_t* group_starts;    // [G + 1]
+    const int32_t* group_blocks;    // [G]
+    int4* seqs;                     // [B] {q0, q_len, ctx, group or -1}
+    int4* groups;                   // [G] {first row, rows, common tiles, first common part}
+    int2* counts;                   // [G] {sequences, their row groups}
+    int G;
+    int common_cap, tail_cap;       // parts of common and of own tokens that the workspace holds
+    int comb_cap;
+};
+hipError_t launch_attention_shared(const SharedArgs& s, hipStream_t stream);
 
 // The bf16 MFMA kernel at head dims 64, 80, 96 and 256, and at 112, 160, 192 and 224 (a
 // translation unit each).

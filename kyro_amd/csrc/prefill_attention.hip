@@ -158,7 +158,11 @@ struct PfState {
 
 // POL: cache policy of the K/V copies. Streaming where no other row group reads the slabs (a verify
 // step's 72 rows per kv head, 64 sequences of 4096 tokens: 201 us with cached loads, 178 us so).
-template <bool BF16, int DR, int POL>
+//
+// SHARED: the list is that of shared_attention.hip. Its entries are row groups over a part of the context: of a
+// sequence from its group's common tokens on, or (kSharedAll) of a whole group's rows over the common tokens, all of
+// which see them all. A part's state goes to wave slots of its own (e1.w).
+template <bool BF16, int DR, int POL, bool SHARED = false>
 __global__ __launch_bounds__(kPfThreads, prefill_wgs_per_cu(BF16, DR)) void attn_prefill_kernel(PrefillArgs p) {
     using C = PfCfg<BF16, DR>;
     const AttnArgs& a = p.a;
@@ -170,7 +174,7 @@ __global__ __launch_bounds__(kPfThreads, prefill_wgs_per_cu(BF16, DR)) void attn
     const int entry = (int)blockIdx.x / a.Hkv;
     const int kvh = (int)blockIdx.x - entry * a.Hkv;
     int4 e0, e1;
-    if (p.list) {
+    if (SHARED || p.list) {
         if (entry >= p.head[0]) return;
         e0 = p.list[2 * entry];
         e1 = p.list[2 * entry + 1];
@@ -193,7 +197,9 @@ __global__ __launch_bounds__(kPfThreads, prefill_wgs_per_cu(BF16, DR)) void attn
     const int ctx = __builtin_amdgcn_readfirstlane(e0.w);
     const int row0 = __builtin_amdgcn_readfirstlane(e1.x);
     const int tile0 = __builtin_amdgcn_readfirstlane(e1.y);
-    const int nt = __builtin_amdgcn_readfirstlane(e1.z);
+    const int nt = __builtin_amdgcn_readfirstlane(SHARED ? e1.z & ~kSharedAll : e1.z);
+    const bool common = SHARED && (__builtin_amdgcn_readfirstlane(e1.z) & kSharedAll);
+    const bool causal = a.causal && !common;
     const int part = __builtin_amdgcn_readfirstlane(e1.w);
     SeqInfo si;
     si.b = b;
@@ -209,13 +215,13 @@ __global__ __launch_bounds__(kPfThreads, prefill_wgs_per_cu(BF16, DR)) void attn
     const int h = lane >> 5;
     const int wrow0 = row0 + 32 * wave;  // the wave's first row
     const bool active = wrow0 < si.rows;
-    const int past = a.causal ? ctx - q_len + 1 : ctx;  // tokens row 0 of the sequence sees
+    const int past = causal ? ctx - q_len + 1 : ctx;  // tokens row 0 of the sequence sees
     const int n = wrow0 + col;
     // Rows past the unit take Q = 0 and every token; they are never stored.
-    const int vis = n < si.rows ? (a.causal ? past + n / a.group : ctx) : ctx;
-    const int wave_lo = a.causal ? past + wrow0 / a.group : ctx;
-    const int wave_hi = a.causal ? past + min(wrow0 + 31, si.rows - 1) / a.group : ctx;
-    const int wg_hi = a.causal ? past + min(row0 + kPrefillRows - 1, si.rows - 1) / a.group : ctx;
+    const int vis = n < si.rows ? (causal ? past + n / a.group : ctx) : ctx;
+    const int wave_lo = causal ? past + wrow0 / a.group : ctx;
+    const int wave_hi = causal ? past + min(wrow0 + 31, si.rows - 1) / a.group : ctx;
+    const int wg_hi = causal ? past + min(row0 + kPrefillRows - 1, si.rows - 1) / a.group : ctx;
     const int nslots = (max(wg_hi, 0) + kPfBS - 1) / kPfBS;  // slots the row group sees
     const float c = a.scale_log2;
 
@@ -521,7 +527,8 @@ __global__ __launch_bounds__(kPfThreads, prefill_wgs_per_cu(BF16, DR)) void attn
         return;
     }
     // A part's state: m and l by row, O^T in the order the lanes hold it (whole 1 KiB stores).
-    const size_t wv = ((size_t)part * a.Hkv + kvh) * kPfWaves + wave;
+    const size_t wv = SHARED ? (size_t)part + (size_t)kvh * (common ? kPfWaves : p.tail_waves) + wave
+                             : ((size_t)part * a.Hkv + kvh) * kPfWaves + wave;
     if constexpr (!BF16) {
         // Relative to the rounded scaled maximum that the merge weighs parts by.
         const float m = st.m * c;
@@ -543,6 +550,7 @@ __global__ __launch_bounds__(kPfThreads, prefill_wgs_per_cu(BF16, DR)) void attn
                 make_float4(st.o[dt][4 * k], st.o[dt][4 * k + 1], st.o[dt][4 * k + 2], st.o[dt][4 * k + 3]);
 }
 
+#if KYRO_PREFILL_UNIT < 3
 // Merges the split row groups: a workgroup takes one 32-column tile of one (split row group, kv
 // head), a lane the 16 columns of its row that it held in the first pass.
 template <int DR>
@@ -648,6 +656,15 @@ void launch_prefill_dim(const PrefillArgs& p, hipStream_t stream) {
         attn_prefill_combine_kernel<DR><<<dim3((unsigned)(units < kMaxGrid ? units : kMaxGrid)), kPfThreads, 0, stream>>>(p);
     }
 }
+
+#else
+template <bool BF16, int DR>
+void launch_shared_dim(const PrefillArgs& p, hipStream_t stream) {
+    const dim3 grid((unsigned)((long long)p.list_cap * p.a.Hkv));
+    if (p.a.stream_kv) attn_prefill_kernel<BF16, DR, kLoadStream, true><<<grid, kPfThreads, 0, stream>>>(p);
+    else attn_prefill_kernel<BF16, DR, kLoadCached, true><<<grid, kPfThreads, 0, stream>>>(p);
+}
+#endif
 
 #if KYRO_PREFILL_UNIT == 0
 // ------------------------------------------------------------------------------------- plan
@@ -821,7 +838,7 @@ hipError_t launch_prefill_wide(const PrefillArgs& p, hipStream_t stream) {
     }
     return hipGetLastError();
 }
-#else
+#elif KYRO_PREFILL_UNIT == 2
 hipError_t launch_prefill_f32(const PrefillArgs& p, hipStream_t stream) {
     switch (p.a.D) {
         case 64: launch_prefill_dim<false, 64>(p, stream); break;
@@ -829,6 +846,41 @@ hipError_t launch_prefill_f32(const PrefillArgs& p, hipStream_t stream) {
         case 96: launch_prefill_dim<false, 96>(p, stream); break;
         case 112: launch_prefill_dim<false, 112>(p, stream); break;
         case 128: launch_prefill_dim<false, 128>(p, stream); break;
+        default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+#elif KYRO_PREFILL_UNIT == 3
+hipError_t launch_shared_bf16(const PrefillArgs& p, hipStream_t stream) {
+    switch (p.a.D) {
+        case 64: launch_shared_dim<true, 64>(p, stream); break;
+        case 80: launch_shared_dim<true, 80>(p, stream); break;
+        case 96: launch_shared_dim<true, 96>(p, stream); break;
+        case 112: launch_shared_dim<true, 112>(p, stream); break;
+        case 128: launch_shared_dim<true, 128>(p, stream); break;
+        default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+#elif KYRO_PREFILL_UNIT == 4
+hipError_t launch_shared_wide(const PrefillArgs& p, hipStream_t stream) {
+    switch (p.a.D) {
+        case 160: launch_shared_dim<true, 160>(p, stream); break;
+        case 192: launch_shared_dim<true, 192>(p, stream); break;
+        case 224: launch_shared_dim<true, 224>(p, stream); break;
+        case 256: launch_shared_dim<true, 256>(p, stream); break;
+        default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+#else
+hipError_t launch_shared_f32(const PrefillArgs& p, hipStream_t stream) {
+    switch (p.a.D) {
+        case 64: launch_shared_dim<false, 64>(p, stream); break;
+        case 80: launch_shared_dim<false, 80>(p, stream); break;
+        case 96: launch_shared_dim<false, 96>(p, stream); break;
+        case 112: launch_shared_dim<false, 112>(p, stream); break;
+        case 128: launch_shared_dim<false, 128>(p, stream); break;
         default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

@@ -566,6 +566,90 @@ void attention_workspace(AttnSetup& s, char* base) {
     }
 }
 
+// What a kyro_paged_attention_shared launch decides from its params alone, for caches on 16-byte boundaries. `takes`:
+// whether the kernel over shared prefixes does; s.a is what attention_setup made of the params.
+struct SharedSetup {
+    kyro::SharedArgs s{};
+    bool takes = false;
+    size_t part_rows = 0;  // rows of partial state
+    size_t ws_bytes = 0;
+};
+
+SharedSetup shared_setup(const kyro_paged_attention_params* p, int num_cus, int num_groups, const AttnSetup& from) {
+    SharedSetup r;
+    const bool bf16 = p->dtype == KYRO_BF16;
+    if (from.empty || num_groups == 0 || p->block_size % 16 != 0 || !kyro::prefill_head_dim(p->head_dim, bf16) ||
+        (long long)p->num_blocks * p->num_kv_heads * (p->block_size / 16) >= (1ll << 31) ||
+        (long long)p->max_blocks_per_seq * p->block_size >= (1ll << 30))
+        return r;
+    kyro::SharedArgs& s = r.s;
+    kyro::PrefillArgs& f = s.f;
+    kyro::AttnArgs& a = f.a;
+    a = from.a;
+    a.ubs = 16;
+    a.sub = a.bs / 16;
+    a.rows_per_group = kyro::kPrefillRows;
+    a.row_groups = (int)(((long long)a.rows_cap + kyro::kPrefillRows - 1) / kyro::kPrefillRows);
+    a.plan = 0;
+    a.stream_kv = 0;
+    f.tile_tokens = kyro::prefill_tile_tokens(bf16, a.D);
+    f.slots = kyro::prefill_wgs_per_cu(bf16, a.D) * num_cus;
+    f.split_cost = bf16 ? 6 : 2;
+    f.tail_waves = (std::min(a.rows_cap, kyro::kPrefillRows) + 31) / 32;
+    s.G = num_groups;
+    const long long all = (long long)a.B * a.row_groups, rows = (long long)a.total_q * a.group / kyro::kPrefillRows;
+    const long long own = std::min(all, rows + a.B), common = rows + num_groups;
+    const long long split = f.slots / a.Hkv + 1;  // parts beyond one each: the share is at least a slot's
+    const long long waves = a.Hkv * ((common + split) * 4 + (own + split) * f.tail_waves);
+    if (all > INT32_MAX || waves > INT32_MAX || (own + common + split) * a.Hkv * 256 > 0xffffffffLL) return r;
+    s.common_cap = (int)(common + split);
+    s.tail_cap = (int)(own + split);
+    s.comb_cap = (int)own;
+    f.list_cap = (int)(own + common + split);
+    f.part_cap = 0;
+    r.part_rows = (size_t)waves * 32;
+    r.ws_bytes = 256 + align_up((size_t)f.list_cap * 2 * sizeof(int4), 256) + align_up((size_t)s.comb_cap * 2 * sizeof(int4), 256) +
+                 align_up((size_t)a.B * sizeof(int4), 256) + align_up((size_t)s.G * sizeof(int4), 256) +
+                 align_up((size_t)s.G * sizeof(int2), 256) + 2 * align_up(r.part_rows * sizeof(float), 256) +
+                 r.part_rows * ((size_t)(a.D + 31) / 32 * 32) * sizeof(float);
+    r.takes = true;
+    return r;
+}
+
+void shared_workspace(SharedSetup& r, char* base) {
+    kyro::SharedArgs& s = r.s;
+    auto take = [&](size_t bytes) -> void* {
+        void* x = base;
+        base += align_up(bytes, 256);
+        return x;
+    };
+    s.f.head = static_cast<int*>(take(256));
+    s.f.list = static_cast<int4*>(take((size_t)s.f.list_cap * 2 * sizeof(int4)));
+    s.f.comb = static_cast<int4*>(take((size_t)s.comb_cap * 2 * sizeof(int4)));
+    s.seqs = static_cast<int4*>(take((size_t)s.f.a.B * sizeof(int4)));
+    s.groups = static_cast<int4*>(take((size_t)s.G * sizeof(int4)));
+    s.counts = static_cast<int2*>(take((size_t)s.G * sizeof(int2)));
+    s.f.a.ws_m = static_cast<float*>(take(r.part_rows * sizeof(float)));
+    s.f.a.ws_l = static_cast<float*>(take(r.part_rows * sizeof(float)));
+    s.f.a.ws_acc = static_cast<float*>(take(0));
+}
+
+// The checks that kyro_paged_attention_shared makes beside those of attention_setup.
+int shared_check(const kyro_paged_attention_params* p, int32_t num_groups) {
+    if (!p) return fail(KYRO_EINVAL, "paged_attention_shared: params is null");
+    if (num_groups < 0) return fail(KYRO_EINVAL, "paged_attention_shared: num_groups %d is negative", num_groups);
+    if (p->path != KYRO_ATTN_AUTO || p->schedule != KYRO_ATTN_SCHEDULE_AUTO || p->num_splits != 0)
+        return fail(KYRO_EINVAL, "paged_attention_shared: path and schedule must be AUTO and num_splits 0");
+    return KYRO_OK;
+}
+
+// The params of the launch that takes a call in its place.
+kyro_paged_attention_params unshared_params(const kyro_paged_attention_params* p) {
+    kyro_paged_attention_params q = *p;
+    if (q.kv_reuse == KYRO_KV_REUSE_AUTO) q.kv_reuse = KYRO_KV_REUSE_SHARED;
+    return q;
+}
+
 // Everything a verify launch decides from its params alone: validation, chunking, window,
 // tail grid and workspace size. No device call.
 struct SpecSetup {
@@ -910,6 +994,61 @@ int kyro_paged_attention_workspace(kyro_ctx ctx, const kyro_paged_attention_para
                 return rc;
             *bytes = std::max(*bytes, other.ws_bytes);
         }
+        return KYRO_OK;
+    });
+}
+
+int kyro_paged_attention_shared(kyro_ctx ctx, const kyro_paged_attention_params* p, int32_t num_groups,
+                                const void* query, const int32_t* q_start_loc, const void* key_cache,
+                                const void* value_cache, const int64_t* block_table, const int64_t* context_lens,
+                                const int32_t* group_starts, const int32_t* group_blocks, void* out) {
+    return guarded([&]() -> int {
+        if (int rc = shared_check(p, num_groups)) return rc;
+        AttnSetup from;
+        if (int rc = attention_setup(p, q_start_loc != nullptr, ctx ? ctx->num_cus : kDefaultCUs, from)) return rc;
+        if (from.empty) return check_ctx(ctx);
+        if (!query || !key_cache || !value_cache || !block_table || !context_lens || !out ||
+            (num_groups > 0 && (!group_starts || !group_blocks)))
+            return fail(KYRO_EINVAL, "paged_attention_shared: null device pointer");
+        if (int rc = check_ctx(ctx)) return rc;  // last, so that a host without a device can have the rest checked
+        SharedSetup r = shared_setup(p, ctx->num_cus, num_groups, from);
+        const bool aligned = ((reinterpret_cast<uintptr_t>(key_cache) | reinterpret_cast<uintptr_t>(value_cache)) & 15) == 0;
+        if (!r.takes || !aligned) {
+            const kyro_paged_attention_params plain = unshared_params(p);
+            return kyro_paged_attention_mq(ctx, &plain, query, q_start_loc, key_cache, value_cache, block_table, context_lens, out);
+        }
+        DeviceGuard dg(ctx->device);
+        KYRO_HIP(dg.status);
+        if (int rc = ensure_arena(ctx, r.ws_bytes)) return rc;
+        shared_workspace(r, static_cast<char*>(ctx->arena));
+        kyro::AttnArgs& a = r.s.f.a;
+        a.q = query;
+        a.q_start = q_start_loc;
+        a.k = key_cache;
+        a.v = value_cache;
+        a.table = block_table;
+        a.ctx_lens = context_lens;
+        a.out = out;
+        a.err = ctx->err;
+        r.s.group_starts = group_starts;
+        r.s.group_blocks = group_blocks;
+        KYRO_HIP(kyro::launch_attention_shared(r.s, ctx->stream));
+        return KYRO_OK;
+    });
+}
+
+int kyro_paged_attention_shared_workspace(kyro_ctx ctx, const kyro_paged_attention_params* p, int has_q_start_loc,
+                                          int32_t num_groups, size_t* bytes) {
+    return guarded([&]() -> int {
+        if (!bytes) return fail(KYRO_EINVAL, "paged_attention_shared_workspace: bytes is null");
+        *bytes = 0;
+        if (int rc = shared_check(p, num_groups)) return rc;
+        AttnSetup from;
+        const int cus = ctx ? ctx->num_cus : kDefaultCUs;
+        if (int rc = attention_setup(p, has_q_start_loc != 0, cus, from)) return rc;
+        const kyro_paged_attention_params plain = unshared_params(p);
+        if (int rc = kyro_paged_attention_workspace(ctx, &plain, has_q_start_loc, bytes)) return rc;
+        *bytes = std::max(*bytes, shared_setup(p, cus, num_groups, from).ws_bytes);
         return KYRO_OK;
     });
 }
