@@ -241,7 +241,6 @@ struct PrefillArgs {
     int tile_tokens;  // prefill_tile_tokens
     int slots;        // workgroups the device runs at once
     int split_cost;   // tiles a workgroup computes in the time that parking and merging one part takes
-    int tail_waves;   // shared attention: wave slots of a part of a sequence's own tokens
 };
 
 // Without a list: tiles of a part of a sequence's row groups, from the sequence's own context, which the
@@ -256,21 +255,40 @@ __host__ __device__ inline int prefill_part_tiles(const PrefillArgs& p, int ctx)
 
 hipError_t launch_attention_prefill(const PrefillArgs& p, hipStream_t stream);
 
-// Attention for sequences that share prefixes (shared_attention.hip): the many-row kernel over a list that has
-// each group's common tokens once, against the rows of the whole group, and each sequence's own tokens.
+// Attention for sequences that share prefixes (shared_attention.hip): workgroups of the kernel a CU holds (registers of
+// its pipeline, and LDS).
+__host__ __device__ constexpr int shared_wgs_per_cu(bool bf16, int D) { return 2; }
 constexpr int kSharedAll = 1 << 30;  // in an entry's tiles: common tokens, which every row sees
+// A unit is a row group (128 rows of one kv head) over a group's common tokens, or of a sequence over its own. The units
+// of a kv head, the common ones first, lie on a line, each as long as its tiles and kSharedUnitCost more, which is cut
+// into equal shares, one for each of the head's workgroups. What a unit costs beside its tiles (its queries, the
+// first copies, its state) is near 3 tiles' time: with 2 a batch of prompts takes 235 us where it takes 233 with 3
+// and 4, with 4 a decode of 64 samples 28.4 where it takes 26.0 with 2 and 27.2 with 3. A tile costs the same
+// over common tokens, where the matrix unit is the limit, as over own ones, where it is memory: weights of 3 : 2
+// put small units of many sequences into one share and made each batch slower.
+constexpr int kSharedUnitCost = 3;
+constexpr int kSharedLeastPart = 2;  // tiles below which a cut is moved to the unit's end
+constexpr int kSharedLeastShare = kSharedUnitCost + 2 * kSharedLeastPart;
+
 struct SharedArgs {
-    PrefillArgs f;                  // list {b, q0, q_len, ctx}, {first row, first tile, tiles | kSharedAll, wave slot or -1};
-                                    // comb {q0, q_len, first row, its row in the group}, {own wave slot, own parts,
-                                    // common wave slot, common parts}
+    AttnArgs a;                     // ws_*: partial states, by wave slots of 32 rows
     const int32_t* group_starts;    // [G + 1]
     const int32_t* group_blocks;    // [G]
+    int4* list;                     // [units + lanes][2]: unit u of workgroup w at u + w: {b or -1, q0, q_len, ctx},
+                                    // {first row, first tile, tiles | kSharedAll, part slot or -1}
+    int2* ranges;                   // [lanes]: first and last unit of a workgroup
+    int2* common_parts;             // [common_cap]: a common unit's first part slot and parts
+    int4* merges;                   // [own_cap][2] {q0, q_len, first row, its row in the group}, {own part slot, own parts,
+                                    // the group's first unit or -1, 0}
     int4* seqs;                     // [B] {q0, q_len, ctx, group or -1}
-    int4* groups;                   // [G] {first row, rows, common tiles, first common part}
-    int2* counts;                   // [G] {sequences, their row groups}
-    int G;
-    int common_cap, tail_cap;       // parts of common and of own tokens that the workspace holds
-    int comb_cap;
+    int4* groups;                   // [G] {first row, rows, common tiles, first unit}
+    int2* counts;                   // [G] {sequences that share, their row groups}
+    int* head;                      // {workgroups of a kv head in use, row groups to merge}
+    int G, tile_tokens;
+    int lanes;                      // workgroups of a kv head
+    int common_cap, own_cap;        // units of either kind that the workspace holds
+    int tail_waves;                 // wave slots of a part over own tokens; those over common ones have 4
+    int tail_base;                  // first wave slot of parts over own tokens
 };
 hipError_t launch_attention_shared(const SharedArgs& s, hipStream_t stream);
 

@@ -41,76 +41,11 @@
 #include "attention_rows.hpp"
 #include "common.hpp"
 #include "kernels.hpp"
+#include "prefill_tile.hpp"
 
 namespace kyro {
 
 namespace {
-
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-
-constexpr int kPfThreads = 256;
-constexpr int kPfWaves = kPfThreads / 64;
-constexpr int kPfBS = 16;  // tokens per slot (slab) of the cache
-constexpr int kRawWord3 = 0x00020000;
-
-// Read in place of a missing slab; never written.
-__device__ uint4 kPfZeroSlab[kPfBS * 512 / 16];
-
-// Layout of a head dim DR (a multiple of 16) with 2- or 4-byte elements.
-template <bool BF16, int DR>
-struct PfCfg {
-    static constexpr int ES = BF16 ? 2 : 4;
-    static constexpr int D = (DR + 31) / 32 * 32;    // columns of V and O held (padded to 32)
-    static constexpr int DT = D / 32;                // 32-column tiles of O^T
-    static constexpr int KS = DR * ES / 32;          // 32-byte steps of a K or Q row
-    static constexpr int CPR = DR * ES / 16;         // 16-byte chunks of a cache row
-    static constexpr int NCH = D * ES / 16;          // chunk slots of a row in LDS
-    // LDS slab: [NCH / CW column groups][16 tokens][CW chunks]. One copy instruction fills 64
-    // consecutive chunks: 4 whole 256-byte rows at CW = 16.
-    static constexpr int CW = NCH % 16 == 0 ? 16 : NCH % 8 == 0 ? 8 : 4;
-    static constexpr int SLAB = kPfBS * NCH;         // chunks of a slab
-    static constexpr int TK = prefill_tile_tokens(BF16, DR);
-    static constexpr int NS = TK / kPfBS;            // slabs of a tile
-    static constexpr int TT = TK / 32;               // 32-token tiles of S^T
-    // f32 head dims where the kernel stands in for the vector kernel, whose sums are trees: short chains
-    // of additions (8 in a score, 4 in a tile's O^T += V^T P^T) that are added up in two halves. The error
-    // against 64 bits is then level with the vector kernel's over 33 to 4000 tokens (prompts of 200 tokens,
-    // head dims 64 / 80 / 96 / 112, 1e-7: 1.15 1.22 1.24 1.23 here, 1.16 1.22 1.26 1.23 there; with two
-    // chains per score, as at 128, 1.82 at 112). At head dim 128 two long chains per score and one per
-    // output are already closer than the one-block kernel's single chain (1.89 against 2.80).
-    static constexpr bool TREE = !BF16 && DR < 128;
-    // K rows: chunk c of token t sits in slot c ^ swk(t) of its column group, so that the 16
-    // tokens of an operand read (same c) spread over all banks.
-    __device__ static constexpr int swk(int t) { return t * CW / 16; }
-    // V rows (bf16): the transposing loads of lanes 0..31 take 64 bytes of each of 4 consecutive
-    // tokens; slot c ^ swv(t) puts those on distinct banks. f32 V is read 128 bytes of one token
-    // at a time: no swizzle.
-    __device__ static constexpr int swv(int t) { return BF16 ? 4 * ((t * CW / 16) & (CW / 4 - 1)) : 0; }
-    static_assert(DR % 16 == 0 && NCH % 4 == 0, "rows of whole 16-byte chunks");
-    static_assert((NS == 4 || NS == 2) && kPfBS * DR * ES <= (int)sizeof(kPfZeroSlab), "tile shape");
-};
-
-// Copies one slab (16 tokens of one kv head, `base`) into LDS at dst (wave-uniform). V selects the
-// V swizzle. Columns past the head dim (DR < D) repeat the row's last chunk: K's are never read,
-// V's reach only output columns that are not stored.
-template <class C, bool V, int POL>
-__device__ __forceinline__ void copy_slab(uint4* dst, const void* base, int lane) {
-    const __amdgpu_buffer_rsrc_t r =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, kPfBS * C::CPR * 16, kRawWord3);
-#pragma unroll
-    for (int e = 0; e < C::SLAB / 64; ++e) {
-        constexpr int kGroup = kPfBS * C::CW;  // chunks of a column group (a multiple of 64)
-        const int cg = 64 * e / kGroup;
-        const int pos = 64 * e - cg * kGroup + lane;
-        const int t = pos / C::CW;
-        const int slot = pos % C::CW;
-        int c = cg * C::CW + (slot ^ (V ? C::swv(t) : C::swk(t)));
-        if (C::CPR < C::NCH) c = min(c, C::CPR - 1);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst + 64 * e), 16,
-                                                 (t * C::CPR + c) * 16, 0, 0, POL);
-    }
-}
 
 // A sequence's rows [q0, q0 + q_len) and context length; the bits of what is wrong with them, or 0.
 __device__ __forceinline__ int sequence_rows(const AttnArgs& a, int b, int& q0, int& q_len, int& ctx) {
@@ -158,11 +93,7 @@ struct PfState {
 
 // POL: cache policy of the K/V copies. Streaming where no other row group reads the slabs (a verify
 // step's 72 rows per kv head, 64 sequences of 4096 tokens: 201 us with cached loads, 178 us so).
-//
-// SHARED: the list is that of shared_attention.hip. Its entries are row groups over a part of the context: of a
-// sequence from its group's common tokens on, or (kSharedAll) of a whole group's rows over the common tokens, all of
-// which see them all. A part's state goes to wave slots of its own (e1.w).
-template <bool BF16, int DR, int POL, bool SHARED = false>
+template <bool BF16, int DR, int POL>
 __global__ __launch_bounds__(kPfThreads, prefill_wgs_per_cu(BF16, DR)) void attn_prefill_kernel(PrefillArgs p) {
     using C = PfCfg<BF16, DR>;
     const AttnArgs& a = p.a;
@@ -174,7 +105,7 @@ __global__ __launch_bounds__(kPfThreads, prefill_wgs_per_cu(BF16, DR)) void attn
     const int entry = (int)blockIdx.x / a.Hkv;
     const int kvh = (int)blockIdx.x - entry * a.Hkv;
     int4 e0, e1;
-    if (SHARED || p.list) {
+    if (p.list) {
         if (entry >= p.head[0]) return;
         e0 = p.list[2 * entry];
         e1 = p.list[2 * entry + 1];
@@ -197,9 +128,7 @@ __global__ __launch_bounds__(kPfThreads, prefill_wgs_per_cu(BF16, DR)) void attn
     const int ctx = __builtin_amdgcn_readfirstlane(e0.w);
     const int row0 = __builtin_amdgcn_readfirstlane(e1.x);
     const int tile0 = __builtin_amdgcn_readfirstlane(e1.y);
-    const int nt = __builtin_amdgcn_readfirstlane(SHARED ? e1.z & ~kSharedAll : e1.z);
-    const bool common = SHARED && (__builtin_amdgcn_readfirstlane(e1.z) & kSharedAll);
-    const bool causal = a.causal && !common;
+    const int nt = __builtin_amdgcn_readfirstlane(e1.z);
     const int part = __builtin_amdgcn_readfirstlane(e1.w);
     SeqInfo si;
     si.b = b;
@@ -215,13 +144,13 @@ __global__ __launch_bounds__(kPfThreads, prefill_wgs_per_cu(BF16, DR)) void attn
     const int h = lane >> 5;
     const int wrow0 = row0 + 32 * wave;  // the wave's first row
     const bool active = wrow0 < si.rows;
-    const int past = causal ? ctx - q_len + 1 : ctx;  // tokens row 0 of the sequence sees
+    const int past = a.causal ? ctx - q_len + 1 : ctx;  // tokens row 0 of the sequence sees
     const int n = wrow0 + col;
     // Rows past the unit take Q = 0 and every token; they are never stored.
-    const int vis = n < si.rows ? (causal ? past + n / a.group : ctx) : ctx;
-    const int wave_lo = causal ? past + wrow0 / a.group : ctx;
-    const int wave_hi = causal ? past + min(wrow0 + 31, si.rows - 1) / a.group : ctx;
-    const int wg_hi = causal ? past + min(row0 + kPrefillRows - 1, si.rows - 1) / a.group : ctx;
+    const int vis = n < si.rows ? (a.causal ? past + n / a.group : ctx) : ctx;
+    const int wave_lo = a.causal ? past + wrow0 / a.group : ctx;
+    const int wave_hi = a.causal ? past + min(wrow0 + 31, si.rows - 1) / a.group : ctx;
+    const int wg_hi = a.causal ? past + min(row0 + kPrefillRows - 1, si.rows - 1) / a.group : ctx;
     const int nslots = (max(wg_hi, 0) + kPfBS - 1) / kPfBS;  // slots the row group sees
     const float c = a.scale_log2;
 
@@ -527,8 +456,7 @@ __global__ __launch_bounds__(kPfThreads, prefill_wgs_per_cu(BF16, DR)) void attn
         return;
     }
     // A part's state: m and l by row, O^T in the order the lanes hold it (whole 1 KiB stores).
-    const size_t wv = SHARED ? (size_t)part + (size_t)kvh * (common ? kPfWaves : p.tail_waves) + wave
-                             : ((size_t)part * a.Hkv + kvh) * kPfWaves + wave;
+    const size_t wv = ((size_t)part * a.Hkv + kvh) * kPfWaves + wave;
     if constexpr (!BF16) {
         // Relative to the rounded scaled maximum that the merge weighs parts by.
         const float m = st.m * c;
@@ -550,7 +478,6 @@ __global__ __launch_bounds__(kPfThreads, prefill_wgs_per_cu(BF16, DR)) void attn
                 make_float4(st.o[dt][4 * k], st.o[dt][4 * k + 1], st.o[dt][4 * k + 2], st.o[dt][4 * k + 3]);
 }
 
-#if KYRO_PREFILL_UNIT < 3
 // Merges the split row groups: a workgroup takes one 32-column tile of one (split row group, kv
 // head), a lane the 16 columns of its row that it held in the first pass.
 template <int DR>
@@ -656,15 +583,6 @@ void launch_prefill_dim(const PrefillArgs& p, hipStream_t stream) {
         attn_prefill_combine_kernel<DR><<<dim3((unsigned)(units < kMaxGrid ? units : kMaxGrid)), kPfThreads, 0, stream>>>(p);
     }
 }
-
-#else
-template <bool BF16, int DR>
-void launch_shared_dim(const PrefillArgs& p, hipStream_t stream) {
-    const dim3 grid((unsigned)((long long)p.list_cap * p.a.Hkv));
-    if (p.a.stream_kv) attn_prefill_kernel<BF16, DR, kLoadStream, true><<<grid, kPfThreads, 0, stream>>>(p);
-    else attn_prefill_kernel<BF16, DR, kLoadCached, true><<<grid, kPfThreads, 0, stream>>>(p);
-}
-#endif
 
 #if KYRO_PREFILL_UNIT == 0
 // ------------------------------------------------------------------------------------- plan
@@ -838,7 +756,7 @@ hipError_t launch_prefill_wide(const PrefillArgs& p, hipStream_t stream) {
     }
     return hipGetLastError();
 }
-#elif KYRO_PREFILL_UNIT == 2
+#else
 hipError_t launch_prefill_f32(const PrefillArgs& p, hipStream_t stream) {
     switch (p.a.D) {
         case 64: launch_prefill_dim<false, 64>(p, stream); break;
@@ -846,41 +764,6 @@ hipError_t launch_prefill_f32(const PrefillArgs& p, hipStream_t stream) {
         case 96: launch_prefill_dim<false, 96>(p, stream); break;
         case 112: launch_prefill_dim<false, 112>(p, stream); break;
         case 128: launch_prefill_dim<false, 128>(p, stream); break;
-        default: return hipErrorInvalidValue;
-    }
-    return hipGetLastError();
-}
-#elif KYRO_PREFILL_UNIT == 3
-hipError_t launch_shared_bf16(const PrefillArgs& p, hipStream_t stream) {
-    switch (p.a.D) {
-        case 64: launch_shared_dim<true, 64>(p, stream); break;
-        case 80: launch_shared_dim<true, 80>(p, stream); break;
-        case 96: launch_shared_dim<true, 96>(p, stream); break;
-        case 112: launch_shared_dim<true, 112>(p, stream); break;
-        case 128: launch_shared_dim<true, 128>(p, stream); break;
-        default: return hipErrorInvalidValue;
-    }
-    return hipGetLastError();
-}
-#elif KYRO_PREFILL_UNIT == 4
-hipError_t launch_shared_wide(const PrefillArgs& p, hipStream_t stream) {
-    switch (p.a.D) {
-        case 160: launch_shared_dim<true, 160>(p, stream); break;
-        case 192: launch_shared_dim<true, 192>(p, stream); break;
-        case 224: launch_shared_dim<true, 224>(p, stream); break;
-        case 256: launch_shared_dim<true, 256>(p, stream); break;
-        default: return hipErrorInvalidValue;
-    }
-    return hipGetLastError();
-}
-#else
-hipError_t launch_shared_f32(const PrefillArgs& p, hipStream_t stream) {
-    switch (p.a.D) {
-        case 64: launch_shared_dim<false, 64>(p, stream); break;
-        case 80: launch_shared_dim<false, 80>(p, stream); break;
-        case 96: launch_shared_dim<false, 96>(p, stream); break;
-        case 112: launch_shared_dim<false, 112>(p, stream); break;
-        case 128: launch_shared_dim<false, 128>(p, stream); break;
         default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

@@ -14,6 +14,7 @@
 #include <cstring>
 #include <new>
 #include <string>
+#include <type_traits>
 #include <vector>
 
 #include "context.hpp"
@@ -575,6 +576,28 @@ struct SharedSetup {
     size_t ws_bytes = 0;
 };
 
+// Points the launch's lists and partial states into `base` (nullptr: counts alone); the bytes they take.
+size_t shared_workspace(SharedSetup& r, char* base) {
+    kyro::SharedArgs& s = r.s;
+    size_t used = 0;
+    auto take = [&](auto*& x, size_t n) {
+        x = base ? reinterpret_cast<std::remove_reference_t<decltype(x)>>(base + used) : nullptr;
+        used += align_up(n * sizeof(*x), 256);
+    };
+    take(s.head, 64);
+    take(s.list, 2 * ((size_t)s.common_cap + s.own_cap + s.lanes));
+    take(s.ranges, (size_t)s.lanes);
+    take(s.common_parts, (size_t)s.common_cap);
+    take(s.merges, 2 * (size_t)s.own_cap);
+    take(s.seqs, (size_t)s.a.B);
+    take(s.groups, (size_t)s.G);
+    take(s.counts, (size_t)s.G);
+    take(s.a.ws_m, r.part_rows);
+    take(s.a.ws_l, r.part_rows);
+    take(s.a.ws_acc, r.part_rows * ((size_t)(s.a.D + 31) / 32 * 32));
+    return used;
+}
+
 SharedSetup shared_setup(const kyro_paged_attention_params* p, int num_cus, int num_groups, const AttnSetup& from) {
     SharedSetup r;
     const bool bf16 = p->dtype == KYRO_BF16;
@@ -583,55 +606,30 @@ SharedSetup shared_setup(const kyro_paged_attention_params* p, int num_cus, int 
         (long long)p->max_blocks_per_seq * p->block_size >= (1ll << 30))
         return r;
     kyro::SharedArgs& s = r.s;
-    kyro::PrefillArgs& f = s.f;
-    kyro::AttnArgs& a = f.a;
+    kyro::AttnArgs& a = s.a;
     a = from.a;
     a.ubs = 16;
     a.sub = a.bs / 16;
     a.rows_per_group = kyro::kPrefillRows;
     a.row_groups = (int)(((long long)a.rows_cap + kyro::kPrefillRows - 1) / kyro::kPrefillRows);
     a.plan = 0;
-    a.stream_kv = 0;
-    f.tile_tokens = kyro::prefill_tile_tokens(bf16, a.D);
-    f.slots = kyro::prefill_wgs_per_cu(bf16, a.D) * num_cus;
-    f.split_cost = bf16 ? 6 : 2;
-    f.tail_waves = (std::min(a.rows_cap, kyro::kPrefillRows) + 31) / 32;
     s.G = num_groups;
-    const long long all = (long long)a.B * a.row_groups, rows = (long long)a.total_q * a.group / kyro::kPrefillRows;
-    const long long own = std::min(all, rows + a.B), common = rows + num_groups;
-    const long long split = f.slots / a.Hkv + 1;  // parts beyond one each: the share is at least a slot's
-    const long long waves = a.Hkv * ((common + split) * 4 + (own + split) * f.tail_waves);
-    if (all > INT32_MAX || waves > INT32_MAX || (own + common + split) * a.Hkv * 256 > 0xffffffffLL) return r;
-    s.common_cap = (int)(common + split);
-    s.tail_cap = (int)(own + split);
-    s.comb_cap = (int)own;
-    f.list_cap = (int)(own + common + split);
-    f.part_cap = 0;
+    s.tile_tokens = kyro::prefill_tile_tokens(bf16, a.D);
+    s.lanes = std::max(1, kyro::shared_wgs_per_cu(bf16, a.D) * num_cus / a.Hkv);
+    s.tail_waves = (std::min(a.rows_cap, kyro::kPrefillRows) + 31) / 32;
+    const long long rows = (long long)a.total_q * a.group / kyro::kPrefillRows;
+    const long long own = std::min((long long)a.B * a.row_groups, rows + a.B), common = rows + num_groups;
+    const long long waves = a.Hkv * ((common + s.lanes) * 4 + (own + s.lanes) * s.tail_waves);
+    const long long line = (own + common) * ((long long)p->max_blocks_per_seq * p->block_size / s.tile_tokens + 1 + kyro::kSharedUnitCost);
+    if (waves > INT32_MAX || line > INT32_MAX || own * a.Hkv * 256 > 0xffffffffLL || (long long)s.lanes * a.Hkv * 256 > 0xffffffffLL)
+        return r;
+    s.common_cap = (int)common;
+    s.own_cap = (int)own;
+    s.tail_base = (int)(a.Hkv * (common + s.lanes) * 4);
     r.part_rows = (size_t)waves * 32;
-    r.ws_bytes = 256 + align_up((size_t)f.list_cap * 2 * sizeof(int4), 256) + align_up((size_t)s.comb_cap * 2 * sizeof(int4), 256) +
-                 align_up((size_t)a.B * sizeof(int4), 256) + align_up((size_t)s.G * sizeof(int4), 256) +
-                 align_up((size_t)s.G * sizeof(int2), 256) + 2 * align_up(r.part_rows * sizeof(float), 256) +
-                 r.part_rows * ((size_t)(a.D + 31) / 32 * 32) * sizeof(float);
+    r.ws_bytes = shared_workspace(r, nullptr);
     r.takes = true;
     return r;
-}
-
-void shared_workspace(SharedSetup& r, char* base) {
-    kyro::SharedArgs& s = r.s;
-    auto take = [&](size_t bytes) -> void* {
-        void* x = base;
-        base += align_up(bytes, 256);
-        return x;
-    };
-    s.f.head = static_cast<int*>(take(256));
-    s.f.list = static_cast<int4*>(take((size_t)s.f.list_cap * 2 * sizeof(int4)));
-    s.f.comb = static_cast<int4*>(take((size_t)s.comb_cap * 2 * sizeof(int4)));
-    s.seqs = static_cast<int4*>(take((size_t)s.f.a.B * sizeof(int4)));
-    s.groups = static_cast<int4*>(take((size_t)s.G * sizeof(int4)));
-    s.counts = static_cast<int2*>(take((size_t)s.G * sizeof(int2)));
-    s.f.a.ws_m = static_cast<float*>(take(r.part_rows * sizeof(float)));
-    s.f.a.ws_l = static_cast<float*>(take(r.part_rows * sizeof(float)));
-    s.f.a.ws_acc = static_cast<float*>(take(0));
 }
 
 // The checks that kyro_paged_attention_shared makes beside those of attention_setup.
@@ -1021,7 +1019,7 @@ int kyro_paged_attention_shared(kyro_ctx ctx, const kyro_paged_attention_params*
         KYRO_HIP(dg.status);
         if (int rc = ensure_arena(ctx, r.ws_bytes)) return rc;
         shared_workspace(r, static_cast<char*>(ctx->arena));
-        kyro::AttnArgs& a = r.s.f.a;
+        kyro::AttnArgs& a = r.s.a;
         a.q = query;
         a.q_start = q_start_loc;
         a.k = key_cache;
