@@ -91,6 +91,45 @@ __device__ __forceinline__ int wave_incl_scan_i(int x) {
     return x;
 }
 
+// Sum that stays at the largest value where it would pass it.
+__device__ __forceinline__ uint32_t add_sat(uint32_t x, uint32_t y) { return __builtin_elementwise_add_sat(x, y); }
+
+// Inclusive sums over the N threads of a workgroup, of up to M values at once, none of which wraps (add_sat). `part` is
+// 2 * M * N / 64 words of LDS. A scan has one barrier, which its caller can count on: the next one writes the other half
+// of `part`, and the one after that comes behind a barrier that everyone reaches with this one's values read.
+template <int N, int M>
+struct BlockSums {
+    uint32_t* part;
+    int turn = 0;
+    template <int K>
+    __device__ __forceinline__ void scan(uint32_t (&x)[K], uint32_t (&all)[K]) {
+        static_assert(K <= M, "room for the waves' sums");
+        uint32_t* p = part + turn * M * (N / 64);
+        turn ^= 1;
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+#define KYRO_STEP_S(ctrl, rmask) x[k] = add_sat(x[k], (uint32_t)KYRO_DPP((int)x[k], ctrl, rmask))
+            KYRO_DPP_SCAN(KYRO_STEP_S);
+#undef KYRO_STEP_S
+            if (lane == 63) p[k * (N / 64) + wave] = x[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            uint32_t before = 0, sum = 0;
+#pragma unroll
+            for (int w = 0; w < N / 64; ++w) {
+                const uint32_t v = p[k * (N / 64) + w];
+                before = add_sat(before, w < wave ? v : 0);
+                sum = add_sat(sum, v);
+            }
+            x[k] = add_sat(x[k], before);
+            all[k] = sum;
+        }
+    }
+};
+
 // Lane l's float as a scalar (the builtin is typed int: the bits move, not a converted value).
 __device__ __forceinline__ float readlane_f(float v, int l) {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l));

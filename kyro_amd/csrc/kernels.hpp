@@ -257,17 +257,19 @@ hipError_t launch_attention_prefill(const PrefillArgs& p, hipStream_t stream);
 
 // Attention for sequences that share prefixes (shared_attention.hip): workgroups of the kernel a CU holds (registers of
 // its pipeline, and LDS).
-__host__ __device__ constexpr int shared_wgs_per_cu(bool bf16, int D) { return 2; }
+__host__ __device__ constexpr int shared_wgs_per_cu(bool bf16, int D) { return !bf16 && D <= 64 ? 3 : 2; }
 constexpr int kSharedAll = 1 << 30;  // in an entry's tiles: common tokens, which every row sees
 // A unit is a row group (128 rows of one kv head) over a group's common tokens, or of a sequence over its own. The units
-// of a kv head, the common ones first, lie on a line, each as long as its tiles and kSharedUnitCost more, which is cut
+// of a kv head, the common ones first, lie on a line, each as long as its tiles and shared_unit_cost more, which is cut
 // into equal shares, one for each of the head's workgroups. What a unit costs beside its tiles (its queries, the
-// first copies, its state) is near 3 tiles' time: with 2 a batch of prompts takes 235 us where it takes 233 with 3
-// and 4, with 4 a decode of 64 samples 28.4 where it takes 26.0 with 2 and 27.2 with 3. A tile costs the same
-// over common tokens, where the matrix unit is the limit, as over own ones, where it is memory: weights of 3 : 2
-// put small units of many sequences into one share and made each batch slower.
+// first copies, its state) is near 3 tiles' time: 64 sequences that verify 8 rows take 93.0 us with 3, 94.2 with 2
+// and 94.5 with 4; decode 51.9, 51.5 and 51.5. A tile costs the same over common tokens, where the matrix unit is the
+// limit, as over own ones, where it is memory: weights of 3 : 2 put small units of many sequences into one share and
+// made each batch slower.
 constexpr int kSharedUnitCost = 3;
-constexpr int kSharedLeastPart = 2;  // tiles below which a cut is moved to the unit's end
+// Tiles below which a cut is moved to the unit's end: 2 for 1 took 24.7 us for 22.9 where 4 samples share 1000
+// tokens, 52.5 for 42.4 in f32, whose tiles are long, and the others within 3 %.
+constexpr int kSharedLeastPart = 1;
 constexpr int kSharedLeastShare = kSharedUnitCost + 2 * kSharedLeastPart;
 
 struct SharedArgs {
@@ -278,13 +280,14 @@ struct SharedArgs {
                                     // {first row, first tile, tiles | kSharedAll, part slot or -1}
     int2* ranges;                   // [lanes]: first and last unit of a workgroup
     int2* common_parts;             // [common_cap]: a common unit's first part slot and parts
-    int4* merges;                   // [own_cap][2] {q0, q_len, first row, its row in the group}, {own part slot, own parts,
-                                    // the group's first unit or -1, 0}
-    int4* seqs;                     // [B] {q0, q_len, ctx, group or -1}
-    int4* groups;                   // [G] {first row, rows, common tiles, first unit}
+    int4* merges;                   // [own_cap][2] {q0, q_len or 0 (nothing to merge), first row, its row in the group},
+                                    // {own part slot, own parts, the group's first unit or -1, 0}
+    int4* seqs;                     // [B] {q0, q_len, ctx, group or -1}; this and the next for batches that LDS does not hold
     int2* counts;                   // [G] {sequences that share, their row groups}
-    int* head;                      // {workgroups of a kv head in use, row groups to merge}
-    int G, tile_tokens;
+    int2* places;                   // [G] {place on the line, first unit or -1}
+    int* bases;                     // [B] first own unit
+    int* head;                      // {workgroups of a kv head in use, own units}
+    int G, tile_shift;              // tokens of a tile: 1 << tile_shift
     int lanes;                      // workgroups of a kv head
     int common_cap, own_cap;        // units of either kind that the workspace holds
     int tail_waves;                 // wave slots of a part over own tokens; those over common ones have 4

@@ -590,8 +590,9 @@ size_t shared_workspace(SharedSetup& r, char* base) {
     take(s.common_parts, (size_t)s.common_cap);
     take(s.merges, 2 * (size_t)s.own_cap);
     take(s.seqs, (size_t)s.a.B);
-    take(s.groups, (size_t)s.G);
     take(s.counts, (size_t)s.G);
+    take(s.places, (size_t)s.G);
+    take(s.bases, (size_t)s.a.B);
     take(s.a.ws_m, r.part_rows);
     take(s.a.ws_l, r.part_rows);
     take(s.a.ws_acc, r.part_rows * ((size_t)(s.a.D + 31) / 32 * 32));
@@ -614,13 +615,13 @@ SharedSetup shared_setup(const kyro_paged_attention_params* p, int num_cus, int 
     a.row_groups = (int)(((long long)a.rows_cap + kyro::kPrefillRows - 1) / kyro::kPrefillRows);
     a.plan = 0;
     s.G = num_groups;
-    s.tile_tokens = kyro::prefill_tile_tokens(bf16, a.D);
+    s.tile_shift = kyro::prefill_tile_tokens(bf16, a.D) == 64 ? 6 : 5;
     s.lanes = std::max(1, kyro::shared_wgs_per_cu(bf16, a.D) * num_cus / a.Hkv);
     s.tail_waves = (std::min(a.rows_cap, kyro::kPrefillRows) + 31) / 32;
     const long long rows = (long long)a.total_q * a.group / kyro::kPrefillRows;
     const long long own = std::min((long long)a.B * a.row_groups, rows + a.B), common = rows + num_groups;
     const long long waves = a.Hkv * ((common + s.lanes) * 4 + (own + s.lanes) * s.tail_waves);
-    const long long line = (own + common) * ((long long)p->max_blocks_per_seq * p->block_size / s.tile_tokens + 1 + kyro::kSharedUnitCost);
+    const long long line = (own + common) * (((long long)p->max_blocks_per_seq * p->block_size >> s.tile_shift) + 1 + kyro::kSharedUnitCost);
     if (waves > INT32_MAX || line > INT32_MAX || own * a.Hkv * 256 > 0xffffffffLL || (long long)s.lanes * a.Hkv * 256 > 0xffffffffLL)
         return r;
     s.common_cap = (int)common;

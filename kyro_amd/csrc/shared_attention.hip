@@ -22,17 +22,15 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Tiles up to the last token that row group rg of q_len rows sees, or -1 where it has no rows.
+// Tiles up to the last token that row group rg of q_len rows sees.
 __device__ __forceinline__ int visible_tiles(const SharedArgs& s, int rg, int q_len, int ctx) {
-    const int rows = q_len * s.a.group;
-    if (rg * kPrefillRows >= rows) return -1;
-    const int last = min((rg + 1) * kPrefillRows, rows) - 1;
-    const int vis = s.a.causal ? ctx - q_len + last / s.a.group + 1 : ctx;
-    return (max(vis, 0) + s.tile_tokens - 1) / s.tile_tokens;
+    const int last = min((rg + 1) * kPrefillRows, q_len * s.a.group) - 1;
+    const int vis = s.a.causal ? ctx - q_len + (int)((unsigned)last / (unsigned)s.a.group) + 1 : ctx;
+    return (max(vis, 0) + (1 << s.tile_shift) - 1) >> s.tile_shift;
 }
 
 __device__ __forceinline__ int row_groups_of(const SharedArgs& s, int rows) {
-    return (int)(((long long)rows * s.a.group + kPrefillRows - 1) / kPrefillRows);
+    return (int)(((uint64_t)(unsigned)rows * (unsigned)s.a.group + kPrefillRows - 1) / kPrefillRows);
 }
 
 // A unit of T tiles at `at` on the line whose shares are `share` long: workgroups first .. last hold a piece
@@ -58,219 +56,209 @@ struct Pieces {
     __device__ bool ends(int w, int line) const { return w < last || (w + 1) * share == end() || end() == line; }
 };
 
-// Inclusive sum over the workgroup's N threads, and the total. `part` holds a value per wave.
-template <int N>
-__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* part, int64_t& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t y = __shfl_up(x, o, 64);
-        if (lane >= o) x += y;
-    }
-    __syncthreads();  // everyone has left the last scan's part
-    if (lane == 63) part[wave] = x;
-    __syncthreads();
-    int64_t before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < N / 64; ++w) {
-        before += w < wave ? part[w] : 0;
-        total += part[w];
-    }
-    return before + x;
-}
-
-// One workgroup of N threads lists the work. A thread has sequence b = thread (and b + N, ..), and group g = thread;
-// records are in LDS for batches of up to N sequences and N groups, in scratch otherwise.
-template <int N>
+// One workgroup of N threads lists the work: thread i has sequence i, group i and the sequences' own unit i, and goes on
+// with i + N, .. in the form for any batch (!ONE), whose records are in scratch; ONE holds them in LDS. It runs on one CU
+// while the others wait, and most of its time is the latency of what follows from each other, and of fetching code that
+// runs once: loads are issued together, barriers are few, sums are of 32 bits, and nothing is divided that a
+// shift does. [[FIGURES]]
+template <int N, bool ONE>
 __global__ __launch_bounds__(N) void attn_shared_plan_kernel(SharedArgs s) {
     const AttnArgs& a = s.a;
-    __shared__ int64_t part[N / 64], red_sum[N / 64];
-    __shared__ int bad_groups;
-    __shared__ int l_starts[N + 1];
-    __shared__ int4 l_seqs[N], l_groups[N];
-    __shared__ int2 l_counts[N];
+    constexpr int kHeld = ONE ? N : 1;
+    __shared__ uint32_t part[2 * 3 * (N / 64)];
+    __shared__ int l_starts[kHeld + 1], l_rows[kHeld + 1], l_base[kHeld];
+    __shared__ int4 l_seqs[kHeld], l_units[kHeld];
+    __shared__ int2 l_counts[kHeld], l_places[kHeld];
+    __shared__ int l_blocks[kHeld], bad_groups;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const bool few = s.G <= N;
-    int4* seqs = a.B <= N ? l_seqs : s.seqs;
-    int4* groups = few ? l_groups : s.groups;
-    int2* counts = few ? l_counts : s.counts;
-    const int32_t* starts = few ? l_starts : s.group_starts;
+    const int32_t* const starts = ONE ? l_starts : s.group_starts;     // first sequences of the groups
+    int4* const seqs = ONE ? l_seqs : s.seqs;                          // {first row, rows, context length, group or -1}
+    int2* const counts = ONE ? l_counts : s.counts;                    // {sequences that share, their row groups}
+    int2* const places = ONE ? l_places : s.places;                    // {place on the line, first unit or -1}
+    int* const base = ONE ? l_base : s.bases;                          // first own unit
+    BlockSums<N, 3> sums{part};
+    auto each = [&](int n, auto&& f) {
+        if constexpr (ONE) {
+            if (t < n) f(t);
+        } else {
+            for (int i = t; i < n; i += N) f(i);
+        }
+    };
+    auto q_row = [&](int b) -> int { return ONE ? l_rows[b] : a.q_start ? a.q_start[b] : b; };
+
     if (t == 0) bad_groups = 0;
-    // Sequences: {first row, rows, context length, -1}, no rows where something is wrong.
-    for (int b = t; b < a.B; b += N) {
+    __syncthreads();
+    each(max(a.B, s.G), [&](int i) {
+        const int b = min(i, a.B - 1), g = min(i, s.G - 1);
         const int64_t c = a.ctx_lens[b];
         const int q0 = a.q_start ? a.q_start[b] : b, q1 = a.q_start ? a.q_start[b + 1] : b + 1;
-        int err = 0;
-        if (c < 0 || c > (int64_t)a.max_blocks * a.bs) err |= ERR_CTX_LEN;
-        if (q0 < 0 || q1 < q0 || q1 > a.total_q || q1 - q0 > a.max_q_len) err |= ERR_Q_LAYOUT;
-        if (err) latch_error(a.err, err);
-        seqs[b] = make_int4(q0, err ? 0 : q1 - q0, err ? 0 : (int)c, -1);
-    }
-    __syncthreads();
-    // Groups: {first row, rows, common tiles, first unit}.
-    for (int g = t; g < s.G; g += N) {
         const int s0 = s.group_starts[g], s1 = s.group_starts[g + 1], nb = s.group_blocks[g];
-        if (few) {
-            l_starts[g] = s0;
-            if (g == s.G - 1) l_starts[s.G] = s1;
+        int err = 0;
+        if (i < a.B) {
+            if (c < 0 || c > (int64_t)a.max_blocks * a.bs) err |= ERR_CTX_LEN;
+            if (q0 < 0 || q1 < q0 || q1 > a.total_q || q1 - q0 > a.max_q_len) err |= ERR_Q_LAYOUT;
+            seqs[b] = make_int4(q0, err ? 0 : q1 - q0, err ? 0 : (int)c, -1);
+            if (ONE) {
+                l_rows[b] = q0;
+                if (b == a.B - 1) l_rows[a.B] = q1;
+            }
         }
-        int4 e = make_int4(0, 0, 0, 0);
-        if (s0 < 0 || s1 < s0 || s1 > a.B) {
-            bad_groups = 1;
-        } else if (nb < 0 || nb > a.max_blocks) {
-            latch_error(a.err, ERR_GROUPS);
-        } else if (nb > 0) {
-            const int q0 = a.q_start ? a.q_start[s0] : s0, q1 = a.q_start ? a.q_start[s1] : s1;
-            if (q0 >= 0 && q0 <= q1 && q1 <= a.total_q)
-                e = make_int4(q0, q1 - q0, (int)((long long)nb * a.bs / s.tile_tokens), 0);
+        if (i < s.G) {
+            if (s0 < 0 || s1 < s0 || s1 > a.B) bad_groups = 1;
+            if (nb < 0 || nb > a.max_blocks) err |= ERR_GROUPS;
+            counts[g] = make_int2(0, 0);
+            if (ONE) {
+                l_starts[g] = s0;
+                l_blocks[g] = nb;
+                if (g == s.G - 1) l_starts[s.G] = s1;
+            }
         }
-        groups[g] = e;
-        counts[g] = make_int2(0, 0);
-    }
+        if (err) latch_error(a.err, err);
+    });
     __syncthreads();
     const int G = bad_groups ? 0 : s.G;
-    if (bad_groups && t == 0) latch_error(a.err, ERR_GROUPS);
-    // The group that a sequence shares with, if every row of it sees the common tokens.
-    for (int b = t; b < a.B; b += N) {
-        const int4 e = seqs[b];
-        if (e.y == 0 || G == 0) continue;
-        int lo = 0, hi = G;  // the last group that starts at or before b is lo - 1
+    if (G == 0 && t == 0) latch_error(a.err, ERR_GROUPS);
+
+    // {first row, rows, common tiles} of a group; no tiles where its numbers are wrong.
+    auto group_of = [&](int g) -> int3 {
+        const int nb = ONE ? l_blocks[g] : s.group_blocks[g], q0 = q_row(starts[g]), q1 = q_row(starts[g + 1]);
+        const bool ok = nb > 0 && nb <= a.max_blocks && q0 >= 0 && q0 <= q1 && q1 <= a.total_q;
+        return ok ? make_int3(q0, q1 - q0, (nb * a.bs) >> s.tile_shift) : make_int3(0, 0, 0);
+    };
+    // The last of n ascending values that is at most x, or -1.
+    auto last_at_most = [](const int* from, int n, int x) -> int {
+        int lo = 0, hi = n;
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (starts[mid] <= b) lo = mid + 1;
+            if (from[mid] <= x) lo = mid + 1;
             else hi = mid;
         }
-        const int g = lo - 1;
-        if (g < 0 || b >= starts[g + 1]) continue;
-        const int4 gr = groups[g];
-        const long long sees = a.causal ? (long long)e.z - e.y + 1 : e.z;
-        if (gr.z > 0 && sees >= (long long)gr.z * s.tile_tokens && e.x >= gr.x && e.x + e.y <= gr.x + gr.y) {
+        return lo - 1;
+    };
+    // The group that a sequence shares with, if every row of it sees the common tokens.
+    each(G > 0 ? a.B : 0, [&](int b) {
+        const int4 e = seqs[b];
+        const int g = last_at_most(starts, G, b);
+        if (e.y == 0 || g < 0 || b >= starts[g + 1]) return;
+        const int3 gr = group_of(g);
+        const int sees = a.causal ? e.z - e.y + 1 : e.z;
+        if (gr.z > 0 && sees >= gr.z << s.tile_shift && e.x >= gr.x && e.x + e.y <= gr.x + gr.y) {
             seqs[b].w = g;
             atomicAdd(&counts[g].x, 1);
             atomicAdd(&counts[g].y, row_groups_of(s, e.y));
         }
-    }
-    __syncthreads();
-    // A group shares where that saves workgroups tiles. The common units' places: {length, units} summed over the groups.
-    int64_t line = 0, units = 0;
-    for (int g0 = 0; g0 < G; g0 += N) {
-        const int g = g0 + t;
-        int64_t len = 0, n = 0;
-        if (g < G) {
-            const int4 gr = groups[g];
-            const int2 k = counts[g];
-            const int rgs = row_groups_of(s, gr.y);
-            if (k.x < 2 || (long long)(k.y - rgs) * gr.z < 1) {
-                groups[g].z = 0;
-            } else {
-                n = rgs;
-                len = n * (gr.z + kSharedUnitCost);
-            }
+    });
+    if (!ONE) __threadfence();  // atomics on scratch
+    // Own units: one a sequence where no sequence has more, also for one without rows.
+    int units = a.B;
+    if (a.row_groups > 1) {
+        uint32_t before = 0;
+        for (int b0 = 0; b0 < a.B; b0 += N) {
+            const int b = b0 + t;
+            uint32_t x[1] = {b < a.B ? (uint32_t)row_groups_of(s, seqs[b].y) : 0}, all[1];
+            const uint32_t n = x[0];
+            sums.scan(x, all);
+            if (b < a.B) base[b] = (int)min(add_sat(before, x[0] - n), (uint32_t)INT32_MAX);
+            before = add_sat(before, all[0]);
+            if (ONE) break;
         }
-        int64_t all_len, all_n;
-        const int64_t at = line + block_scan<N>(len, part, all_len) - len, u = units + block_scan<N>(n, part, all_n) - n;
-        if (g < G) groups[g].w = (int)min(u, (int64_t)INT32_MAX), counts[g] = make_int2((int)at, 0);
-        line += all_len;
-        units += all_n;
+        units = (int)min(before, (uint32_t)INT32_MAX);
     }
+    const bool crowded = units > s.own_cap;  // ranges that overlap around an invalid one
+    if (crowded) units = 0;
     __syncthreads();
-    const int64_t common_units = units, common_line = line;
-    auto common_tiles = [&](const int4& e) -> int { return e.w >= 0 ? groups[e.w].z : 0; };
-    // The whole line: with the sequences' own units.
-    int64_t sum = 0;
-    for (int b = t; b < a.B; b += N) {
-        const int4 e = seqs[b];
-        const int first = common_tiles(e), nrg = row_groups_of(s, e.y);
-        for (int rg = 0; rg < nrg; ++rg) sum += visible_tiles(s, rg, e.y, e.z) - first + kSharedUnitCost;
+
+    // The line: the common units of all groups, then the own units. A group shares where that saves tiles.
+    auto shares = [&](int g, int3& gr) -> bool {
+        gr = group_of(g);
+        const int2 k = counts[g];
+        return k.x > 1 && k.y > row_groups_of(s, gr.y);
+    };
+    uint32_t common_line = 0, common_units = 0, own_line = 0;
+    for (int i0 = 0; i0 < max(G, units); i0 += N) {
+        const int i = i0 + t;
+        uint32_t x[3] = {0, 0, 0}, all[3];
+        int4 unit;
+        int3 gr;
+        if (i < G && shares(i, gr)) {
+            x[1] = (uint32_t)row_groups_of(s, gr.y);
+            x[0] = (uint32_t)min((uint64_t)x[1] * (uint32_t)(gr.z + kSharedUnitCost), (uint64_t)UINT32_MAX);
+        }
+        if (i < units) {
+            const int b = a.row_groups > 1 ? last_at_most(base, a.B, i) : i;
+            const int4 e = seqs[b];
+            const int rg = a.row_groups > 1 ? i - base[b] : 0;
+            const int first = e.w >= 0 && shares(e.w, gr) ? gr.z : 0;
+            unit = make_int4(0, e.y > 0 ? visible_tiles(s, rg, e.y, e.z) - first : -1, b, first);
+            if (e.y > 0) x[2] = (uint32_t)(unit.y + kSharedUnitCost);
+        }
+        const uint32_t len = x[0], n = x[1], own = x[2];
+        sums.scan(x, all);
+        if (i < G) places[i] = make_int2((int)add_sat(common_line, x[0] - len), n ? (int)add_sat(common_units, x[1] - n) : -1);
+        if (i < units) {
+            unit.x = (int)add_sat(own_line, x[2] - own);
+            (ONE ? l_units[i] : s.merges[2 * i]) = unit;
+        }
+        common_line = add_sat(common_line, all[0]);
+        common_units = add_sat(common_units, all[1]);
+        own_line = add_sat(own_line, all[2]);
+        if (ONE) break;
     }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if (lane == 0) red_sum[wave] = sum;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < N / 64; ++w) line += red_sum[w];
-    const int whole = (int)line;  // in 31 bits, as the host has bounded it, unless rows overlap
-    const int share = (int)max((line + s.lanes - 1) / s.lanes, (int64_t)kSharedLeastShare);
-    // Rows that overlap around an invalid range can make more units than were sized: latch it and run nothing.
-    bool over = common_units > s.common_cap || line > INT32_MAX - share;
-    for (int g = wave; g < G && !over; g += N / 64) {
-        const int4 gr = groups[g];
-        if (gr.z == 0) continue;
-        const int at = counts[g].x;
-        const int len = gr.z + kSharedUnitCost, rgs = row_groups_of(s, gr.y), b0 = starts[g];
-        const int most = (len - 1) / share + 2;  // pieces of a unit at most
+    const uint64_t line = (uint64_t)common_line + own_line;
+    const uint32_t share = max((uint32_t)((min(line, (uint64_t)INT32_MAX) + s.lanes - 1)) / (uint32_t)s.lanes,
+                               (uint32_t)kSharedLeastShare);
+    const int whole = (int)line;
+    // More than was sized, which valid ranges cannot be: latch it and run nothing.
+    const bool over = crowded || common_units > (uint32_t)s.common_cap || line + share > INT32_MAX;
+    if (t == 0) {
+        if (over) latch_error(a.err, ERR_PLAN);
+        s.head[0] = over ? 0 : (int)((whole + share - 1) / share);
+        s.head[1] = over ? 0 : units;
+    }
+    if (over) return;
+    if (!ONE || G > 0) __syncthreads();  // places
+    for (int g = wave; g < G; g += N / 64) {
+        const int2 place = places[g];
+        if (place.y < 0) continue;
+        const int3 gr = group_of(g);
+        const int len = gr.z + kSharedUnitCost, rgs = row_groups_of(s, gr.y);
+        const int most = (int)((unsigned)(len - 1) / share) + 2;  // pieces of a unit at most
         for (int x = lane; x < rgs * most; x += 64) {
-            const int r = x / most, u = gr.w + r;
-            const Pieces p(at + r * len, gr.z, share);
+            const int r = (int)((unsigned)x / (unsigned)most), u = place.y + r;
+            const Pieces p(place.x + r * len, gr.z, (int)share);
             const int w = p.first + (x - r * most);
             if (x == r * most) s.common_parts[u] = make_int2(u + p.first_piece(), p.pieces());
             if (w > p.last) continue;
             const int from = p.cut(w - 1), to = p.cut(w);
-            s.list[2 * (u + w)] = make_int4(from < to ? b0 : -1, gr.x, gr.y, gr.z * s.tile_tokens);
+            s.list[2 * (u + w)] = make_int4(from < to ? starts[g] : -1, gr.x, gr.y, gr.z << s.tile_shift);
             s.list[2 * (u + w) + 1] = make_int4(r * kPrefillRows, from, (to - from) | kSharedAll, u + w);
             if (p.begins(w)) s.ranges[w].x = u;
             if (p.ends(w, whole)) s.ranges[w].y = u;
         }
     }
-    // The sequences' own units, and the row groups to merge.
-    int64_t merges = 0;
-    line = common_line;
-    for (int b0 = 0; b0 < a.B; b0 += N) {
-        const int b = b0 + t;
-        int4 e = make_int4(0, 0, 0, -1);
-        int first = 0, nrg = 0;
-        int64_t len = 0;
-        if (b < a.B) {
-            e = seqs[b];
-            first = common_tiles(e);
-            nrg = row_groups_of(s, e.y);
-            for (int rg = 0; rg < nrg; ++rg) len += visible_tiles(s, rg, e.y, e.z) - first + kSharedUnitCost;
+    // The sequences' own units, and which row groups are merged.
+    each(units, [&](int v) {
+        const int4 unit = ONE ? l_units[v] : s.merges[2 * v];
+        const int4 e = seqs[unit.z];
+        const int row = a.row_groups > 1 ? (v - base[unit.z]) * kPrefillRows : 0, first = unit.w;
+        const int u = (int)common_units + v;
+        Pieces p((int)common_line + unit.x, max(unit.y, 0), (int)share);
+        if (unit.y < 0) p.last = p.first;
+        const int pieces = p.pieces();
+        const bool parked = unit.y >= 0 && (first > 0 || pieces > 1), none = unit.y < 0 || (first > 0 && p.T == 0);
+        for (int w = p.first; w <= p.last; ++w) {
+            const int from = p.cut(w - 1), to = p.cut(w);
+            const bool piece = !none && (from < to || (p.T == 0 && w == p.last));
+            s.list[2 * (u + w)] = make_int4(piece ? unit.z : -1, e.x, e.y, e.z);
+            s.list[2 * (u + w) + 1] = make_int4(row, first + from, to - from, parked ? v + w : -1);
+            if (unit.y < 0) break;
+            if (p.begins(w)) s.ranges[w].x = u;
+            if (p.ends(w, whole)) s.ranges[w].y = u;
         }
-        int64_t all_len, all_n;
-        int64_t at = line + block_scan<N>(len, part, all_len) - len, u = units + block_scan<N>(nrg, part, all_n) - nrg;
-        line += all_len;
-        units += all_n;
-        over = over || units - common_units > s.own_cap;
-        // Merges: counted first, as the pieces of a unit decide.
-        int64_t mine = 0;
-        if (!over) {
-            int p0 = (int)at;
-            for (int rg = 0; rg < nrg; ++rg) {
-                const Pieces p(p0, visible_tiles(s, rg, e.y, e.z) - first, share);
-                mine += first > 0 || p.pieces() > 1;
-                p0 = p.end();
-            }
-        }
-        int64_t all_merges;
-        int64_t merge = merges + block_scan<N>(mine, part, all_merges) - mine;
-        merges += all_merges;
-        if (over) continue;
-        const int4 gr = first > 0 ? groups[e.w] : make_int4(0, 0, 0, -1);
-        for (int rg = 0; rg < nrg; ++rg, ++u) {
-            const Pieces p((int)at, visible_tiles(s, rg, e.y, e.z) - first, share);
-            at = p.end();
-            const int pieces = p.pieces();
-            const bool parked = first > 0 || pieces > 1, none = first > 0 && p.T == 0;
-            for (int w = p.first; w <= p.last; ++w) {
-                const int from = p.cut(w - 1), to = p.cut(w);
-                const bool piece = !none && (from < to || (p.T == 0 && w == p.last));
-                s.list[2 * (u + w)] = make_int4(piece ? b : -1, e.x, e.y, e.z);
-                s.list[2 * (u + w) + 1] = make_int4(rg * kPrefillRows, first + from, to - from, parked ? (int)(u - common_units) + w : -1);
-                if (p.begins(w)) s.ranges[w].x = (int)u;
-                if (p.ends(w, whole)) s.ranges[w].y = (int)u;
-            }
-            if (parked) {
-                s.merges[2 * merge] = make_int4(e.x, e.y, rg * kPrefillRows, (e.x - gr.x) * a.group + rg * kPrefillRows);
-                s.merges[2 * merge + 1] = make_int4((int)(u - common_units) + p.first_piece(), none ? 0 : pieces, gr.w, 0);
-                ++merge;
-            }
-        }
-    }
-    if (t == 0) {
-        if (over) latch_error(a.err, ERR_PLAN);
-        s.head[0] = over ? 0 : (whole + share - 1) / share;
-        s.head[1] = over ? 0 : (int)merges;
-    }
+        const int3 gr = first > 0 ? group_of(e.w) : make_int3(0, 0, 0);
+        s.merges[2 * v] = make_int4(e.x, parked ? e.y : 0, row, (e.x - gr.x) * a.group + row);
+        s.merges[2 * v + 1] = make_int4(v + p.first_piece(), none ? 0 : pieces, first > 0 ? places[e.w].y : -1, 0);
+    });
 }
 
 // Merges the partial states of the listed row groups. A workgroup takes a slice of one row group's (row, four
@@ -359,8 +347,8 @@ hipError_t launch_shared_f32(const SharedArgs& s, hipStream_t stream);
 
 hipError_t launch_attention_shared(const SharedArgs& s, hipStream_t stream) {
     const AttnArgs& a = s.a;
-    if (a.B <= 256 && s.G <= 256) attn_shared_plan_kernel<256><<<dim3(1), 256, 0, stream>>>(s);
-    else attn_shared_plan_kernel<1024><<<dim3(1), 1024, 0, stream>>>(s);
+    if (a.B <= 256 && s.G <= 256 && s.own_cap <= 256) attn_shared_plan_kernel<256, true><<<dim3(1), 256, 0, stream>>>(s);
+    else attn_shared_plan_kernel<1024, false><<<dim3(1), 1024, 0, stream>>>(s);
     const hipError_t e = !a.dtype_bf16 ? launch_shared_f32(s, stream) : a.D > 128 ? launch_shared_wide(s, stream) : launch_shared_bf16(s, stream);
     if (e != hipSuccess) return e;
     switch (a.D) {
