@@ -469,7 +469,7 @@ struct alignas(16) TablesEntry {
 };
 constexpr int kTablesMaxRows = 131072;  // requests of a state: two bits each in LDS
 // Batches whose tables have up to so many entries and whose rows are up to so many are one launch.
-constexpr int kTablesOneEntries = 16384;
+constexpr int kTablesOneEntries = 32768;
 constexpr int kTablesOneRows = 4096;
 struct TablesArgs {
     const int32_t* state_rows;  // [B] or nullptr

@@ -15,7 +15,8 @@ namespace {
 constexpr int kTabThreads = 1024;
 constexpr int kTabWaves = kTabThreads / 64;
 constexpr int kFillThreads = 256;
-constexpr int kFillEntries = 2048;  // table entries, rows or freed blocks of one fill workgroup
+constexpr int kFillEntries = 2048;  // table entries or freed blocks of one fill workgroup
+constexpr int kFillRows = 512;      // rows of one fill workgroup: what a row reads follows from what it read before
 
 // What the scan hands to the fill, for each entry of the batch.
 struct Entry {
@@ -25,38 +26,20 @@ struct Entry {
 };
 static_assert(sizeof(Entry) == kTablesEntryBytes, "scratch of an entry");
 
-// Inclusive sum over the workgroup's threads, and the total. `part` holds kTabWaves values.
-__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* part, int64_t& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t y = __shfl_up(x, o, 64);
-        if (lane >= o) x += y;
-    }
-    __syncthreads();  // everyone has left the last scan's part
-    if (lane == 63) part[wave] = x;
-    __syncthreads();
-    int64_t before = 0;
-    total = 0;
-    for (int w = 0; w < kTabWaves; ++w) {
-        before += w < wave ? part[w] : 0;
-        total += part[w];
-    }
-    return before + x;
-}
-
 // The batch's state rows, checked: marks in LDS which requests are named, and which twice.
 struct Names {
     uint32_t* once;   // bits of requests named
     uint32_t* twice;  // named again
 
-    __device__ void mark(const TablesArgs& a, uint32_t* lds) {
+    // `mine` is the state row of entry threadIdx.x, which the caller has loaded.
+    __device__ void mark(const TablesArgs& a, uint32_t* lds, int mine) {
         const int words = (a.num_rows + 31) / 32;
         once = lds;
         twice = lds + words;
         for (int i = threadIdx.x; i < 2 * words; i += kTabThreads) lds[i] = 0;
         __syncthreads();
         for (int b = threadIdx.x; b < a.B; b += kTabThreads) {
-            const int r = a.state_rows ? a.state_rows[b] : b;
+            const int r = b < kTabThreads ? mine : state_row(a, b);
             if (r < 0 || r >= a.num_rows) continue;
             const uint32_t bit = 1u << (r & 31);
             if (atomicOr(&once[r >> 5], bit) & bit) atomicOr(&twice[r >> 5], bit);
@@ -64,9 +47,10 @@ struct Names {
         __syncthreads();
     }
 
-    // Request of entry b, or -1 for padding and for one that is not (latched).
-    __device__ int request(const TablesArgs& a, int b) const {
-        const int r = a.state_rows ? a.state_rows[b] : b;
+    static __device__ int state_row(const TablesArgs& a, int b) { return a.state_rows ? a.state_rows[b] : b; }
+
+    // Request of an entry with state row r, or -1 for padding and for one that is not (latched).
+    __device__ int request(const TablesArgs& a, int r) const {
         if (r < 0) return -1;
         if (r >= a.num_rows || ((twice[r >> 5] >> (r & 31)) & 1u)) {
             latch_error(a.err, ERR_STATE_ROW);
@@ -76,36 +60,51 @@ struct Names {
     }
 };
 
-// A request's record {tokens, held, shared, -}; false (latched) where the numbers do not fit each other.
-__device__ __forceinline__ bool load_record(const TablesArgs& a, int r, int4& rec) {
-    rec = a.requests[r];
+// The record {tokens, held, shared, -} of state row r where there is one.
+__device__ __forceinline__ int4 load_record(const TablesArgs& a, int r) {
+    return r >= 0 && r < a.num_rows ? a.requests[r] : make_int4(0, 0, 0, 0);
+}
+
+// False (latched) where a record's numbers do not fit each other.
+__device__ __forceinline__ bool check_record(const TablesArgs& a, const int4& rec) {
     const bool ok = rec.x >= 0 && rec.z >= 0 && rec.z <= rec.y && rec.y <= a.state_blocks &&
                     (int64_t)rec.x <= (int64_t)rec.y * a.bs;
     if (!ok) latch_error(a.err, ERR_REQUEST);
     return ok;
 }
 
-__device__ __forceinline__ int pool_count(const TablesArgs& a) {
-    const int n = *a.pool_count;
+// The pool's count, or -1 (latched) where it is none.
+__device__ __forceinline__ int check_count(const TablesArgs& a, int n) {
     if (n >= 0 && n <= a.pool_cap) return n;
     if (threadIdx.x == 0) latch_error(a.err, ERR_POOL);
     return -1;
 }
 
-// Entry i of a table row of entry e; a block that is new is the request's from now on.
-__device__ __forceinline__ void fill_block(const TablesArgs& a, const Entry& e, int b, int i) {
-    int64_t id = 0;
-    if (e.row >= 0 && i < e.total) {
-        int64_t* own = a.blocks + (size_t)e.row * a.state_blocks + i;
-        if (i < e.held) {
-            id = *own;
-        } else {
-            id = a.pool[e.base - (i - e.held)];
-            *own = id;
+// Entries i, i + STRIDE, .. below `to` of the table row of entry e; a block that is new is the request's from now on. The
+// loads of kFillBatch entries are in flight together: one without a block loads what is there anyway.
+constexpr int kFillBatch = 8;
+template <int STRIDE>
+__device__ __forceinline__ void fill_blocks(const TablesArgs& a, const Entry& e, int b, int i, int to) {
+    int64_t* own = a.blocks + (size_t)max(e.row, 0) * a.state_blocks;
+    int64_t* table = a.table + (size_t)b * a.width;
+    const int total = e.row >= 0 ? e.total : 0;
+    for (; i < to; i += kFillBatch * STRIDE) {
+        int64_t id[kFillBatch];
+#pragma unroll
+        for (int k = 0; k < kFillBatch; ++k) {
+            const int x = i + k * STRIDE;
+            const int64_t* from = x < total && x >= e.held ? a.pool + (e.base - (x - e.held)) : own + (x < total ? x : 0);
+            id[k] = *from;
         }
-        if (id < 0 || id >= a.num_blocks) latch_error(a.err, ERR_BLOCK_ID);
+#pragma unroll
+        for (int k = 0; k < kFillBatch; ++k) {
+            const int x = i + k * STRIDE;
+            if (x >= to) continue;
+            if (x < total && (id[k] < 0 || id[k] >= a.num_blocks)) latch_error(a.err, ERR_BLOCK_ID);
+            if (x < total && x >= e.held) own[x] = id[k];
+            table[x] = x < total ? id[k] : 0;
+        }
     }
-    a.table[(size_t)b * a.width + i] = id;
 }
 
 // Position and slot of row j of entry e.
@@ -135,82 +134,90 @@ __device__ __forceinline__ int entry_of_row(int B, int64_t i, Start&& start) {
     return lo;
 }
 
-// ONE: the whole call (at most kTabThreads entries).
+// ONE: the whole call (at most kTabThreads entries), whose table rows a wave each fills.
 template <bool ONE>
 __global__ __launch_bounds__(kTabThreads) void tables_extend_kernel(TablesArgs a) {
     extern __shared__ uint32_t names_lds[];
-    __shared__ int64_t part[kTabWaves];
+    __shared__ uint32_t part[2 * 2 * kTabWaves];
+    __shared__ int taken;  // blocks that the entries served take
     __shared__ Entry held[ONE ? kTabThreads : 1];
+    struct Item {
+        int r, m;
+        int4 rec;
+    };
+    auto load = [&](int b) -> Item {
+        Item x{-1, 0, make_int4(0, 0, 0, 0)};
+        if (b >= a.B) return x;
+        x.r = Names::state_row(a, b);
+        x.m = a.new_rows[b];
+        x.rec = load_record(a, x.r);
+        return x;
+    };
+    const int in_pool = *a.pool_count;
+    Item x = load(threadIdx.x);
+    if (threadIdx.x == 0) taken = 0;
     Names names;
-    names.mark(a, names_lds);
-    const int count = pool_count(a);
-    int64_t rows_before = 0, need_before = 0;
-    int64_t taken = 0;  // by the entries served
+    names.mark(a, names_lds, x.r);
+    const int count = check_count(a, in_pool);
+    BlockSums<kTabThreads, 2> sums{part};
+    uint32_t rows_before = 0, need_before = 0;
     for (int b0 = 0; b0 < a.B; b0 += kTabThreads) {
         const int b = b0 + threadIdx.x;
-        const bool in = b < a.B;
-        int r = -1, m = 0;
-        int4 rec = make_int4(0, 0, 0, 0);
-        if (in) {
-            r = names.request(a, b);
-            m = a.new_rows[b];
-            if (m < 0) {
-                latch_error(a.err, ERR_Q_LAYOUT);
-                m = 0;
-                r = -1;
-            }
-            if (r >= 0 && !load_record(a, r, rec)) r = -1;
+        if (b0 > 0) x = load(b);
+        int r = b < a.B ? names.request(a, x.r) : -1, m = x.m;
+        if (m < 0) {
+            latch_error(a.err, ERR_Q_LAYOUT);
+            m = 0;
+            r = -1;
         }
-        int64_t rows_all, need_all;
-        const int64_t rows_to = rows_before + block_scan(m, part, rows_all);
-        const int64_t ctx = (int64_t)rec.x + m;
-        if (r >= 0 && rows_to > a.max_rows) {
+        if (r >= 0 && !check_record(a, x.rec)) r = -1;
+        const int64_t ctx = (int64_t)x.rec.x + m;
+        const bool long_ = ctx > (int64_t)min(a.width, a.state_blocks) * a.bs;
+        const int need = r >= 0 && !long_ ? max((int)((ctx + a.bs - 1) / a.bs) - x.rec.y, 0) : 0;
+        // Rows and blocks of the batch up to here. Entries past max_rows are left out, and so are all that follow, so
+        // that what they would need counts against none that is served.
+        uint32_t to[2] = {(uint32_t)m, (uint32_t)need}, all[2];
+        sums.scan(to, all);
+        const uint32_t rows_to = add_sat(rows_before, to[0]), need_to = add_sat(need_before, to[1]);
+        if (r >= 0 && rows_to > (uint32_t)a.max_rows) {
             latch_error(a.err, ERR_Q_LAYOUT);
             r = -1;
         }
-        if (r >= 0 && ctx > (int64_t)min(a.width, a.state_blocks) * a.bs) {
+        if (r >= 0 && long_) {
             latch_error(a.err, ERR_CTX_LEN);
             r = -1;
         }
-        const int64_t need = r >= 0 ? max((ctx + a.bs - 1) / a.bs - rec.y, (int64_t)0) : 0;
-        const int64_t need_to = need_before + block_scan(need, part, need_all);
-        bool served = r >= 0;
-        if (served && need > 0 && need_to > count) {
+        if (r >= 0 && need > 0 && (count < 0 || need_to > (uint32_t)count)) {
             if (count >= 0) latch_error(a.err, ERR_NO_BLOCKS);
-            served = false;
+            r = -1;
         }
-        int64_t taken_all;
-        (void)block_scan(served ? need : 0, part, taken_all);
-        taken += taken_all;
-        if (in) {
+        if (b < a.B) {
             Entry e;
-            e.row = served ? r : -1;
-            e.held = rec.y;
-            e.total = rec.y + (int)need;
-            e.base = (int)(count - 1 - (need_to - need));
-            e.q0 = (int)min(rows_to - m, (int64_t)INT32_MAX);
+            e.row = r;
+            e.held = x.rec.y;
+            e.total = x.rec.y + need;
+            e.base = count - 1 - (int)(need_to - need);
+            e.q0 = (int)min(rows_to - m, (uint32_t)INT32_MAX);
             e.rows = m;
-            e.ctx = served ? (int)ctx : 0;
-            e.tokens = rec.x;
+            e.ctx = r >= 0 ? (int)ctx : 0;
+            e.tokens = x.rec.x;
             if (ONE) held[threadIdx.x] = e;
             else a.entries[b] = *reinterpret_cast<TablesEntry*>(&e);
             a.ctx_lens[b] = e.ctx;
             if (b == 0) a.q_start[0] = 0;
-            a.q_start[b + 1] = (int)min(rows_to, (int64_t)INT32_MAX);
-            if (served && need > 0) reinterpret_cast<int*>(a.requests + r)[1] = e.total;
+            a.q_start[b + 1] = (int)min(rows_to, (uint32_t)INT32_MAX);
+            if (r >= 0 && need > 0) {
+                reinterpret_cast<int*>(a.requests + r)[1] = e.total;
+                atomicMax(&taken, (int)need_to);  // those served are the first ones that need blocks
+            }
         }
-        rows_before += rows_all;
-        need_before += need_all;
+        rows_before = add_sat(rows_before, all[0]);
+        need_before = add_sat(need_before, all[1]);
     }
-    // Those served are the first ones that need blocks, so what they took is a front of the sums.
-    if (threadIdx.x == 0 && taken > 0) *a.pool_count = count - (int)taken;
-    if (!ONE) return;
     __syncthreads();
-    const int n = a.B * a.width;  // small: the host checks
-    for (int x = threadIdx.x; x < n; x += kTabThreads) {
-        const int b = x / a.width;
-        fill_block(a, held[b], b, x - b * a.width);
-    }
+    if (threadIdx.x == 0 && taken > 0) *a.pool_count = count - taken;
+    if (!ONE) return;
+    for (int b = threadIdx.x >> 6; b < a.B; b += kTabWaves) fill_blocks<64>(a, held[b], b, threadIdx.x & 63, a.width);
     if (!a.positions && !a.slots) return;
     for (int i = threadIdx.x; i < a.max_rows; i += kTabThreads) {
         const int b = entry_of_row(a.B, i, [&](int x) -> int64_t { return x < a.B ? held[x].q0 : (int64_t)held[a.B - 1].q0 + held[a.B - 1].rows; });
@@ -224,15 +231,25 @@ __global__ __launch_bounds__(kFillThreads) void tables_fill_kernel(TablesArgs a)
         const int chunks = (a.width + kFillEntries - 1) / kFillEntries;
         const int b = (int)(blockIdx.x / chunks), c = (int)(blockIdx.x - (unsigned)b * chunks);
         const Entry e = entries[b];
-        const int to = min(a.width, (c + 1) * kFillEntries);
-#pragma unroll 4
-        for (int i = c * kFillEntries + threadIdx.x; i < to; i += kFillThreads) fill_block(a, e, b, i);
+        fill_blocks<kFillThreads>(a, e, b, c * kFillEntries + threadIdx.x, min(a.width, (c + 1) * kFillEntries));
         return;
     }
-    const int64_t first = ((int64_t)blockIdx.x - a.table_wgs) * kFillEntries;
-    const int64_t to = min((int64_t)a.max_rows, first + kFillEntries);
+    // The entries of the workgroup's rows, whose starts it takes to LDS unless many without rows lie between them.
+    __shared__ int starts[kFillRows + 2];
+    const int64_t first = ((int64_t)blockIdx.x - a.table_wgs) * kFillRows;
+    const int64_t to = min((int64_t)a.max_rows, first + kFillRows);
+    auto start = [&](int x) -> int64_t { return a.q_start[x]; };
+    const int64_t rows = start(a.B);
+    const int from = max(entry_of_row(a.B, first, start), 0);
+    const int n = rows <= first ? 0 : entry_of_row(a.B, min(to, rows) - 1, start) - from + 1;
+    const bool held = n <= kFillRows;
+    if (held) {
+        for (int x = threadIdx.x; x <= n; x += kFillThreads) starts[x] = a.q_start[from + x];
+        __syncthreads();
+    }
     for (int64_t i = first + threadIdx.x; i < to; i += kFillThreads) {
-        const int b = entry_of_row(a.B, i, [&](int x) -> int64_t { return a.q_start[x]; });
+        int b = -1;
+        if (i < rows) b = held ? from + entry_of_row(n, i, [&](int x) -> int64_t { return starts[x]; }) : entry_of_row(a.B, i, start);
         const Entry e = entries[max(b, 0)];
         fill_row(a, e, i, b < 0 ? -1 : (int)(i - e.q0));
     }
@@ -242,60 +259,81 @@ __global__ __launch_bounds__(kFillThreads) void tables_fill_kernel(TablesArgs a)
 template <bool KEEP>
 __global__ __launch_bounds__(kTabThreads) void tables_shrink_kernel(TablesArgs a) {
     extern __shared__ uint32_t names_lds[];
-    __shared__ int64_t part[kTabWaves];
+    __shared__ uint32_t part[2 * kTabWaves];
     __shared__ int to_base[kTabThreads], from_row[kTabThreads], from_at[kTabThreads];
+    struct Item {
+        int r, q0, q1, kept;
+        int64_t c;
+        int4 rec;
+    };
+    auto load = [&](int b) -> Item {
+        Item x{-1, 0, 0, 0, 0, make_int4(0, 0, 0, 0)};
+        if (b >= a.B) return x;
+        x.r = Names::state_row(a, b);
+        if (KEEP) {
+            x.q0 = a.q_start[b];
+            x.q1 = a.q_start[b + 1];
+            x.kept = a.kept[b];
+            x.c = a.ctx_lens[b];
+        }
+        x.rec = load_record(a, x.r);
+        return x;
+    };
+    const int in_pool = *a.pool_count;
+    const Item mine = load(threadIdx.x);
     Names names;
-    names.mark(a, names_lds);
-    const int count = pool_count(a);
+    names.mark(a, names_lds, mine.r);
+    const int count = check_count(a, in_pool);
     // What an entry gives back: blocks [stay, held) of request r.
     struct Shrink {
         int r, stay, held, tokens;
     };
     auto look = [&](int b) -> Shrink {
         Shrink s{-1, 0, 0, 0};
-        int4 rec;
-        s.r = names.request(a, b);
-        if (s.r >= 0 && !load_record(a, s.r, rec)) s.r = -1;
+        if (b >= a.B) return s;
+        const Item x = b < kTabThreads ? mine : load(b);
+        s.r = names.request(a, x.r);
+        if (s.r >= 0 && !check_record(a, x.rec)) s.r = -1;
         if (s.r < 0) return s;
-        s.held = rec.y;
-        s.stay = rec.z;
+        s.held = x.rec.y;
+        s.stay = x.rec.z;
         if (!KEEP) return s;
-        const int q0 = a.q_start[b], q1 = a.q_start[b + 1];
-        const int64_t m = (int64_t)q1 - q0, c = a.ctx_lens[b];
-        int64_t k = m;
-        if (m > 0) k = (int64_t)a.kept[b] + a.kept_plus;
-        if (q0 < 0 || m < 0 || k < 0 || k > m) {
+        const int64_t m = (int64_t)x.q1 - x.q0;
+        const int64_t k = m > 0 ? (int64_t)x.kept + a.kept_plus : m;
+        if (x.q0 < 0 || m < 0 || k < 0 || k > m) {
             latch_error(a.err, ERR_Q_LAYOUT);
             s.r = -1;
-        } else if (c < m || c - m + k > (int64_t)rec.y * a.bs) {
-            if (c != 0) latch_error(a.err, ERR_CTX_LEN);  // 0: extend left the entry out
+        } else if (x.c < m || x.c - m + k > (int64_t)x.rec.y * a.bs) {
+            if (x.c != 0) latch_error(a.err, ERR_CTX_LEN);  // 0: extend left the entry out
             s.r = -1;
         } else {
-            s.tokens = (int)(c - m + k);
-            s.stay = min(rec.y, max(rec.z, (s.tokens + a.bs - 1) / a.bs));
+            s.tokens = (int)(x.c - m + k);
+            s.stay = min(x.rec.y, max(x.rec.z, (s.tokens + a.bs - 1) / a.bs));
         }
         return s;
     };
     // First what all give back: a pool that cannot take it leaves everything as it is.
-    int64_t all = 0;
+    BlockSums<kTabThreads, 1> sums{part};
+    uint32_t all = 0, to[1], total[1];
     Shrink s{-1, 0, 0, 0};
     for (int b0 = 0; b0 < a.B; b0 += kTabThreads) {
-        const int b = b0 + threadIdx.x;
-        s = b < a.B ? look(b) : Shrink{-1, 0, 0, 0};
-        int64_t total;
-        (void)block_scan(s.r >= 0 ? s.held - s.stay : 0, part, total);
-        all += total;
+        s = look(b0 + threadIdx.x);
+        to[0] = s.r >= 0 ? (uint32_t)(s.held - s.stay) : 0;
+        sums.scan(to, total);
+        all = add_sat(all, total[0]);
     }
-    const bool fits = count >= 0 && count + all <= a.pool_cap;
+    const bool fits = count >= 0 && (uint64_t)count + all <= (uint64_t)a.pool_cap;
     if (!fits && threadIdx.x == 0) latch_error(a.err, ERR_POOL);
-    int64_t before = fits ? count : 0;
+    int before = fits ? count : 0;
     for (int b0 = 0; b0 < a.B; b0 += kTabThreads) {
         const int b = b0 + threadIdx.x;
-        if (a.B > kTabThreads) s = b < a.B ? look(b) : Shrink{-1, 0, 0, 0};  // a single strip has it from above
+        if (a.B > kTabThreads) {  // a single strip has it from above
+            s = look(b);
+            to[0] = s.r >= 0 ? (uint32_t)(s.held - s.stay) : 0;
+            sums.scan(to, total);
+        }
         const bool live = fits && s.r >= 0;
-        const int freed = live ? s.held - s.stay : 0;
-        int64_t total;
-        const int64_t to = before + block_scan(freed, part, total);
+        const int base = (int)(to[0] - (s.r >= 0 ? (uint32_t)(s.held - s.stay) : 0));  // behind `before`
         if (b < a.B) {
             if (KEEP) {
                 a.out_ctx[b] = live ? s.tokens : 0;
@@ -305,25 +343,26 @@ __global__ __launch_bounds__(kTabThreads) void tables_shrink_kernel(TablesArgs a
                 e.row = live ? s.r : -1;
                 e.held = s.stay;
                 e.total = s.held;
-                e.base = (int)(to - freed);
+                e.base = before + base;
                 a.entries[b] = *reinterpret_cast<TablesEntry*>(&e);
                 if (live) a.requests[s.r] = make_int4(0, 0, 0, 0);
             }
         }
-        if (KEEP) {
-            to_base[threadIdx.x] = (int)(to - freed - before);
+        if (!fits) continue;
+        if (KEEP && total[0] > 0) {
+            to_base[threadIdx.x] = base;
             from_row[threadIdx.x] = s.r;
             from_at[threadIdx.x] = s.stay;
             __syncthreads();
             const int strip = min(kTabThreads, a.B - b0);
-            for (int64_t x = threadIdx.x; x < total; x += kTabThreads) {
+            for (int64_t x = threadIdx.x; x < total[0]; x += kTabThreads) {
                 // The last entry whose blocks start at or before x: those that give none share its start.
-                const int t = entry_of_row(strip, x, [&](int y) -> int64_t { return y < strip ? (int64_t)to_base[y] : total; });
+                const int t = entry_of_row(strip, x, [&](int y) -> int64_t { return y < strip ? (int64_t)to_base[y] : total[0]; });
                 a.pool_out[before + x] = a.blocks[(size_t)from_row[t] * a.state_blocks + from_at[t] + (x - to_base[t])];
             }
             __syncthreads();
         }
-        before += total;
+        before += (int)total[0];
     }
     if (threadIdx.x == 0 && fits && all > 0) *a.pool_count = count + (int)all;
 }
@@ -350,7 +389,7 @@ bool tables_one_launch(const TablesArgs& a) {
 
 int64_t tables_fill_wgs(const TablesArgs& a, int64_t& table_wgs) {
     table_wgs = (int64_t)a.B * ((a.width + kFillEntries - 1) / kFillEntries);
-    return table_wgs + (a.positions || a.slots ? ((int64_t)a.max_rows + kFillEntries - 1) / kFillEntries : 0);
+    return table_wgs + (a.positions || a.slots ? ((int64_t)a.max_rows + kFillRows - 1) / kFillRows : 0);
 }
 
 int64_t tables_free_wgs(const TablesArgs& a) { return (int64_t)a.B * ((a.state_blocks + kFillEntries - 1) / kFillEntries); }
