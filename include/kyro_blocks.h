@@ -118,6 +118,15 @@ int kyro_bm_write_tables(kyro_bm bm, kyro_ctx ctx, const uint64_t* request_ids, 
                          int32_t max_blocks, int64_t* block_table, int64_t* context_lens,
                          int32_t* out_shared);
 
+/* The requests in an order in which those that hold the same first blocks stand together, and the groups of neighbours
+ * that kyro_paged_attention_shared takes: order [B] has indices into request_ids, group g is the requests order[i]
+ * for i in [group_starts[g], group_starts[g+1]), and their first group_blocks[g] blocks are the same (0 for a request by
+ * itself). The groups cover the batch; group_starts has room for B + 1 entries, group_blocks for B, num_groups receives
+ * their number. Of all such groups they are those that leave out the most blocks ((n - 1) d for n requests with d
+ * blocks in common), so a prefix that many share can win over longer ones that few do. Host only. */
+int kyro_bm_prefix_groups(kyro_bm bm, const uint64_t* request_ids, int32_t B, int32_t* order, int32_t* group_starts,
+                          int32_t* group_blocks, int32_t* num_groups);
+
 /* ---------------------------------------------------------------- block copies */
 
 typedef struct kyro_copy_blocks_params {

@@ -187,6 +187,7 @@ _SIGNATURES = {
     "kyro_bm_check": ([_P], ctypes.c_int),
     "kyro_bm_num_cached_blocks": ([_P], ctypes.c_int64),
     "kyro_bm_match_prefix": ([_P, _P, ctypes.c_int64, _P, ctypes.c_int64, _P, _P], ctypes.c_int),
+    "kyro_bm_prefix_groups": ([_P, _P, ctypes.c_int32, _P, _P, _P, _P], ctypes.c_int),
     "kyro_bm_write_tables": ([_P, _P, _P, ctypes.c_int32, ctypes.c_int32, _P, _P, _P], ctypes.c_int),
     "kyro_copy_blocks": ([_P, ctypes.POINTER(CopyBlocksParams), _P, _P, _P, _P, ctypes.c_int64], ctypes.c_int),
     # include/kyro_evict.h

@@ -234,6 +234,19 @@ class BlockManager:
             context_lens.data_ptr() if context_lens is not None else None, ctypes.byref(shared)))
         return bool(shared.value)
 
+    def prefix_groups(self, request_ids) -> tuple[np.ndarray, np.ndarray, np.ndarray]:
+        """(order, group_starts, group_blocks), int32, for :meth:`kyro_amd.PagedAttention.forward_shared`:
+        ``request_ids[order]`` has requests that hold the same first blocks next to each other, group g is the
+        entries [group_starts[g], group_starts[g + 1]) of that order, and its first ``group_blocks[g]`` blocks are
+        common to all of them (0 for a request by itself). Of all such groups, those that leave out the most blocks."""
+        rid = np.ascontiguousarray(np.asarray(request_ids, dtype=np.uint64).reshape(-1))
+        B = rid.size
+        order, starts, blocks = np.zeros(B, np.int32), np.zeros(B + 1, np.int32), np.zeros(B, np.int32)
+        n = ctypes.c_int32()
+        _lib.check(_lib.lib().kyro_bm_prefix_groups(self._h, _ptr(rid), B, _ptr(order), _ptr(starts), _ptr(blocks),
+                                                    ctypes.byref(n)))
+        return order, starts[: n.value + 1].copy(), blocks[: n.value].copy()
+
 
 def copy_blocks(key_cache, value_cache, pairs) -> None:
     """key_cache[dst] = key_cache[src] (and value_cache) for every (src, dst) pair, on torch's

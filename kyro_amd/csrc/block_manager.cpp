@@ -350,5 +350,61 @@ std::vector<std::pair<int64_t, int64_t>> BlockManager::take_copies() {
     return out;
 }
 
+// Sorted, lists with a common start are neighbours, and the runs of neighbours that share at least d blocks nest. They
+// are walked innermost first with a stack of the open ones. Where a run with d blocks in common ends, each run (or list)
+// right inside it, of n lists whose own groups leave out s, either keeps those groups or joins the one group of
+// the run, to which it adds n d; the group as a whole leaves out d less than its parts add.
+std::vector<PrefixGroup> prefix_groups(const std::vector<const std::vector<int64_t>*>& lists) {
+    struct Part {
+        std::vector<PrefixGroup> groups;
+        int64_t n, saved;
+    };
+    struct Run {
+        int64_t blocks;
+        std::vector<Part> parts;
+    };
+    auto close = [](Run& run) -> Part {
+        int64_t apart = 0, joined = -run.blocks, n = 0;
+        for (const Part& p : run.parts) {
+            apart += p.saved;
+            joined += std::max(p.saved, p.n * run.blocks);
+            n += p.n;
+        }
+        Part out{{}, n, std::max(apart, joined)};
+        PrefixGroup group{{}, run.blocks};
+        for (Part& p : run.parts)
+            for (PrefixGroup& g : p.groups) {
+                if (joined > apart && p.saved <= p.n * run.blocks)
+                    group.members.insert(group.members.end(), g.members.begin(), g.members.end());
+                else out.groups.push_back(std::move(g));
+            }
+        if (!group.members.empty()) out.groups.push_back(std::move(group));
+        return out;
+    };
+    const size_t n = lists.size();
+    std::vector<int32_t> order(n);
+    for (size_t i = 0; i < n; ++i) order[i] = (int32_t)i;
+    std::stable_sort(order.begin(), order.end(), [&](int32_t a, int32_t b) { return *lists[(size_t)a] < *lists[(size_t)b]; });
+    std::vector<Run> open;
+    open.push_back({0, {}});
+    for (size_t i = 0; i < n; ++i) {
+        Part last{{{{order[i]}, 0}}, 1, 0};  // what has just ended: the list by itself, or a run up to it
+        int64_t d = 0;                       // blocks in common with the next list
+        if (i + 1 < n) {
+            const std::vector<int64_t>&a = *lists[(size_t)order[i]], &b = *lists[(size_t)order[i + 1]];
+            const size_t m = std::min(a.size(), b.size());
+            d = std::mismatch(a.begin(), a.begin() + (ptrdiff_t)m, b.begin()).first - a.begin();
+        }
+        while (open.back().blocks > d) {
+            open.back().parts.push_back(std::move(last));
+            last = close(open.back());
+            open.pop_back();
+        }
+        if (open.back().blocks < d) open.push_back({d, {}});
+        open.back().parts.push_back(std::move(last));
+    }
+    return close(open.back()).groups;
+}
+
 }  // namespace bm
 }  // namespace kyro

@@ -78,6 +78,14 @@ struct Request {
     int64_t num_tokens = 0;
 };
 
+// Block lists in groups that hold their first `blocks` blocks in common (0 for a group of one), chosen so that the most
+// blocks are left out: a group of n with d blocks leaves out (n - 1) d.
+struct PrefixGroup {
+    std::vector<int32_t> members;
+    int64_t blocks;
+};
+std::vector<PrefixGroup> prefix_groups(const std::vector<const std::vector<int64_t>*>& lists);
+
 enum Status : int { OK = 0, EINVAL_ = 1, ENOSPACE = 5 };
 
 class BlockManager {

@@ -414,6 +414,31 @@ int kyro_bm_write_tables(kyro_bm bm, kyro_ctx ctx, const uint64_t* request_ids, 
     });
 }
 
+int kyro_bm_prefix_groups(kyro_bm bm, const uint64_t* request_ids, int32_t B, int32_t* order, int32_t* group_starts,
+                          int32_t* group_blocks, int32_t* num_groups) {
+    return guarded([&]() -> int {
+        if (!bm || B < 0 || !group_starts || !num_groups || (B > 0 && (!request_ids || !order || !group_blocks)))
+            return fail(KYRO_EINVAL, "bm_prefix_groups: bad arguments");
+        std::vector<const std::vector<int64_t>*> lists((size_t)B);
+        for (int32_t b = 0; b < B; ++b) {
+            const kyro::bm::Request* r = bm->m.find(request_ids[b]);
+            if (!r)
+                return fail(KYRO_EINVAL, "bm_prefix_groups: unknown request %llu", (unsigned long long)request_ids[b]);
+            lists[(size_t)b] = &r->blocks;
+        }
+        const std::vector<kyro::bm::PrefixGroup> groups = kyro::bm::prefix_groups(lists);
+        int32_t at = 0;
+        for (size_t g = 0; g < groups.size(); ++g) {
+            group_starts[g] = at;
+            group_blocks[g] = (int32_t)groups[g].blocks;
+            for (const int32_t b : groups[g].members) order[at++] = b;
+        }
+        group_starts[groups.size()] = at;
+        *num_groups = (int32_t)groups.size();
+        return KYRO_OK;
+    });
+}
+
 // ------------------------------------------------------------------------------- copies
 
 int kyro_copy_blocks(kyro_ctx ctx, const kyro_copy_blocks_params* p, void* key_cache, void* value_cache,
