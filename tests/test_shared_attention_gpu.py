@@ -212,6 +212,20 @@ def test_more_sequences_and_groups_than_the_plan_holds_in_lds(gpu, B, G):
     check(run(gpu, case, starts, np.full(G, 6, np.int32)), case, reference(case))
 
 
+@pytest.mark.parametrize("B,most", [(300, 140), (40, 2000), (1100, 40)])
+def test_more_row_groups_than_the_plan_holds_in_lds(gpu, B, most):
+    """Sequences of none to several row groups (32 rows of a kv head each), some of which share."""
+    rng = np.random.default_rng(B)
+    rows = rng.integers(0, most, B)
+    rows[rng.integers(0, B, B // 4)] = 0
+    SHAPES["row_groups"] = ((4, 1), [0, B // 3, B // 3 + 1, B - 2], [130, 0, 64], (rows + rng.integers(0, 60, B)).tolist(), rows.tolist())
+    try:
+        case, starts, blocks = make("row_groups", "bf16", 64)
+    finally:
+        del SHAPES["row_groups"]
+    check(run(gpu, case, starts, blocks), case, reference(case))
+
+
 @pytest.mark.parametrize("dtype,D,block", [("bf16", 72, 16), ("bf16", 128, 8), ("f32", 256, 16), ("f32", 40, 24)])
 def test_other_geometries_run_without_the_groups(gpu, dtype, D, block):
     case, starts, blocks = make("verify", dtype, D, block=block, seed=9)
