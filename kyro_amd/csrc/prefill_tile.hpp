@@ -58,25 +58,33 @@ struct PfCfg {
     static_assert((NS == 4 || NS == 2) && kPfBS * DR * ES <= (int)sizeof(kPfZeroSlab), "tile shape");
 };
 
-// Copies one slab (16 tokens of one kv head, `base`) into LDS at dst (wave-uniform). V selects the
-// V swizzle. Columns past the head dim (DR < D) repeat the row's last chunk: K's are never read,
-// V's reach only output columns that are not stored.
+// One of the C::SLAB / 64 copies of 64 consecutive chunks that take a slab (16 tokens of one kv head, `from`) into LDS
+// at dst (wave-uniform). V selects the V swizzle. Columns past the head dim (DR < D) repeat the row's last chunk: K's are
+// never read, V's reach only output columns that are not stored.
+template <class C, bool V, int POL>
+__device__ __forceinline__ void copy_chunks(uint4* dst, __amdgpu_buffer_rsrc_t from, int lane, int e) {
+    constexpr int kGroup = kPfBS * C::CW;  // chunks of a column group (a multiple of 64)
+    const int cg = 64 * e / kGroup;
+    const int pos = 64 * e - cg * kGroup + lane;
+    const int t = pos / C::CW;
+    const int slot = pos % C::CW;
+    int c = cg * C::CW + (slot ^ (V ? C::swv(t) : C::swk(t)));
+    if (C::CPR < C::NCH) c = min(c, C::CPR - 1);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)(dst + 64 * e), 16,
+                                             (t * C::CPR + c) * 16, 0, 0, POL);
+}
+
+// A slab as a buffer; one of no bytes reads as zeros.
+template <class C>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t slab_buffer(const void* base, bool empty = false) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, empty ? 0 : kPfBS * C::CPR * 16, kRawWord3);
+}
+
 template <class C, bool V, int POL>
 __device__ __forceinline__ void copy_slab(uint4* dst, const void* base, int lane) {
-    const __amdgpu_buffer_rsrc_t r =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, kPfBS * C::CPR * 16, kRawWord3);
+    const __amdgpu_buffer_rsrc_t r = slab_buffer<C>(base);
 #pragma unroll
-    for (int e = 0; e < C::SLAB / 64; ++e) {
-        constexpr int kGroup = kPfBS * C::CW;  // chunks of a column group (a multiple of 64)
-        const int cg = 64 * e / kGroup;
-        const int pos = 64 * e - cg * kGroup + lane;
-        const int t = pos / C::CW;
-        const int slot = pos % C::CW;
-        int c = cg * C::CW + (slot ^ (V ? C::swv(t) : C::swk(t)));
-        if (C::CPR < C::NCH) c = min(c, C::CPR - 1);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst + 64 * e), 16,
-                                                 (t * C::CPR + c) * 16, 0, 0, POL);
-    }
+    for (int e = 0; e < C::SLAB / 64; ++e) copy_chunks<C, V, POL>(dst, r, lane, e);
 }
 
 // Operand addresses (bytes) of a lane in a tile, one per swizzle pattern.

@@ -33,6 +33,7 @@ __global__ __launch_bounds__(kPfThreads, shared_wgs_per_cu(BF16, DR)) void attn_
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31;
     const int h = lane >> 5;
+    const bool younger = 2 * blockIdx.x >= gridDim.x;  // dispatched to a CU that has a workgroup
     const TileLane<C> at(lane);
     const float c = a.scale_log2;
     constexpr size_t kSlabBytes = (size_t)kPfBS * C::CPR * 16;
@@ -112,7 +113,7 @@ __global__ __launch_bounds__(kPfThreads, shared_wgs_per_cu(BF16, DR)) void attn_
             __syncthreads();                     // everyone's; and everyone is done with the tile before
         };
 
-        f32x16 o[C::DT], S[C::TT];
+        f32x16 o[C::DT], S[C::TT], T[C::TT];
         float m = kNegInf, l = 0.f;  // running maximum, the lane's share of the row sum
 #pragma unroll
         for (int dt = 0; dt < C::DT; ++dt)
@@ -155,7 +156,7 @@ __global__ __launch_bounds__(kPfThreads, shared_wgs_per_cu(BF16, DR)) void attn_
         // Weight of a score, relative to ref.
         auto weight = [&](float x, float ref) { return fast_exp2(BF16 ? __builtin_fmaf(x, c, -ref) : (x - ref) * c); };
         // Tile i, whose scores are in S: its weights and its output.
-        auto step = [&](int i, const uint4* vb, uint32_t tbad) {
+        auto step = [&](int i, const uint4* vb, uint32_t tbad, f32x16* S) {
             if (i >= whole || tbad) mask(i, tbad, S);
             raise(row_max(S));
             const float ref = m == kNegInf ? 0.f : m;
@@ -174,11 +175,14 @@ __global__ __launch_bounds__(kPfThreads, shared_wgs_per_cu(BF16, DR)) void attn_
                 tile_output<C>(reinterpret_cast<const char*>(vb), S[tt], w, at, o, tt);
             }
         };
-        // The same, with the scores of tile i + 1 (K at kb), which take its place in S; mx is the maximum of either
+        // The same, with the scores of tile i + 1 (K at kb), which go to `next`; mx is the maximum of either
         // tile's scores before any mask. The order is written out: a product, the read of the operand kRing products
         // later, and some of the vector work, in turn (left to itself the compiler reads each operand right before
-        // its product and keeps the work apart from both).
-        auto step_ahead = [&](int i, const uint4* kbuf, const uint4* vbuf, uint32_t tbad, float& mx) {
+        // its product and keeps the work apart from both). `copy` issues one of the wave's 2 * kSlabCopies copies for
+        // the tiles to come: all at once after the barrier, four waves' copies take the address unit 500 cycles, in
+        // which no wave has a product to run.
+        auto step_ahead = [&](int i, const uint4* kbuf, const uint4* vbuf, uint32_t tbad, float& mx, f32x16* S, f32x16* next,
+                              auto&& copy) {
             if constexpr (PIPE) {
                 static_assert(C::TT == 2, "two halves of a tile");
                 const char* kb = reinterpret_cast<const char*>(kbuf);
@@ -189,13 +193,12 @@ __global__ __launch_bounds__(kPfThreads, shared_wgs_per_cu(BF16, DR)) void attn_
                 }
                 raise(mx);
                 const float ref = m == kNegInf ? 0.f : m;
-                constexpr int NA = C::KS, NB = 2 * C::DT, kOps = 2 * (NA + NB), kRing = 4;
+                constexpr int NA = C::KS, NB = 2 * C::DT, kOps = 2 * (NA + NB), kRing = 4, kCopies = 2 * (C::SLAB / 64);
                 // Products in order: scores of the next tile's first half, output of this one's first half, then the second.
                 auto read = [&](int x) -> uint4 {
                     const int tt = x / (NA + NB), y = x % (NA + NB);
                     return y < NA ? k_operand<C>(kb, at, tt, y) : v_operand<C>(vb, at, tt, (y - NA) / C::DT, (y - NA) % C::DT);
                 };
-                f32x16 next[2];
                 uint4 ring[kRing], w[2][2];
                 float pt[4] = {0.f, 0.f, 0.f, 0.f};
                 float top = kNegInf;
@@ -231,6 +234,7 @@ __global__ __launch_bounds__(kPfThreads, shared_wgs_per_cu(BF16, DR)) void attn_
                         o[z % C::DT] = mfma_bf16(ring[x % kRing], w[tt][z / C::DT], o[z % C::DT]);
                     }
                     if (x + kRing < kOps) ring[x % kRing] = read(x + kRing);
+                    if ((x + 1) * kCopies / kOps > x * kCopies / kOps) copy(x * kCopies / kOps);
                     // Weights of the first half beside the next one's scores, of the second beside the first's output and
                     // the next second's scores; maxima beside what is left.
                     if (tt == 0 && y < NA) weigh(0, 16 * y / NA, 16 * (y + 1) / NA);
@@ -242,8 +246,6 @@ __global__ __launch_bounds__(kPfThreads, shared_wgs_per_cu(BF16, DR)) void attn_
                 l += (pt[0] + pt[1]) + (pt[2] + pt[3]);
                 const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
                 mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-#pragma unroll
-                for (int tt = 0; tt < C::TT; ++tt) S[tt] = next[tt];
             }
         };
 
@@ -275,19 +277,32 @@ __global__ __launch_bounds__(kPfThreads, shared_wgs_per_cu(BF16, DR)) void attn_
             issue_v(0, sV0);
             if constexpr (PIPE) {
                 float mx = kNegInf;
+                constexpr int kSlabCopies = C::SLAB / 64;
                 // Tile i of nt: after the wait V of it is in v0 and K of the next in k1; V of the next goes to v1, K of
                 // the one after that to k0.
-                auto turn = [&](int i, uint4* k0, uint4* k1, uint4* v0, uint4* v1) {
+                auto turn = [&](int i, uint4* k0, uint4* k1, uint4* v0, uint4* v1, f32x16* now, f32x16* next) {
+                    // The two workgroups of a CU take turns at being first: left alone the older one is, and the other one
+                    // still runs when it has ended (c2).
+                    if (younger == (now == S)) __builtin_amdgcn_s_setprio(1);
+                    else __builtin_amdgcn_s_setprio(0);
                     landed();
                     clear_tail(i, v0);
                     const uint32_t tbad = tile_bad(i);
                     next_ids(i + 1);
-                    issue_v(i + 1, v1);
-                    if (i + 2 < nt) issue_k(i + 2, (i + 2) % kFill == 0 ? ids_next : ids, k0);
-                    if (active) step_ahead(i, k1, v0, tbad, mx);
+                    const auto vr = slab_buffer<C>(slab_ptr(a.v, ids, i + 1, wave));
+                    const auto kr = slab_buffer<C>(slab_ptr(a.k, (i + 2) % kFill == 0 ? ids_next : ids, i + 2, wave), i + 2 >= nt);
+                    auto copy = [&](int e) {
+                        if (e < kSlabCopies) copy_chunks<C, true, kLoadCached>(v1 + wave * C::SLAB, vr, lane, e);
+                        else copy_chunks<C, false, kLoadCached>(k0 + wave * C::SLAB, kr, lane, e - kSlabCopies);
+                    };
+                    if (active) {
+                        step_ahead(i, k1, v0, tbad, mx, now, next, copy);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 2 * kSlabCopies; ++e) copy(e);
+                    }
                 };
                 // The first scores wait for K of the first tile alone: the copies behind it are one slab, or two.
-                constexpr int kSlabCopies = C::SLAB / 64;
                 static_assert(!PIPE || (C::NS == 4 && 2 * kSlabCopies < 16), "copies of a wave, in the wait's low bits");
                 if (nt > 1) {
                     issue_k(1, ids, sK1);
@@ -308,14 +323,18 @@ __global__ __launch_bounds__(kPfThreads, shared_wgs_per_cu(BF16, DR)) void attn_
                 int i = 0;
                 while (true) {
                     if (i + 1 >= nt) break;
-                    turn(i++, sK0, sK1, sV0, sV1);
-                    if (i + 1 >= nt) break;
-                    turn(i++, sK1, sK0, sV1, sV0);
+                    turn(i++, sK0, sK1, sV0, sV1, S, T);
+                    if (i + 1 >= nt) {
+#pragma unroll
+                        for (int tt = 0; tt < C::TT; ++tt) S[tt] = T[tt];
+                        break;
+                    }
+                    turn(i++, sK1, sK0, sV1, sV0, T, S);
                 }
                 landed();
                 uint4* v = i % 2 ? sV1 : sV0;
                 clear_tail(i, v);
-                if (active) step(i, v, tile_bad(i));
+                if (active) step(i, v, tile_bad(i), S);
             } else {
                 // Registers hold one tile's scores: both operands of the next tile land while this one is computed.
                 auto turn = [&](int i, uint4* k0, uint4* v0, uint4* k1, uint4* v1) {
@@ -330,7 +349,7 @@ __global__ __launch_bounds__(kPfThreads, shared_wgs_per_cu(BF16, DR)) void attn_
                     if (!active) return;
 #pragma unroll
                     for (int tt = 0; tt < C::TT; ++tt) S[tt] = tile_scores<C>(reinterpret_cast<const char*>(k0), q, at, tt);
-                    step(i, v0, tbad);
+                    step(i, v0, tbad, S);
                 };
                 for (int i = 0;;) {
                     turn(i, sK0, sV0, sK1, sV1);
