@@ -278,7 +278,7 @@ struct SharedArgs {
     const int32_t* group_blocks;    // [G]
     int4* list;                     // [units + lanes][2]: unit u of workgroup w at u + w: {b or -1, q0, q_len, ctx},
                                     // {first row, first tile, tiles | kSharedAll, part slot or -1}
-    int2* ranges;                   // [lanes]: first and last unit of a workgroup
+    int4* starts;                   // [lanes][3]: {first, last unit of a workgroup, -, -}, the first one's entry of the list
     int2* common_parts;             // [common_cap]: a common unit's first part slot and parts
     int4* merges;                   // [own_cap][2] {q0, q_len or 0 (nothing to merge), first row, its row in the group},
                                     // {own part slot, own parts, the group's first unit or -1, 0}

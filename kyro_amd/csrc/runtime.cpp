@@ -586,7 +586,7 @@ size_t shared_workspace(SharedSetup& r, char* base) {
     };
     take(s.head, 64);
     take(s.list, 2 * ((size_t)s.common_cap + s.own_cap + s.lanes));
-    take(s.ranges, (size_t)s.lanes);
+    take(s.starts, 3 * (size_t)s.lanes);
     take(s.common_parts, (size_t)s.common_cap);
     take(s.merges, 2 * (size_t)s.own_cap);
     take(s.seqs, (size_t)s.a.B);

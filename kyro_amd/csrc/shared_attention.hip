@@ -217,6 +217,17 @@ __global__ __launch_bounds__(N) void attn_shared_plan_kernel(SharedArgs s) {
     }
     if (over) return;
     if (!ONE || G > 0) __syncthreads();  // places
+    // Workgroup w's piece of unit u; an empty unit begins and ends no share.
+    auto put = [&](const Pieces& p, int u, int w, const int4& e0, const int4& e1, bool some = true) {
+        s.list[2 * (u + w)] = e0;
+        s.list[2 * (u + w) + 1] = e1;
+        if (some && p.begins(w)) {
+            s.starts[3 * w].x = u;
+            s.starts[3 * w + 1] = e0;
+            s.starts[3 * w + 2] = e1;
+        }
+        if (some && p.ends(w, whole)) s.starts[3 * w].y = u;
+    };
     for (int g = wave; g < G; g += N / 64) {
         const int2 place = places[g];
         if (place.y < 0) continue;
@@ -230,10 +241,8 @@ __global__ __launch_bounds__(N) void attn_shared_plan_kernel(SharedArgs s) {
             if (x == r * most) s.common_parts[u] = make_int2(u + p.first_piece(), p.pieces());
             if (w > p.last) continue;
             const int from = p.cut(w - 1), to = p.cut(w);
-            s.list[2 * (u + w)] = make_int4(from < to ? starts[g] : -1, gr.x, gr.y, gr.z << s.tile_shift);
-            s.list[2 * (u + w) + 1] = make_int4(r * kPrefillRows, from, (to - from) | kSharedAll, u + w);
-            if (p.begins(w)) s.ranges[w].x = u;
-            if (p.ends(w, whole)) s.ranges[w].y = u;
+            put(p, u, w, make_int4(from < to ? starts[g] : -1, gr.x, gr.y, gr.z << s.tile_shift),
+                make_int4(r * kPrefillRows, from, (to - from) | kSharedAll, u + w));
         }
     }
     // The sequences' own units, and which row groups are merged.
@@ -249,11 +258,8 @@ __global__ __launch_bounds__(N) void attn_shared_plan_kernel(SharedArgs s) {
         for (int w = p.first; w <= p.last; ++w) {
             const int from = p.cut(w - 1), to = p.cut(w);
             const bool piece = !none && (from < to || (p.T == 0 && w == p.last));
-            s.list[2 * (u + w)] = make_int4(piece ? unit.z : -1, e.x, e.y, e.z);
-            s.list[2 * (u + w) + 1] = make_int4(row, first + from, to - from, parked ? v + w : -1);
-            if (unit.y < 0) break;
-            if (p.begins(w)) s.ranges[w].x = u;
-            if (p.ends(w, whole)) s.ranges[w].y = u;
+            put(p, u, w, make_int4(piece ? unit.z : -1, e.x, e.y, e.z), make_int4(row, first + from, to - from, parked ? v + w : -1),
+                unit.y >= 0);
         }
         const int3 gr = first > 0 ? group_of(e.w) : make_int3(0, 0, 0);
         s.merges[2 * v] = make_int4(e.x, parked ? e.y : 0, row, (e.x - gr.x) * a.group + row);
@@ -268,8 +274,9 @@ __global__ __launch_bounds__(kThreads) void attn_shared_combine_kernel(SharedArg
     const AttnArgs& a = s.a;
     constexpr int DT = (DR + 31) / 32, Q = DR / 4;
     const int entry = (int)blockIdx.x / a.Hkv, kvh = (int)blockIdx.x - entry * a.Hkv;
-    if (entry >= s.head[1]) return;
+    const int used = s.head[1];
     const int4 e = s.merges[2 * entry], f = s.merges[2 * entry + 1];
+    if (entry >= used) return;
     const int rows = min(kPrefillRows, e.y * a.group - e.z);
     const int x = (int)blockIdx.y * kThreads + threadIdx.x;
     if (x >= rows * Q) return;

@@ -27,8 +27,10 @@ __global__ __launch_bounds__(kPfThreads, shared_wgs_per_cu(BF16, DR)) void attn_
 
     const int wg = (int)blockIdx.x / a.Hkv;
     const int kvh = (int)blockIdx.x - wg * a.Hkv;
-    if (wg >= s.head[0]) return;
-    const int2 range = s.ranges[wg];
+    // Loads that follow from each other take 1 us each where the chip is cold, so the first unit comes with the range.
+    const int used = s.head[0];
+    const int4 range = s.starts[3 * wg], first0 = s.starts[3 * wg + 1], first1 = s.starts[3 * wg + 2];
+    if (wg >= used) return;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31;
@@ -40,7 +42,8 @@ __global__ __launch_bounds__(kPfThreads, shared_wgs_per_cu(BF16, DR)) void attn_
     const size_t head_off = (size_t)kvh * a.bs * (C::CPR * 16);
 
     for (int u = range.x; u <= range.y; ++u) {
-        const int4 e0 = s.list[2 * (u + wg)], e1 = s.list[2 * (u + wg) + 1];
+        const bool first = u == range.x;
+        const int4 e0 = first ? first0 : s.list[2 * (u + wg)], e1 = first ? first1 : s.list[2 * (u + wg) + 1];
         const int b = __builtin_amdgcn_readfirstlane(e0.x);
         if (b < 0) continue;  // the unit begins or ends a few tiles past this workgroup's share
         const int ctx = __builtin_amdgcn_readfirstlane(e0.w);
@@ -68,13 +71,6 @@ __global__ __launch_bounds__(kPfThreads, shared_wgs_per_cu(BF16, DR)) void attn_
         const bool active = wrow0 < si.rows;
         const int whole = max(wave_lo, 0) / C::TK - tile0;  // tiles that all the wave's rows see whole
 
-        uint4 q[C::KS];
-        {
-            const char* qp = reinterpret_cast<const char*>(a.q) + out_row(a, si, n < si.rows ? n : 0) * (C::CPR * 16);
-#pragma unroll
-            for (int x = 0; x < C::KS; ++x) q[x] = n < si.rows ? load16(qp + (2 * x + h) * 16) : make_uint4(0, 0, 0, 0);
-        }
-
         // Slab ids of 64 slots, one per lane (slab index of kv head 0, -1 for a bad block id), and of the next 64.
         constexpr int kFill = 64 / C::NS;
         auto load_ids = [&](int tile) -> int {
@@ -88,7 +84,16 @@ __global__ __launch_bounds__(kPfThreads, shared_wgs_per_cu(BF16, DR)) void attn_
             }
             return (int)id * a.Hkv * a.sub + (x - blk * a.sub);
         };
-        int ids = 0, ids_next = 0;
+        int ids = load_ids(tile0);  // before the queries, which it would wait for
+        int ids_next = 0;
+
+        uint4 q[C::KS];
+        {
+            const char* qp = reinterpret_cast<const char*>(a.q) + out_row(a, si, n < si.rows ? n : 0) * (C::CPR * 16);
+#pragma unroll
+            for (int x = 0; x < C::KS; ++x) q[x] = n < si.rows ? load16(qp + (2 * x + h) * 16) : make_uint4(0, 0, 0, 0);
+        }
+
         uint64_t bad = 0;
         auto slab_ptr = [&](const void* cache, int from, int i, int x) -> const void* {
             const int id = __builtin_amdgcn_readlane(from, (i % kFill) * C::NS + x);
@@ -270,8 +275,7 @@ __global__ __launch_bounds__(kPfThreads, shared_wgs_per_cu(BF16, DR)) void attn_
 
         __syncthreads();  // everyone has left the unit before
         if (nt > 0) {
-            ids = load_ids(tile0);
-            ids_next = load_ids(tile0 + kFill);
+            ids_next = nt > kFill ? load_ids(tile0 + kFill) : 0;
             bad = __ballot(ids < 0);
             issue_k(0, ids, sK0);
             issue_v(0, sV0);
