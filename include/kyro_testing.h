@@ -19,6 +19,10 @@ extern "C" {
  * KYRO_EINVAL. Returns the previous cap. */
 int64_t kyro_testing_set_plan_slot_cap(int64_t cap);
 
+/* Whether kyro_paged_attention_shared takes its own kernel, and shares in it, however little that saves
+ * (process-wide; 0, the initial state, does so where it pays). Returns the previous setting. */
+int kyro_testing_set_shared_any_size(int on);
+
 struct kyro_paged_attention_params;
 
 /* Tiles of a part that the many-row attention kernel gives the row groups of a sequence of `ctx` tokens in a

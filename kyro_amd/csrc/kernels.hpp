@@ -271,6 +271,10 @@ constexpr int kSharedUnitCost = 3;
 // tokens, 52.5 for 42.4 in f32, whose tiles are long, and the others within 3 %.
 constexpr int kSharedLeastPart = 1;
 constexpr int kSharedLeastShare = kSharedUnitCost + 2 * kSharedLeastPart;
+// Tiles that a unit costs more where a group shares: its state is written and merged. 8 prompts of 100 to 300 rows behind
+// 6000 tokens, which save 4 of 54 row groups, take 205 us shared and 202 not, 64 sequences of 30 rows behind 4096
+// (4 of 64) 230 and 214, 4 prompts of 75 rows behind 6000 (2 of 12) 59.6 and 62.9: all at 4.5 to 6.
+constexpr int kSharedMergeCost = 5;
 
 struct SharedArgs {
     AttnArgs a;                     // ws_*: partial states, by wave slots of 32 rows
@@ -288,6 +292,7 @@ struct SharedArgs {
     int* bases;                     // [B] first own unit
     int* head;                      // {workgroups of a kv head in use, own units}
     int G, tile_shift;              // tokens of a tile: 1 << tile_shift
+    int merge_cost;                 // kSharedMergeCost
     int lanes;                      // workgroups of a kv head
     int common_cap, own_cap;        // units of either kind that the workspace holds
     int tail_waves;                 // wave slots of a part over own tokens; those over common ones have 4

@@ -27,6 +27,8 @@ thread_local std::string g_last_error;
 // Partial-state slots a balanced-schedule launch sizes at most (0: the bound); set only through
 // kyro_testing_set_plan_slot_cap.
 std::atomic<int64_t> g_test_plan_slot_cap{0};
+// Shared-prefix attention shares in calls of any size; set only through kyro_testing_set_shared_any_size.
+std::atomic<bool> g_test_shared_any_size{false};
 }  // namespace
 
 struct kyro_buf_s {
@@ -617,6 +619,7 @@ SharedSetup shared_setup(const kyro_paged_attention_params* p, int num_cus, int 
     s.G = num_groups;
     s.tile_shift = kyro::prefill_tile_tokens(bf16, a.D) == 64 ? 6 : 5;
     s.lanes = std::max(1, kyro::shared_wgs_per_cu(bf16, a.D) * num_cus / a.Hkv);
+    s.merge_cost = g_test_shared_any_size.load(std::memory_order_relaxed) ? 0 : kyro::kSharedMergeCost;
     s.tail_waves = (std::min(a.rows_cap, kyro::kPrefillRows) + 31) / 32;
     const long long rows = (long long)a.total_q * a.group / kyro::kPrefillRows;
     const long long own = std::min((long long)a.B * a.row_groups, rows + a.B), common = rows + num_groups;
@@ -640,6 +643,22 @@ int shared_check(const kyro_paged_attention_params* p, int32_t num_groups) {
     if (p->path != KYRO_ATTN_AUTO || p->schedule != KYRO_ATTN_SCHEDULE_AUTO || p->num_splits != 0)
         return fail(KYRO_EINVAL, "paged_attention_shared: path and schedule must be AUTO and num_splits 0");
     return KYRO_OK;
+}
+
+// Whether a call has so much to read that sharing can pay: the kernels for each sequence by itself are one launch less,
+// and what several of them read comes from the caches. Sequences with all but 16 tokens in common, 32/8 heads of
+// 128 in bf16, shared and not: 16 of one row behind 2000 tokens (132 MB if each reads its own) 21.7 us and 16.9, behind
+// 4000 23.4 and 33.0; 16 of 8 rows 27.8 and 27.3, 34.3 and 42.7. In f32, where products are the limit, rows count as
+// well: 24 of 5 rows, 14/2 heads of 96, behind 1000 (38 MB) 38.5 and 34.9, behind 2000 41.9 and 58.2; of one row behind
+// 4000 (149 MB) 41.0 and 35.4. Prompts, whose rows the kernel for many rows does not split over tokens, are not
+// measured by this: 4 of 40 rows behind 1000 take 25.8 and 37.7. The width of the table stands for the contexts,
+// which the host does not see.
+bool shared_pays(const kyro_paged_attention_params* p) {
+    const bool bf16 = p->dtype == KYRO_BF16;
+    const long long rows = (long long)std::max(p->max_q_len, 1) * (p->num_heads / p->num_kv_heads);
+    const double mib = 2.0 * p->batch_size * p->max_blocks_per_seq * p->block_size * p->num_kv_heads * p->head_dim * (bf16 ? 2 : 4) / (1 << 20);
+    if (g_test_shared_any_size.load(std::memory_order_relaxed)) return true;
+    return bf16 ? rows > 32 || mib > 128 : rows > 64 || mib > 128 || mib * rows > 1728;
 }
 
 // The params of the launch that takes a call in its place.
@@ -748,6 +767,8 @@ int kyro_abi_version(void) { return KYRO_ABI_VERSION; }
 int64_t kyro_testing_set_plan_slot_cap(int64_t cap) {
     return g_test_plan_slot_cap.exchange(cap < 0 ? 0 : cap, std::memory_order_relaxed);
 }
+
+int kyro_testing_set_shared_any_size(int on) { return g_test_shared_any_size.exchange(on != 0, std::memory_order_relaxed) ? 1 : 0; }
 
 int kyro_testing_prefill_part_tiles(const kyro_paged_attention_params* p, int has_q_start_loc, int64_t ctx, int* splits) {
     return guarded([&]() -> int {
@@ -1010,7 +1031,8 @@ int kyro_paged_attention_shared(kyro_ctx ctx, const kyro_paged_attention_params*
             (num_groups > 0 && (!group_starts || !group_blocks)))
             return fail(KYRO_EINVAL, "paged_attention_shared: null device pointer");
         if (int rc = check_ctx(ctx)) return rc;  // last, so that a host without a device can have the rest checked
-        SharedSetup r = shared_setup(p, ctx->num_cus, num_groups, from);
+        SharedSetup r;
+        if (shared_pays(p)) r = shared_setup(p, ctx->num_cus, num_groups, from);
         const bool aligned = ((reinterpret_cast<uintptr_t>(key_cache) | reinterpret_cast<uintptr_t>(value_cache)) & 15) == 0;
         if (!r.takes || !aligned) {
             const kyro_paged_attention_params plain = unshared_params(p);

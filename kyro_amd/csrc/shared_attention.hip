@@ -168,11 +168,13 @@ __global__ __launch_bounds__(N) void attn_shared_plan_kernel(SharedArgs s) {
     if (crowded) units = 0;
     __syncthreads();
 
-    // The line: the common units of all groups, then the own units. A group shares where that saves tiles.
+    // The line: the common units of all groups, then the own units. A group shares where the tiles it saves are worth the
+    // states it adds.
     auto shares = [&](int g, int3& gr) -> bool {
         gr = group_of(g);
         const int2 k = counts[g];
-        return k.x > 1 && k.y > row_groups_of(s, gr.y);
+        const int rgs = row_groups_of(s, gr.y);
+        return k.x > 1 && (int64_t)(k.y - rgs) * gr.z > (int64_t)(k.y + rgs) * s.merge_cost;
     };
     uint32_t common_line = 0, common_units = 0, own_line = 0;
     for (int i0 = 0; i0 < max(G, units); i0 += N) {
