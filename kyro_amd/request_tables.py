@@ -57,6 +57,7 @@ class RequestTables:
                              f"{tuple(requests.shape)}, {tuple(blocks.shape)}, {tuple(pool_count.shape)}")
         self.requests, self.blocks, self.pool, self.pool_count = requests, blocks, pool, pool_count
         self.device = dev
+        self._index = requests.get_device()
 
     @classmethod
     def new(cls, block_size: int, *, rows: int, max_blocks: int, pool, num_blocks: int, device):
@@ -81,6 +82,10 @@ class RequestTables:
         self.requests[row] = torch.tensor([tokens, ids.size, ids.size, 0], dtype=torch.int32, device=self.device)
 
     def _vector(self, t, name, dtype, n):
+        # One expression for a tensor as it should be; _require names what is not.
+        if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.numel() == n and t.dim() == 1
+                and t.get_device() == self._index and t.is_contiguous()):
+            return
         _require(t, name, (dtype,), 1, self.device)
         if t.shape[0] != n:
             raise ValueError(f"{name} must have {n} entries, got {t.shape[0]}")
@@ -92,9 +97,9 @@ class RequestTables:
             raise ValueError("without state_rows every entry of the batch needs a request of the state")
 
     def _context(self):
-        if self.device.type != "cuda":
+        idx = self._index
+        if idx < 0:
             raise ValueError("RequestTables runs on a GPU device; got " + str(self.device))
-        idx = self.device.index or 0
         ctx = _lib.context(idx)
         ctx.set_stream(_lib.current_stream(idx))
         return ctx
