@@ -16,6 +16,8 @@ acceptance, and the paged KV write. This package is the Python host mirror of th
     BlockManager(block_size, num_gpu_blocks, num_cpu_blocks), RadixCache(max_capacity)
         (src/scheduler/block_manager.rs, src/scheduler/radix_cache.rs) and the device tables
     RequestTables(...).extend(...) / .keep(...)  the same tables built on the GPU, accepted lengths included
+    PagedAttention.forward_shared(...), BlockManager.prefix_groups(...)  attention that reads a prefix which several
+        sequences share once
     sample_tokens(...)  (src/worker.rs:141-197 logit processors, then sample_token :267-362)
     NgramTable(corpus, order).draft(...)  (src/speculative.rs:196-256, the Ngram draft strategy)
 """
@@ -29,9 +31,8 @@ from .request_tables import RequestTables, StepTables
 from .sampling import grammar_mask, penalty_adds, sample_token, sample_tokens, sample_tokens_async
 from .speculative import VerifyResult, verify_drafts, verify_drafts_async
 
-__all__ = ["BlockManager", "CacheEviction", "Context", "KyroError", "NgramTable", "PagedAttention", "PagedKVCache", "RadixCache", "RequestTables", "StepTables",
-           "context_tails",
-           "VerifyResult", "context", "copy_blocks", "grammar_mask", "lib", "penalty_adds", "rope_tables", "sample_token",
+__all__ = ["BlockManager", "CacheEviction", "Context", "KyroError", "NgramTable", "PagedAttention", "PagedKVCache",
+           "RadixCache", "RequestTables", "StepTables", "VerifyResult", "context_tails", "context", "copy_blocks", "grammar_mask", "lib", "penalty_adds", "rope_tables", "sample_token",
            "sample_tokens", "sample_tokens_async",
            "sync", "verify_drafts", "verify_drafts_async"]
 
