@@ -79,66 +79,11 @@ class PagedAttention:
     def forward_async(self, query, key_cache, value_cache, block_table, context_lens, *,
                       q_start_loc=None, max_q_len=None, causal=True, out_dtype=torch.float32,
                       path="auto", num_splits=0, scale=None, out=None, kv_reuse="auto", schedule="auto",
-                      context=None):
+                      context=None, _groups=None):
         """Queues the kernel on torch's current stream and returns without synchronising.
         Device-detected errors surface at the next ``kyro_amd.sync(device)``. ``context`` (a
         ``kyro_amd._lib.Context``) runs the call on that context and its arena instead of the
         process-wide one of the device."""
-        params, out = self._params(query, key_cache, value_cache, block_table, context_lens, q_start_loc, max_q_len, causal,
-                                   out_dtype, path, num_splits, scale, out, kv_reuse, schedule)
-        index = query.device.index or 0
-        ctx = context if context is not None else _lib.context(index)
-        ctx.set_stream(_lib.current_stream(index))
-        _lib.check(_lib.lib().kyro_paged_attention_mq(
-            ctx.handle, ctypes.byref(params), query.data_ptr(),
-            q_start_loc.data_ptr() if q_start_loc is not None else None,
-            key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
-            context_lens.data_ptr(), out.data_ptr()))
-        return out
-
-    def forward_shared(self, query, key_cache, value_cache, block_table, context_lens, group_starts, group_blocks, *,
-                       q_start_loc=None, max_q_len=None, causal=True, out_dtype=torch.float32, scale=None, out=None,
-                       kv_reuse="auto"):
-        """:meth:`forward` for a batch whose sequences come in groups that hold the same first blocks (a system prompt,
-        a document, the prompt that several samples continue): what a group has in common is read and multiplied once
-        for all its rows. ``group_starts`` (int32 [G + 1]): the sequences of group g are [group_starts[g],
-        group_starts[g + 1]); ``group_blocks`` (int32 [G]): the leading blocks their tables have in common (0: none),
-        which are read from the table of the group's first sequence. :meth:`kyro_amd.BlockManager.prefix_groups`
-        finds both. The result is that of :meth:`forward`, but for rounding, which also takes calls too small for
-        sharing to pay, with the groups unread. Sequences whose context does not
-        reach past the common tokens read their own table. The call synchronises, so errors the device detects raise
-        KyroError here; :meth:`forward_shared_async` is the non-blocking variant."""
-        out = self.forward_shared_async(query, key_cache, value_cache, block_table, context_lens, group_starts,
-                                        group_blocks, q_start_loc=q_start_loc, max_q_len=max_q_len, causal=causal,
-                                        out_dtype=out_dtype, scale=scale, out=out, kv_reuse=kv_reuse)
-        _lib.context(query.device.index or 0).sync()
-        return out
-
-    def forward_shared_async(self, query, key_cache, value_cache, block_table, context_lens, group_starts,
-                             group_blocks, *, q_start_loc=None, max_q_len=None, causal=True, out_dtype=torch.float32,
-                             scale=None, out=None, kv_reuse="auto", context=None):
-        """Queues :meth:`forward_shared` on torch's current stream, as :meth:`forward_async` does."""
-        params, out = self._params(query, key_cache, value_cache, block_table, context_lens, q_start_loc, max_q_len, causal,
-                                   out_dtype, "auto", 0, scale, out, kv_reuse, "auto")
-        dev = query.device
-        _require(group_starts, "group_starts", dtype=torch.int32, ndim=1, device=dev)
-        _require(group_blocks, "group_blocks", dtype=torch.int32, ndim=1, device=dev)
-        groups = group_blocks.shape[0]
-        if group_starts.shape[0] != groups + 1:
-            raise ValueError("group_starts must have one entry more than group_blocks")
-        index = dev.index or 0
-        ctx = context if context is not None else _lib.context(index)
-        ctx.set_stream(_lib.current_stream(index))
-        _lib.check(_lib.lib().kyro_paged_attention_shared(
-            ctx.handle, ctypes.byref(params), groups, query.data_ptr(),
-            q_start_loc.data_ptr() if q_start_loc is not None else None,
-            key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
-            context_lens.data_ptr(), group_starts.data_ptr(), group_blocks.data_ptr(), out.data_ptr()))
-        return out
-
-    def _params(self, query, key_cache, value_cache, block_table, context_lens, q_start_loc, max_q_len, causal, out_dtype,
-                path, num_splits, scale, out, kv_reuse, schedule):
-        """Checks a call's tensors; its params structure and its output."""
         dev = query.device
         if dev.type != "cuda":
             raise ValueError("PagedAttention.forward runs on a GPU device; got " + str(dev))
@@ -197,11 +142,64 @@ class PagedAttention:
             _require(out, "out", dtype=out_dtype, ndim=3, device=dev)
             if tuple(out.shape) != (total_q, h, d):
                 raise ValueError("out has the wrong shape")
-        return _lib.PagedAttentionParams(
+        params = _lib.PagedAttentionParams(
             self.block_size, self.num_heads, self.head_dim, self.num_kv_heads, batch, total_q,
             block_table.shape[1], nb, _DTYPES[query.dtype], _DTYPES[out_dtype], 1 if causal else 0,
             float(scale) if scale else 0.0, _PATHS[path], int(num_splits), int(max_q_len),
-            _KV_REUSE[kv_reuse], _SCHEDULES[schedule]), out
+            _KV_REUSE[kv_reuse], _SCHEDULES[schedule])
+        ctx = context if context is not None else _lib.context(dev.index or 0)
+        ctx.set_stream(_lib.current_stream(dev.index or 0))
+        if _groups is not None:  # forward_shared_async
+            starts, blocks = _groups
+            _lib.check(_lib.lib().kyro_paged_attention_shared(
+                ctx.handle, ctypes.byref(params), blocks.numel(), query.data_ptr(),
+                q_start_loc.data_ptr() if q_start_loc is not None else None,
+                key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
+                context_lens.data_ptr(), starts.data_ptr(), blocks.data_ptr(), out.data_ptr()))
+            return out
+        _lib.check(_lib.lib().kyro_paged_attention_mq(
+            ctx.handle, ctypes.byref(params), query.data_ptr(),
+            q_start_loc.data_ptr() if q_start_loc is not None else None,
+            key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
+            context_lens.data_ptr(), out.data_ptr()))
+        return out
+
+
+    def forward_shared(self, query, key_cache, value_cache, block_table, context_lens, group_starts, group_blocks, *,
+                       q_start_loc=None, max_q_len=None, causal=True, out_dtype=torch.float32, scale=None, out=None,
+                       kv_reuse="auto"):
+        """:meth:`forward` for a batch whose sequences come in groups that hold the same first blocks (a system prompt,
+        a document, the prompt that several samples continue): what a group has in common is read and multiplied once
+        for all its rows. ``group_starts`` (int32 [G + 1]): the sequences of group g are [group_starts[g],
+        group_starts[g + 1]); ``group_blocks`` (int32 [G]): the leading blocks their tables have in common (0: none),
+        which are read from the table of the group's first sequence. :meth:`kyro_amd.BlockManager.prefix_groups`
+        finds both. The result is that of :meth:`forward`, but for rounding, which also takes calls too small for
+        sharing to pay, with the groups unread. Sequences whose context does not
+        reach past the common tokens read their own table. The call synchronises, so errors the device detects raise
+        KyroError here; :meth:`forward_shared_async` is the non-blocking variant."""
+        out = self.forward_shared_async(query, key_cache, value_cache, block_table, context_lens, group_starts,
+                                        group_blocks, q_start_loc=q_start_loc, max_q_len=max_q_len, causal=causal,
+                                        out_dtype=out_dtype, scale=scale, out=out, kv_reuse=kv_reuse)
+        _lib.context(query.device.index or 0).sync()
+        return out
+
+    def forward_shared_async(self, query, key_cache, value_cache, block_table, context_lens, group_starts,
+                             group_blocks, *, q_start_loc=None, max_q_len=None, causal=True, out_dtype=torch.float32,
+                             scale=None, out=None, kv_reuse="auto", context=None):
+        """Queues :meth:`forward_shared` on torch's current stream, as :meth:`forward_async` does."""
+        index = query.get_device()
+        if not (isinstance(group_starts, torch.Tensor) and isinstance(group_blocks, torch.Tensor)
+                and group_starts.dtype is torch.int32 and group_blocks.dtype is torch.int32
+                and group_starts.dim() == 1 and group_blocks.dim() == 1
+                and group_starts.is_contiguous() and group_blocks.is_contiguous()
+                and group_starts.get_device() == index and group_blocks.get_device() == index):
+            _require(group_starts, "group_starts", dtype=torch.int32, ndim=1, device=query.device)
+            _require(group_blocks, "group_blocks", dtype=torch.int32, ndim=1, device=query.device)
+        if group_starts.numel() != group_blocks.numel() + 1:
+            raise ValueError("group_starts must have one entry more than group_blocks")
+        return self.forward_async(query, key_cache, value_cache, block_table, context_lens, q_start_loc=q_start_loc,
+                                  max_q_len=max_q_len, causal=causal, out_dtype=out_dtype, scale=scale, out=out,
+                                  kv_reuse=kv_reuse, context=context, _groups=(group_starts, group_blocks))
 
 
 def describe_attention(attn: PagedAttention, *, batch: int, total_q: int, max_q_len: int, max_blocks_per_seq: int,

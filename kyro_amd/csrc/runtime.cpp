@@ -650,15 +650,20 @@ int shared_check(const kyro_paged_attention_params* p, int32_t num_groups) {
 // 128 in bf16, shared and not: 16 of one row behind 2000 tokens (132 MB if each reads its own) 21.7 us and 16.9, behind
 // 4000 23.4 and 33.0; 16 of 8 rows 27.8 and 27.3, 34.3 and 42.7. In f32, where products are the limit, rows count as
 // well: 24 of 5 rows, 14/2 heads of 96, behind 1000 (38 MB) 38.5 and 34.9, behind 2000 41.9 and 58.2; of one row behind
-// 4000 (149 MB) 41.0 and 35.4. Prompts, whose rows the kernel for many rows does not split over tokens, are not
-// measured by this: 4 of 40 rows behind 1000 take 25.8 and 37.7. The width of the table stands for the contexts,
+// 4000 (149 MB) 41.0 and 35.4, and a wave's 32 rows are mostly empty for 34 sequences of 5 rows with 8 kv heads of 128 and
+// up to 1800 tokens (515 MB): 109 and 46, against 139 and 264 for 63 of 7 rows behind 6400 (2.1 GB). Prompts are split
+// over tokens here and not there: 4 of 40 rows behind 1000 take 25.8 and 37.7, but short ones or up to 80 rows a kv head, 64 of them
+// behind 1600 tokens 22.4 and 15.5, 216 over 390 tokens 22.5 and 16.0. The width of the table stands for the contexts,
 // which the host does not see.
-bool shared_pays(const kyro_paged_attention_params* p) {
+bool shared_pays(const kyro_paged_attention_params* p, bool have_q_start) {
     const bool bf16 = p->dtype == KYRO_BF16;
-    const long long rows = (long long)std::max(p->max_q_len, 1) * (p->num_heads / p->num_kv_heads);
+    if (p->num_kv_heads <= 0) return true;  // refused further on
+    const long long most = p->max_q_len > 0 ? p->max_q_len : have_q_start ? p->total_q : 1;
+    const long long rows = most * (p->num_heads / p->num_kv_heads);
     const double mib = 2.0 * p->batch_size * p->max_blocks_per_seq * p->block_size * p->num_kv_heads * p->head_dim * (bf16 ? 2 : 4) / (1 << 20);
     if (g_test_shared_any_size.load(std::memory_order_relaxed)) return true;
-    return bf16 ? rows > 32 || mib > 128 : rows > 64 || mib > 128 || mib * rows > 1728;
+    if (bf16) return rows <= 32 ? mib > 128 : mib > 32 || (rows > 80 && (long long)p->max_blocks_per_seq * p->block_size > 640);
+    return rows <= 8 ? mib > 512 : rows > 64 || mib > 128 || mib * rows > 1728;
 }
 
 // The params of the launch that takes a call in its place.
@@ -1024,6 +1029,10 @@ int kyro_paged_attention_shared(kyro_ctx ctx, const kyro_paged_attention_params*
                                 const int32_t* group_starts, const int32_t* group_blocks, void* out) {
     return guarded([&]() -> int {
         if (int rc = shared_check(p, num_groups)) return rc;
+        if (ctx && num_groups > 0 && group_starts && group_blocks && !shared_pays(p, q_start_loc != nullptr)) {
+            const kyro_paged_attention_params plain = unshared_params(p);
+            return kyro_paged_attention_mq(ctx, &plain, query, q_start_loc, key_cache, value_cache, block_table, context_lens, out);
+        }
         AttnSetup from;
         if (int rc = attention_setup(p, q_start_loc != nullptr, ctx ? ctx->num_cus : kDefaultCUs, from)) return rc;
         if (from.empty) return check_ctx(ctx);
@@ -1031,8 +1040,7 @@ int kyro_paged_attention_shared(kyro_ctx ctx, const kyro_paged_attention_params*
             (num_groups > 0 && (!group_starts || !group_blocks)))
             return fail(KYRO_EINVAL, "paged_attention_shared: null device pointer");
         if (int rc = check_ctx(ctx)) return rc;  // last, so that a host without a device can have the rest checked
-        SharedSetup r;
-        if (shared_pays(p)) r = shared_setup(p, ctx->num_cus, num_groups, from);
+        SharedSetup r = shared_setup(p, ctx->num_cus, num_groups, from);
         const bool aligned = ((reinterpret_cast<uintptr_t>(key_cache) | reinterpret_cast<uintptr_t>(value_cache)) & 15) == 0;
         if (!r.takes || !aligned) {
             const kyro_paged_attention_params plain = unshared_params(p);

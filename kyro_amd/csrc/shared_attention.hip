@@ -279,18 +279,25 @@ __global__ __launch_bounds__(N) void attn_shared_plan_kernel(SharedArgs s) {
 
 // Merges the partial states of the listed row groups. A workgroup takes a slice of one row group's (row, four
 // columns) for one kv head, rows fastest, so that the lanes read the neighbouring rows that a state keeps together.
-template <int DR>
+// WAYS of its threads share one such item's states: where row groups are of few rows, workgroups are few and states many
+// (a row of 32 sequences behind 32768 tokens has 64: 6.8 us for 11.0). With 32 rows a sequence there are workgroups enough,
+// and four threads an item take 14.0 for 10.5.
+template <int DR, int WAYS>
 __global__ __launch_bounds__(kThreads) void attn_shared_combine_kernel(SharedArgs s) {
     const AttnArgs& a = s.a;
-    constexpr int DT = (DR + 31) / 32, Q = DR / 4;
+    constexpr int DT = (DR + 31) / 32, Q = DR / 4, kItems = kThreads / WAYS;
+    __shared__ float merged[WAYS > 1 ? WAYS - 1 : 1][6][kItems];
+    const int item = (int)threadIdx.x % kItems, way = (int)threadIdx.x / kItems;
     const int entry = (int)blockIdx.x / a.Hkv, kvh = (int)blockIdx.x - entry * a.Hkv;
     const int used = s.head[1];
     const int4 e = s.merges[2 * entry], f = s.merges[2 * entry + 1];
     if (entry >= used) return;
     const int rows = min(kPrefillRows, e.y * a.group - e.z);
-    const int x = (int)blockIdx.y * kThreads + threadIdx.x;
-    if (x >= rows * Q) return;
-    const int c = x / rows, r = x - c * rows;  // columns 4 c .. 4 c + 3 of row e.z + r
+    if (rows <= 0) return;
+    const int x = (int)blockIdx.y * kItems + item;
+    if (WAYS == 1 && x >= rows * Q) return;
+    const bool some = x < rows * Q;
+    const int c = some ? x / rows : 0, r = some ? x - c * rows : 0;  // columns 4 c .. 4 c + 3 of row e.z + r
     const int dt = c / 8, k = c / 2 % 4, h = c % 2;
     // The row's partial states: `common` ones over common tokens, then own ones.
     size_t at_common = 0;
@@ -311,7 +318,7 @@ __global__ __launch_bounds__(kThreads) void attn_shared_combine_kernel(SharedArg
     // are worth more than more loads of each: 8 took 28 us for 23 of 1600 prompt rows, and 20 for 17 of 128 requests,
     // though 9 for 11 where 128 rows have 64 states each.
     constexpr int kBatch = 4;
-    for (int i0 = 0; i0 < n; i0 += kBatch) {
+    for (int i0 = way * kBatch; i0 < n; i0 += WAYS * kBatch) {
         float m[kBatch], l[kBatch];
         float4 v[kBatch];
 #pragma unroll
@@ -344,6 +351,30 @@ __global__ __launch_bounds__(kThreads) void attn_shared_combine_kernel(SharedArg
             o.w += w * v[i].w;
         }
     }
+    if constexpr (WAYS > 1) {
+        if (way > 0) {
+            const float held[6] = {M, L, o.x, o.y, o.z, o.w};
+#pragma unroll
+            for (int k = 0; k < 6; ++k) merged[way - 1][k][item] = held[k];
+        }
+        __syncthreads();
+        if (way > 0 || !some) return;
+        float mb = M;
+#pragma unroll
+        for (int w = 0; w < WAYS - 1; ++w) mb = fmaxf(mb, merged[w][0][item]);
+        const float mref = mb == kNegInf ? 0.f : mb;
+        const float old = fast_exp2(M - mref);
+        L *= old, o.x *= old, o.y *= old, o.z *= old, o.w *= old;
+#pragma unroll
+        for (int w = 0; w < WAYS - 1; ++w) {
+            const float f = fast_exp2(merged[w][0][item] - mref);
+            L += f * merged[w][1][item];
+            o.x += f * merged[w][2][item];
+            o.y += f * merged[w][3][item];
+            o.z += f * merged[w][4][item];
+            o.w += f * merged[w][5][item];
+        }
+    }
     const float inv = L > 0.f ? 1.f / L : 0.f;
     SeqInfo si;
     si.q0 = e.x;
@@ -351,12 +382,15 @@ __global__ __launch_bounds__(kThreads) void attn_shared_combine_kernel(SharedArg
     store_row4<DR>(a, out_row(a, si, e.z + r), 4 * c, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
+constexpr int kSharedFewRows = 8;  // of a kv head: up to so many, four threads an item
+
 template <int DR>
 void launch_combine(const SharedArgs& s, hipStream_t stream) {
     const AttnArgs& a = s.a;
-    const int rows = a.rows_cap < kPrefillRows ? a.rows_cap : kPrefillRows;
-    attn_shared_combine_kernel<DR><<<dim3((unsigned)((long long)s.own_cap * a.Hkv), (unsigned)((rows * (DR / 4) + kThreads - 1) / kThreads)),
-                                     kThreads, 0, stream>>>(s);
+    const int rows = a.rows_cap < kPrefillRows ? a.rows_cap : kPrefillRows, items = rows * (DR / 4);
+    const unsigned groups = (unsigned)((long long)s.own_cap * a.Hkv);
+    if (rows <= kSharedFewRows) attn_shared_combine_kernel<DR, 4><<<dim3(groups, (unsigned)((items + 63) / 64)), kThreads, 0, stream>>>(s);
+    else attn_shared_combine_kernel<DR, 1><<<dim3(groups, (unsigned)((items + kThreads - 1) / kThreads)), kThreads, 0, stream>>>(s);
 }
 
 }  // namespace

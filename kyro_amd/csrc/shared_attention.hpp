@@ -27,7 +27,7 @@ namespace {
 template <bool BF16, int DR>
 __global__ __launch_bounds__(kPfThreads, shared_wgs_per_cu(BF16, DR)) void attn_shared_kernel(SharedArgs s) {
     using C = PfCfg<BF16, DR>;
-    constexpr bool PIPE = BF16 && DR <= 128;
+    constexpr bool PIPE = shared_pipelined(BF16, DR);
     const AttnArgs& a = s.a;
     // An object for each buffer: the compiler's waits tell copies into one from reads of the other by the object.
     __shared__ uint4 sK0[C::NS * C::SLAB], sK1[C::NS * C::SLAB];
