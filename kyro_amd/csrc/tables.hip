@@ -8,7 +8,7 @@
 // (tables_fill_kernel), or, where they are few, by the first one right away, which saves the second launch.
 //
 // What bounds it: latency. One request: 4.8 us, 64 with tables of 264 blocks and 8 rows each: 10.7 in one launch (6.7 + 3.6
-// in two, and 3.4 more of the host), both less than the call from Python (11.9). 264 entries with tables of 8192 blocks, 28 MB
+// in two, and 3.4 more of the host), both less than the call from Python (11.6). 264 entries with tables of 8192 blocks, 28 MB
 // to move: 4.2 + 8.6, the second at 3.3 TB/s. Rows that stay: 3.8 us for 64 requests, 7.1 for 1024.
 #include "common.hpp"
 
