@@ -1,6 +1,7 @@
 // C ABI of the block manager, the prefix cache, the device block-table writer and block copies
 // (include/kyro_blocks.h), and of the accumulated attention weights and the eviction by them
-// (include/kyro_evict.h), and of the block tables that live on the GPU (include/kyro_tables.h). Host logic lives in block_manager.cpp; this file validates arguments,
+// (include/kyro_evict.h), and of the block tables that live on the GPU (include/kyro_tables.h).
+// Host logic lives in block_manager.cpp; this file validates arguments,
 // converts statuses and queues the device work on the context's stream.
 #include <algorithm>
 #include <cmath>

@@ -264,7 +264,7 @@ __host__ __device__ constexpr bool shared_pipelined(bool bf16, int D) { return b
 __host__ __device__ constexpr int shared_wgs_per_cu(bool bf16, int D) { return D <= 64 ? 3 : 2; }
 constexpr int kSharedAll = 1 << 30;  // in an entry's tiles: common tokens, which every row sees
 // A unit is a row group (128 rows of one kv head) over a group's common tokens, or of a sequence over its own. The units
-// of a kv head, the common ones first, lie on a line, each as long as its tiles and shared_unit_cost more, which is cut
+// of a kv head, the common ones first, lie on a line, each as long as its tiles and kSharedUnitCost more, which is cut
 // into equal shares, one for each of the head's workgroups. What a unit costs beside its tiles (its queries, the
 // first copies, its state) is near 3 tiles' time: 64 sequences that verify 8 rows take 93.0 us with 3, 94.2 with 2
 // and 94.5 with 4; decode 51.9, 51.5 and 51.5. A tile costs the same over common tokens, where the matrix unit is the

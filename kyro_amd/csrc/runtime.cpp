@@ -652,15 +652,16 @@ int shared_check(const kyro_paged_attention_params* p, int32_t num_groups) {
 // well: 24 of 5 rows, 14/2 heads of 96, behind 1000 (38 MB) 38.5 and 34.9, behind 2000 41.9 and 58.2; of one row behind
 // 4000 (149 MB) 41.0 and 35.4, and a wave's 32 rows are mostly empty for 34 sequences of 5 rows with 8 kv heads of 128 and
 // up to 1800 tokens (515 MB): 109 and 46, against 139 and 264 for 63 of 7 rows behind 6400 (2.1 GB). Prompts are split
-// over tokens here and not there: 4 of 40 rows behind 1000 take 25.8 and 37.7, but short ones or up to 80 rows a kv head, 64 of them
-// behind 1600 tokens 22.4 and 15.5, 216 over 390 tokens 22.5 and 16.0. The width of the table stands for the contexts,
-// which the host does not see.
+// over tokens here and not there, 4 of 40 rows behind 1000 take 25.8 and 37.7; but up to 80 rows a kv head, or short
+// contexts, are faster there: 5 sequences of 64 rows of 1600 tokens 22.4 and 15.5, 4 of up to 216 over 390 tokens 22.5 and
+// 16.0. The width of the table stands for the contexts, which the host does not see.
 bool shared_pays(const kyro_paged_attention_params* p, bool have_q_start) {
     const bool bf16 = p->dtype == KYRO_BF16;
     if (p->num_kv_heads <= 0) return true;  // refused further on
     const long long most = p->max_q_len > 0 ? p->max_q_len : have_q_start ? p->total_q : 1;
     const long long rows = most * (p->num_heads / p->num_kv_heads);
-    const double mib = 2.0 * p->batch_size * p->max_blocks_per_seq * p->block_size * p->num_kv_heads * p->head_dim * (bf16 ? 2 : 4) / (1 << 20);
+    const double mib = 2.0 * p->batch_size * p->max_blocks_per_seq * p->block_size * p->num_kv_heads * p->head_dim *
+                       (bf16 ? 2 : 4) / (1 << 20);
     if (g_test_shared_any_size.load(std::memory_order_relaxed)) return true;
     if (bf16) return rows <= 32 ? mib > 128 : mib > 32 || (rows > 80 && (long long)p->max_blocks_per_seq * p->block_size > 640);
     return rows <= 8 ? mib > 512 : rows > 64 || mib > 128 || mib * rows > 1728;

@@ -199,3 +199,36 @@ def test_a_captured_step_against_an_eager_one(gpu):
             assert torch.equal(a, b)
         s.check(step, out, new, *host[1:4])
         s.stay(new, (accepted[:-1] + 1).tolist(), *host[2:4])
+
+
+def test_two_contexts_at_once(gpu):
+    """Batches that differ, on two streams with a context and so scratch each: what each gives alone."""
+    gen = torch.Generator().manual_seed(9)
+    attn = PagedAttention(BS, H, D, HKV)
+
+    def batch(B, common, own, rows):
+        blocks = common + own
+        table = torch.randperm(B * blocks, generator=gen).view(B, blocks)
+        table[:, :common] = table[0, :common]
+        caches = torch.randn((2, B * blocks, HKV, BS, D), generator=gen).to(torch.bfloat16).to(gpu)
+        q = torch.randn((B * rows, H, D), generator=gen).to(torch.bfloat16).to(gpu)
+        i32 = dict(dtype=torch.int32, device=gpu)
+        return ((q, caches[0], caches[1], table.to(gpu), torch.full((B,), blocks * BS - 3, device=gpu),
+                 torch.tensor([0, B], **i32), torch.tensor([common], **i32)),
+                dict(q_start_loc=torch.arange(0, B * rows + 1, rows, **i32), max_q_len=rows))
+
+    batches = [batch(24, 60, 9, 2), batch(5, 100, 40, 7)]
+    alone = [attn.forward_shared(*args, **kw) for args, kw in batches]
+    streams = [torch.cuda.Stream(gpu) for _ in batches]
+    contexts = [kyro_amd.Context(0) for _ in batches]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(10):
+        for i, (args, kw) in enumerate(batches):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(attn.forward_shared_async(*args, context=contexts[i], **kw))
+    torch.cuda.synchronize()
+    for c in contexts:
+        c.sync()
+    for i in range(2):
+        assert all(torch.equal(x, alone[i]) for x in outs[i])
