@@ -268,8 +268,9 @@ int kyro_paged_attention_plan(const kyro_paged_attention_params* params, int num
  * as for kyro_paged_attention_mq, with path and schedule AUTO and num_splits 0. Geometries that the kernel for many
  * query rows does not take (block sizes that are no multiple of 16, other head dims, caches off a 16-byte boundary)
  * run as kyro_paged_attention_mq runs them, with the groups unread, and so do calls of few rows whose tables are too
- * small for sharing to pay (128 MiB of K and V that they could name, less in f32). Groups that are read
- * and out of range or order latch KYRO_EINVAL for the next kyro_sync, and the sequences are computed without them.
+ * small for sharing to pay (in bf16 up to 32 rows a kv head of each sequence and 128 MiB of K and V that the tables could
+ * name; in f32 by rows and bytes). Groups that are read and out of range or order latch KYRO_EINVAL for the
+ * next kyro_sync, and the sequences are computed without them.
  */
 int kyro_paged_attention_shared(kyro_ctx ctx, const kyro_paged_attention_params* params, int32_t num_groups,
                                 const void* query, const int32_t* q_start_loc, const void* key_cache,

@@ -294,7 +294,7 @@ __global__ __launch_bounds__(kPfThreads, shared_wgs_per_cu(BF16, DR)) void attn_
                 // the one after that to k0.
                 auto turn = [&](int i, uint4* k0, uint4* k1, uint4* v0, uint4* v1, f32x16* now, f32x16* next) {
                     // The two workgroups of a CU take turns at being first: left alone the older one is, and the other one
-                    // still runs when it has ended (c2).
+                    // still runs when it has ended (512 rows a kv head over 32768 common tokens: 309 us for 319).
                     if (younger == (now == S)) __builtin_amdgcn_s_setprio(1);
                     else __builtin_amdgcn_s_setprio(0);
                     landed();
