@@ -16,7 +16,7 @@
 //   32 of 1 row behind 32768, 20 to 300 of their own                    5.5 + 34.1 +  6.8   156 MB: 24
 //   8 of 100 to 300 rows behind 6000                                    6.3 + 181  + 17.5   160 GFLOP: 134 at 1.2 PFLOP/s
 // The first and third stream: 4.7 TB/s over the main kernel, whose workgroups' states (64 KiB each, 33 MB) are written and
-// read beside that. The second and fourth multiply at half of the dense peak while they run (shared_attention.hpp).
+// read beside that. What bounds the others stands at the loop (shared_attention.hpp).
 // Common tokens are taken in whole tiles (64 tokens, 32 in f32 and above head dim 128), so that no tile needs a
 // mask at its start; what is left of the last one counts as each sequence's own.
 #include "attention_rows.hpp"

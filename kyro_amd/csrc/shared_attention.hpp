@@ -7,11 +7,13 @@
 // while its maxima are found, those of tile i's output; K of tile i + 2 and V of tile i + 1 are on their way. A wave alone
 // on its SIMD then has something for the matrix unit at any time but at its barriers.
 //
-// Cycles of a tile of 64 tokens (64 sequences of 8 rows, all tokens common, head dim 128, two workgroups a CU, per wave): 32 products of
-// 32 each, 1024; 32 exponentials of 16, and 108 other vector operations of 4, 950; the CU's LDS delivers both
-// workgroups' operands in 2048 of 128 bytes and takes their copies in 512. A step takes 2100 in the workgroup that is
-// first, 2900 in the other; the copies never make it wait. So 0.6 of the matrix unit while both run. 32768 common tokens
-// (275 GFLOP) take 290 us, 0.95 PFLOP/s, and more once some milliseconds of such calls have lowered the clock.
+// Cycles of a tile of 64 tokens for a wave (64 sequences of 8 rows, all tokens common, head dim 128, two workgroups a CU): 32
+// products of 32 each, 1024; 32 exponentials of 16 and 108 other vector operations of 4, 950. A step takes 2100 in the
+// workgroup that is first, 2900 in the other; the copies never make it wait. Counters over 32768 common tokens (275 GFLOP,
+// 285 us, 0.97 PFLOP/s at a clock that has fallen to 1.86 GHz): matrix units busy in 0.50 of the cycles, vector operations
+// issued in 0.50, LDS active in 0.25 without a bank conflict. Other orders of the products (both halves' scores in turn
+// before the outputs) and more operands in flight were level. 8 rows beside 100 to 1500 own tokens: 0.24, 0.30, 0.12 and
+// 3.7 TB/s from memory; what waits there is the latency of own tokens' tiles, of which a workgroup has one on its way.
 // What one unit takes beside its tiles (its entry, ids, K, first scores, state: 12 us alone) is hidden by the CU's other
 // workgroup: loading all of the next unit's while the last tile is worked out changed nothing.
 #pragma once
@@ -294,7 +296,7 @@ __global__ __launch_bounds__(kPfThreads, shared_wgs_per_cu(BF16, DR)) void attn_
                 // the one after that to k0.
                 auto turn = [&](int i, uint4* k0, uint4* k1, uint4* v0, uint4* v1, f32x16* now, f32x16* next) {
                     // The two workgroups of a CU take turns at being first: left alone the older one is, and the other one
-                    // still runs when it has ended (512 rows a kv head over 32768 common tokens: 309 us for 319).
+                    // still runs when it has ended (2048 rows a kv head over 32768 common tokens: 309 us for 319).
                     if (younger == (now == S)) __builtin_amdgcn_s_setprio(1);
                     else __builtin_amdgcn_s_setprio(0);
                     landed();
