@@ -260,8 +260,9 @@ int kyro_paged_attention_plan(const kyro_paged_attention_params* params, int num
  *   group_starts [num_groups + 1] int32: the sequences of group g are [group_starts[g], group_starts[g+1]);
  *     sequences of no group, and those before the first and behind the last, share nothing
  *   group_blocks [num_groups] int32: the leading blocks that the tables of all its sequences have in common (0: none).
- *     The table of its first sequence is read for them: that the others' are the same is the caller's to see to
- *     (kyro_bm_prefix_groups finds groups so).
+ *     The table of the first of its sequences that reads them together (below) is read for them: that the others'
+ *     are the same is the caller's to see to (kyro_bm_prefix_groups finds groups so). One that is left out, with
+ *     context length 0, need not name them.
  * Groups are ranges of the batch, so its sequences are to be ordered by prefix. A sequence whose context does not
  * reach past its group's common tokens with every row (with causal, ctx - q_len + 1 of them) reads its own table
  * instead, and a group whose common tokens are not worth a pass of their own is computed as if it had none. params

@@ -172,8 +172,8 @@ class PagedAttention:
         a document, the prompt that several samples continue): what a group has in common is read and multiplied once
         for all its rows. ``group_starts`` (int32 [G + 1]): the sequences of group g are [group_starts[g],
         group_starts[g + 1]); ``group_blocks`` (int32 [G]): the leading blocks their tables have in common (0: none),
-        which are read from the table of the group's first sequence. :meth:`kyro_amd.BlockManager.prefix_groups`
-        finds both. The result is that of :meth:`forward`, but for rounding, which also takes calls too small for
+        which are read from the table of the first sequence that shares them (one without a context, as padding, need
+        not name them). :meth:`kyro_amd.BlockManager.prefix_groups` finds both. The result is that of :meth:`forward`, but for rounding, which also takes calls too small for
         sharing to pay, with the groups unread. Sequences whose context does not
         reach past the common tokens read their own table. The call synchronises, so errors the device detects raise
         KyroError here; :meth:`forward_shared_async` is the non-blocking variant."""

@@ -294,6 +294,7 @@ struct SharedArgs {
     int2* counts;                   // [G] {sequences that share, their row groups}
     int2* places;                   // [G] {place on the line, first unit or -1}
     int* bases;                     // [B] first own unit
+    int* firsts;                    // [G] first sequence that shares, whose table is read for the common tokens
     int* head;                      // {workgroups of a kv head in use, own units}
     int G, tile_shift;              // tokens of a tile: 1 << tile_shift
     int merge_cost;                 // kSharedMergeCost

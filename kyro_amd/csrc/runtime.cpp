@@ -595,6 +595,7 @@ size_t shared_workspace(SharedSetup& r, char* base) {
     take(s.counts, (size_t)s.G);
     take(s.places, (size_t)s.G);
     take(s.bases, (size_t)s.a.B);
+    take(s.firsts, (size_t)s.G);
     take(s.a.ws_m, r.part_rows);
     take(s.a.ws_l, r.part_rows);
     take(s.a.ws_acc, r.part_rows * ((size_t)(s.a.D + 31) / 32 * 32));

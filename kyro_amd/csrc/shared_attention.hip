@@ -77,13 +77,14 @@ __global__ __launch_bounds__(N) void attn_shared_plan_kernel(SharedArgs s) {
     __shared__ int l_starts[kHeld + 1], l_rows[kHeld + 1], l_base[kHeld];
     __shared__ int4 l_seqs[kHeld], l_units[kHeld];
     __shared__ int2 l_counts[kHeld], l_places[kHeld];
-    __shared__ int l_blocks[kHeld], bad_groups;
+    __shared__ int l_blocks[kHeld], l_firsts[kHeld], bad_groups;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int32_t* const starts = ONE ? l_starts : s.group_starts;     // first sequences of the groups
     int4* const seqs = ONE ? l_seqs : s.seqs;                          // {first row, rows, context length, group or -1}
     int2* const counts = ONE ? l_counts : s.counts;                    // {sequences that share, their row groups}
     int2* const places = ONE ? l_places : s.places;                    // {place on the line, first unit or -1}
     int* const base = ONE ? l_base : s.bases;                          // first own unit
+    int* const firsts = ONE ? l_firsts : s.firsts;                     // first sequence that shares
     BlockSums<N, 3> sums{part};
     auto each = [&](int n, auto&& f) {
         if constexpr (ONE) {
@@ -115,6 +116,7 @@ __global__ __launch_bounds__(N) void attn_shared_plan_kernel(SharedArgs s) {
             if (s0 < 0 || s1 < s0 || s1 > a.B) bad_groups = 1;
             if (nb < 0 || nb > a.max_blocks) err |= ERR_GROUPS;
             counts[g] = make_int2(0, 0);
+            firsts[g] = INT32_MAX;
             if (ONE) {
                 l_starts[g] = s0;
                 l_blocks[g] = nb;
@@ -154,6 +156,7 @@ __global__ __launch_bounds__(N) void attn_shared_plan_kernel(SharedArgs s) {
             seqs[b].w = g;
             atomicAdd(&counts[g].x, 1);
             atomicAdd(&counts[g].y, row_groups_of(s, e.y));
+            atomicMin(&firsts[g], b);
         }
     });
     if (!ONE) __threadfence();  // atomics on scratch
@@ -251,7 +254,7 @@ __global__ __launch_bounds__(N) void attn_shared_plan_kernel(SharedArgs s) {
             if (x == r * most) s.common_parts[u] = make_int2(u + p.first_piece(), p.pieces());
             if (w > p.last) continue;
             const int from = p.cut(w - 1), to = p.cut(w);
-            put(p, u, w, make_int4(from < to ? starts[g] : -1, gr.x, gr.y, gr.z << s.tile_shift),
+            put(p, u, w, make_int4(from < to ? firsts[g] : -1, gr.x, gr.y, gr.z << s.tile_shift),
                 make_int4(r * kPrefillRows, from, (to - from) | kSharedAll, u + w));
         }
     }

@@ -232,3 +232,27 @@ def test_two_contexts_at_once(gpu):
         c.sync()
     for i in range(2):
         assert all(torch.equal(x, alone[i]) for x in outs[i])
+
+
+@pytest.mark.parametrize("B", [6, 400])
+def test_a_group_whose_first_sequence_is_left_out(gpu, B):
+    """As kyro_tables_extend leaves an entry that the pool had no room for, or padding: no context, no blocks. The others
+    read the common tokens all the same."""
+    gen = torch.Generator().manual_seed(B)
+    attn = PagedAttention(BS, H, D, HKV)
+    common, own = 20, 3
+    table = torch.randperm(B * (common + own), generator=gen).view(B, -1) + 1
+    table[:, :common] = table[1, :common]
+    lens = torch.full((B,), (common + own) * BS - 5)
+    table[0], lens[0] = 0, 0
+    caches = torch.randn((2, B * (common + own) + 1, HKV, BS, D), generator=gen).to(torch.bfloat16).to(gpu)
+    q = torch.randn((B, H, D), generator=gen).to(torch.bfloat16).to(gpu)
+    groups = [torch.tensor(x, dtype=torch.int32, device=gpu) for x in ([0, B], [common])]
+    args = q, caches[0], caches[1], table.to(gpu), lens.to(gpu)
+    got = attn.forward_shared(*args, *groups)
+    q, k, v = (x.float() for x in args[:3])
+    exact, size = attn.forward(q, k, v, *args[3:]), attn.forward(q, k, v.abs(), *args[3:])
+    # A weight is rounded once, by at most 2^-8 of it; sums in 32 bits, here and in `exact`, add less than 2^-11 of their
+    # terms' size.
+    assert ((got - exact).abs() <= (2.0 ** -8 + 2.0 ** -11) * size).all()
+    assert not got[0].any() and exact[1:].any()
