@@ -84,25 +84,24 @@ __device__ __forceinline__ int check_count(const TablesArgs& a, int n) {
     return -1;
 }
 
-// Entries i, i + STRIDE, .. below `to` of the table row of entry e; a block that is new is the request's from now on. The
+// Entries i, i + stride, .. below `to` of the table row of entry e; a block that is new is the request's from now on. The
 // loads of kFillBatch entries are in flight together: one without a block loads what is there anyway.
 constexpr int kFillBatch = 8;
-template <int STRIDE>
-__device__ __forceinline__ void fill_blocks(const TablesArgs& a, const Entry& e, int b, int i, int to) {
+__device__ __forceinline__ void fill_blocks(const TablesArgs& a, const Entry& e, int b, int i, int to, int stride) {
     int64_t* own = a.blocks + (size_t)max(e.row, 0) * a.state_blocks;
     int64_t* table = a.table + (size_t)b * a.width;
     const int total = e.row >= 0 ? e.total : 0;
-    for (; i < to; i += kFillBatch * STRIDE) {
+    for (; i < to; i += kFillBatch * stride) {
         int64_t id[kFillBatch];
 #pragma unroll
         for (int k = 0; k < kFillBatch; ++k) {
-            const int x = i + k * STRIDE;
+            const int x = i + k * stride;
             const int64_t* from = x < total && x >= e.held ? a.pool + (e.base - (x - e.held)) : own + (x < total ? x : 0);
             id[k] = *from;
         }
 #pragma unroll
         for (int k = 0; k < kFillBatch; ++k) {
-            const int x = i + k * STRIDE;
+            const int x = i + k * stride;
             if (x >= to) continue;
             if (x < total && (id[k] < 0 || id[k] >= a.num_blocks)) latch_error(a.err, ERR_BLOCK_ID);
             if (x < total && x >= e.held) own[x] = id[k];
@@ -138,7 +137,8 @@ __device__ __forceinline__ int entry_of_row(int B, int64_t i, Start&& start) {
     return lo;
 }
 
-// ONE: the whole call (at most kTabThreads entries), whose table rows a wave each fills.
+// ONE: the whole call (at most kTabThreads entries). A wave fills a table row, or several of them that are short: 375 rows
+// of 6 blocks took 34.8 us a call with one row a wave; now such calls are bound by the host like the others.
 template <bool ONE>
 __global__ __launch_bounds__(kTabThreads) void tables_extend_kernel(TablesArgs a) {
     extern __shared__ uint32_t names_lds[];
@@ -221,7 +221,10 @@ __global__ __launch_bounds__(kTabThreads) void tables_extend_kernel(TablesArgs a
     __syncthreads();
     if (threadIdx.x == 0 && taken > 0) *a.pool_count = count - taken;
     if (!ONE) return;
-    for (int b = threadIdx.x >> 6; b < a.B; b += kTabWaves) fill_blocks<64>(a, held[b], b, threadIdx.x & 63, a.width);
+    int shift = 0;  // log2 of a row's lanes
+    while (shift < 6 && kFillBatch << shift < a.width) ++shift;
+    for (int b = threadIdx.x >> shift; b < a.B; b += kTabThreads >> shift)
+        fill_blocks(a, held[b], b, threadIdx.x & ((1 << shift) - 1), a.width, 1 << shift);
     if (!a.positions && !a.slots) return;
     for (int i = threadIdx.x; i < a.max_rows; i += kTabThreads) {
         const int b = entry_of_row(a.B, i, [&](int x) -> int64_t { return x < a.B ? held[x].q0 : (int64_t)held[a.B - 1].q0 + held[a.B - 1].rows; });
@@ -235,7 +238,7 @@ __global__ __launch_bounds__(kFillThreads) void tables_fill_kernel(TablesArgs a)
         const int chunks = (a.width + kFillEntries - 1) / kFillEntries;
         const int b = (int)(blockIdx.x / chunks), c = (int)(blockIdx.x - (unsigned)b * chunks);
         const Entry e = entries[b];
-        fill_blocks<kFillThreads>(a, e, b, c * kFillEntries + threadIdx.x, min(a.width, (c + 1) * kFillEntries));
+        fill_blocks(a, e, b, c * kFillEntries + threadIdx.x, min(a.width, (c + 1) * kFillEntries), kFillThreads);
         return;
     }
     // The entries of the workgroup's rows, whose starts it takes to LDS unless many without rows lie between them.
