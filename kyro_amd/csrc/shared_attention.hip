@@ -282,9 +282,10 @@ __global__ __launch_bounds__(N) void attn_shared_plan_kernel(SharedArgs s) {
 
 // Merges the partial states of the listed row groups. A workgroup takes a slice of one row group's (row, four
 // columns) for one kv head, rows fastest, so that the lanes read the neighbouring rows that a state keeps together.
-// WAYS of its threads share one such item's states: where row groups are of few rows, workgroups are few and states many
-// (a row of 32 sequences behind 32768 tokens has 64: 6.8 us for 11.0). With 32 rows a sequence there are workgroups enough,
-// and four threads an item take 14.0 for 10.5.
+// WAYS of its threads share one such item's states: where items are few, states are many (a row of 32 sequences behind 32768
+// tokens with 8 kv heads has 64: 6.8 us for 11.0; one of 8 sequences of 8 rows with one kv head has more than 100, and the
+// whole call takes 33 us for 47). With the 524288 items of 64 sequences of 32 rows there are workgroups enough, and
+// four threads an item take 14.0 for 10.5.
 template <int DR, int WAYS>
 __global__ __launch_bounds__(kThreads) void attn_shared_combine_kernel(SharedArgs s) {
     const AttnArgs& a = s.a;
@@ -385,14 +386,14 @@ __global__ __launch_bounds__(kThreads) void attn_shared_combine_kernel(SharedArg
     store_row4<DR>(a, out_row(a, si, e.z + r), 4 * c, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-constexpr int kSharedFewRows = 8;  // of a kv head: up to so many, four threads an item
+constexpr long long kSharedFewItems = 1 << 18;  // of all row groups: up to so many, four threads an item
 
 template <int DR>
 void launch_combine(const SharedArgs& s, hipStream_t stream) {
     const AttnArgs& a = s.a;
     const int rows = a.rows_cap < kPrefillRows ? a.rows_cap : kPrefillRows, items = rows * (DR / 4);
     const unsigned groups = (unsigned)((long long)s.own_cap * a.Hkv);
-    if (rows <= kSharedFewRows) attn_shared_combine_kernel<DR, 4><<<dim3(groups, (unsigned)((items + 63) / 64)), kThreads, 0, stream>>>(s);
+    if ((long long)groups * items <= kSharedFewItems) attn_shared_combine_kernel<DR, 4><<<dim3(groups, (unsigned)((items + 63) / 64)), kThreads, 0, stream>>>(s);
     else attn_shared_combine_kernel<DR, 1><<<dim3(groups, (unsigned)((items + kThreads - 1) / kThreads)), kThreads, 0, stream>>>(s);
 }
 
