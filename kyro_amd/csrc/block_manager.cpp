@@ -350,60 +350,104 @@ std::vector<std::pair<int64_t, int64_t>> BlockManager::take_copies() {
     return out;
 }
 
-// Sorted, lists with a common start are neighbours, and the runs of neighbours that share at least d blocks nest. They
-// are walked innermost first with a stack of the open ones. Where a run with d blocks in common ends, each run (or list)
-// right inside it, of n lists whose own groups leave out s, either keeps those groups or joins the one group of
-// the run, to which it adds n d; the group as a whole leaves out d less than its parts add.
+// Sorted, lists with a common start are neighbours, and the runs of neighbours that share at least d blocks nest: a tree,
+// whose node of d blocks has lists and deeper runs below it. Some of its nodes are opened as groups. A list leaves out most
+// in the deepest open node above it, all d of whose blocks it has in common, and an open node reads them once. So with a
+// the blocks of the nearest open node above v, the most that the lists below v leave out is
+//   f(v, a) = max(v's lists * a + sum of f(run, a),  (v's lists - 1) * d + sum of f(run, d)),
+// worked out from the innermost runs for each node above v as the nearest open one. Those are fewer than v has blocks, so
+// that all of it takes no more room or time than the lists.
 std::vector<PrefixGroup> prefix_groups(const std::vector<const std::vector<int64_t>*>& lists) {
-    struct Part {
-        std::vector<PrefixGroup> groups;
-        int64_t n, saved;
-    };
-    struct Run {
+    struct Node {
         int64_t blocks;
-        std::vector<Part> parts;
-    };
-    auto close = [](Run& run) -> Part {
-        int64_t apart = 0, joined = -run.blocks, n = 0;
-        for (const Part& p : run.parts) {
-            apart += p.saved;
-            joined += std::max(p.saved, p.n * run.blocks);
-            n += p.n;
-        }
-        Part out{{}, n, std::max(apart, joined)};
-        PrefixGroup group{{}, run.blocks};
-        for (Part& p : run.parts)
-            for (PrefixGroup& g : p.groups) {
-                if (joined > apart && p.saved <= p.n * run.blocks)
-                    group.members.insert(group.members.end(), g.members.begin(), g.members.end());
-                else out.groups.push_back(std::move(g));
-            }
-        if (!group.members.empty()) out.groups.push_back(std::move(group));
-        return out;
+        std::vector<int32_t> lists, runs;  // by place in the sorted order; nodes
+        int32_t parent = -1, level = 0;    // nodes above it
+        int32_t open_below = 0;            // it opens where the nearest open node above is at a lower level than this
+        int32_t nearest = 0, group = -1;   // that node's level; the group of its lists, -1: each by itself
     };
     const size_t n = lists.size();
     std::vector<int32_t> order(n);
     for (size_t i = 0; i < n; ++i) order[i] = (int32_t)i;
     std::stable_sort(order.begin(), order.end(), [&](int32_t a, int32_t b) { return *lists[(size_t)a] < *lists[(size_t)b]; });
-    std::vector<Run> open;
-    open.push_back({0, {}});
+    // The tree, runs before what they lie in, the root of no blocks last.
+    std::vector<Node> nodes, open(1);
+    open[0].blocks = 0;
     for (size_t i = 0; i < n; ++i) {
-        Part last{{{{order[i]}, 0}}, 1, 0};  // what has just ended: the list by itself, or a run up to it
-        int64_t d = 0;                       // blocks in common with the next list
+        int64_t d = 0;  // blocks in common with the next list
         if (i + 1 < n) {
             const std::vector<int64_t>&a = *lists[(size_t)order[i]], &b = *lists[(size_t)order[i + 1]];
             const size_t m = std::min(a.size(), b.size());
             d = std::mismatch(a.begin(), a.begin() + (ptrdiff_t)m, b.begin()).first - a.begin();
         }
+        int32_t run = -1;  // what has just ended: the list, or a run up to it
+        auto put = [&](Node& to) { run < 0 ? to.lists.push_back((int32_t)i) : to.runs.push_back(run); };
         while (open.back().blocks > d) {
-            open.back().parts.push_back(std::move(last));
-            last = close(open.back());
+            put(open.back());
+            run = (int32_t)nodes.size();
+            nodes.push_back(std::move(open.back()));
             open.pop_back();
         }
-        if (open.back().blocks < d) open.push_back({d, {}});
-        open.back().parts.push_back(std::move(last));
+        if (open.back().blocks < d) {
+            open.emplace_back();
+            open.back().blocks = d;
+        }
+        put(open.back());
     }
-    return close(open.back()).groups;
+    nodes.push_back(std::move(open.back()));
+    for (size_t v = nodes.size(); v-- > 0;)
+        for (const int32_t r : nodes[v].runs) {
+            nodes[(size_t)r].parent = (int32_t)v;
+            nodes[(size_t)r].level = nodes[v].level + 1;
+        }
+    // best[v][j]: f(v, a) for the node at level j above v as the nearest open one.
+    std::vector<std::vector<int64_t>> best(nodes.size());
+    for (size_t v = 0; v + 1 < nodes.size(); ++v) {
+        Node& node = nodes[v];
+        best[v].resize((size_t)node.level);
+        int64_t opened = ((int64_t)node.lists.size() - 1) * node.blocks;
+        for (const int32_t r : node.runs) opened += best[(size_t)r][(size_t)node.level];
+        int32_t above = node.parent;
+        for (int32_t j = node.level; j-- > 0; above = nodes[(size_t)above].parent) {
+            int64_t apart = (int64_t)node.lists.size() * nodes[(size_t)above].blocks;
+            for (const int32_t r : node.runs) apart += best[(size_t)r][(size_t)j];
+            best[v][(size_t)j] = std::max(apart, opened);
+            if (opened > apart && node.open_below == 0) node.open_below = j + 1;  // apart falls with j
+        }
+        for (const int32_t r : node.runs) std::vector<int64_t>().swap(best[(size_t)r]);
+    }
+    // From the root: which nodes open, and the group of each list.
+    std::vector<int64_t> group_blocks;
+    std::vector<int32_t> group_of(n, -1);
+    for (size_t v = nodes.size(); v-- > 0;) {
+        Node& node = nodes[v];
+        if (node.parent >= 0) {
+            const Node& above = nodes[(size_t)node.parent];
+            node.nearest = above.nearest;
+            node.group = above.group;
+            if (node.nearest < node.open_below) {
+                node.nearest = node.level;
+                node.group = (int32_t)group_blocks.size();
+                group_blocks.push_back(node.blocks);
+            }
+        }
+        for (const int32_t i : node.lists) group_of[(size_t)i] = node.group;
+    }
+    // In the order of each group's first list.
+    std::vector<PrefixGroup> groups;
+    std::vector<int32_t> place(group_blocks.size(), -1);
+    for (size_t i = 0; i < n; ++i) {
+        const int32_t g = group_of[i];
+        if (g < 0) {
+            groups.push_back({{order[i]}, 0});
+            continue;
+        }
+        if (place[(size_t)g] < 0) {
+            place[(size_t)g] = (int32_t)groups.size();
+            groups.push_back({{}, group_blocks[(size_t)g]});
+        }
+        groups[(size_t)place[(size_t)g]].members.push_back(order[i]);
+    }
+    return groups;
 }
 
 }  // namespace bm
