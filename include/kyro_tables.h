@@ -73,10 +73,10 @@ int kyro_tables_extend(kyro_ctx ctx, const kyro_tables_params* params, const int
  *   requests[r].tokens = context_lens[b] - m + k; blocks behind ceil(tokens / block_size) and behind the
  *   request's shared ones go back to the pool, in the order of the batch and then of the request;
  *   out_context_lens[b] = requests[r].tokens.
- * An entry without rows keeps its length, whatever kept holds; one that kyro_tables_extend left out, or padding,
- * is left alone and gets 0. k outside [0, m], and what extend refuses of state rows and records, latch
- * KYRO_EINVAL, and the entry is left alone; so does a pool that would pass its capacity, and then no block moves
- * and no record changes. out_context_lens may be context_lens.
+ * An entry without rows keeps its length, whatever kept holds. One of context length 0 (kyro_tables_extend left it
+ * out, it is padding, or an empty request without rows) is left alone and gets 0. k outside [0, m], and what extend
+ * refuses of state rows and records, latch KYRO_EINVAL, and the entry is left alone; so does a pool that would pass
+ * its capacity, and then no block moves and no record changes. out_context_lens may be context_lens.
  */
 int kyro_tables_keep(kyro_ctx ctx, const kyro_tables_params* params, const int32_t* state_rows,
                      const int64_t* context_lens, const int32_t* q_start_loc, const int32_t* kept,

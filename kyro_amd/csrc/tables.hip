@@ -310,8 +310,10 @@ __global__ __launch_bounds__(kTabThreads) void tables_shrink_kernel(TablesArgs a
         if (x.q0 < 0 || m < 0 || k < 0 || k > m) {
             latch_error(a.err, ERR_Q_LAYOUT);
             s.r = -1;
+        } else if (x.c == 0) {
+            s.r = -1;  // extend left the entry out, with rows or none, or the request is empty and brings none
         } else if (x.c < m || x.c - m + k > (int64_t)x.rec.y * a.bs) {
-            if (x.c != 0) latch_error(a.err, ERR_CTX_LEN);  // 0: extend left the entry out
+            latch_error(a.err, ERR_CTX_LEN);
             s.r = -1;
         } else {
             s.tokens = (int)(x.c - m + k);

@@ -185,7 +185,7 @@ class RequestTables:
         """Of a step's rows (``context_lens`` and ``q_start_loc`` as :meth:`extend` gave them) the first ``kept`` (int32
         [B]) + ``plus`` of each entry stay: the requests' lengths count them, and blocks behind them go back to the pool.
         After :func:`kyro_amd.verify_drafts` that is ``res.accepted`` and 1. Returns the lengths that stay (int64
-        [B], 0 for an entry that extend left out); ``out`` may be ``context_lens``. The call synchronises, so
+        [B], 0 for an entry of context length 0, as extend leaves one out, whose request is left alone); ``out`` may be ``context_lens``. The call synchronises, so
         errors the device detects raise KyroError here."""
         out = self.keep_async(state_rows, context_lens, q_start_loc, kept, plus=plus, out=out)
         _lib.context(self.device.index or 0).sync()
