@@ -317,7 +317,8 @@ __global__ __launch_bounds__(kTabThreads) void tables_shrink_kernel(TablesArgs a
             s.r = -1;
         } else {
             s.tokens = (int)(x.c - m + k);
-            s.stay = min(x.rec.y, max(x.rec.z, (s.tokens + a.bs - 1) / a.bs));
+            // Both are below 2^31, their sum below 2^32.
+            s.stay = min(x.rec.y, max(x.rec.z, (int)(((unsigned)s.tokens + (unsigned)a.bs - 1u) / (unsigned)a.bs)));
         }
         return s;
     };

@@ -82,3 +82,15 @@ def test_keep_of_entries_without_rows(gpu, rows):
     before[3] += 2
     before[0][2, 1] = 2
     assert same(t, before)
+
+
+def test_lengths_near_two_to_the_31(gpu):
+    """A block of 1.5e9 tokens: length and block size together pass 31 bits."""
+    bs, tokens = 1_500_000_000, 1_400_000_000
+    t = RequestTables.new(bs, rows=1, max_blocks=1, pool=[0], num_blocks=1, device=gpu)
+    t.requests[0] = i32([tokens, 1, 0, 0], gpu)
+    t.pool_count.zero_()
+    step = t.extend(None, i32([3], gpu), total_q=3)
+    assert step.context_lens.tolist() == [tokens + 3] and step.slots.tolist() == [tokens, tokens + 1, tokens + 2]
+    assert t.keep(None, step.context_lens, step.q_start_loc, i32([2], gpu)).tolist() == [tokens + 2]
+    assert t.requests.tolist() == [[tokens + 2, 1, 0, 0]] and t.pool_count.item() == 0
