@@ -58,7 +58,8 @@ typedef struct kyro_tables_params {
  *     block * block_size + offset in the caches; -1 behind the last row. Either may be NULL.
  * An entry that the pool has no blocks left for (in the order of the batch: the sum of what it and those before it
  * need exceeds *pool_count, and it needs some) gets none: context length 0, a zero row of block_table, positions and
- * slots of -1, while q_start_loc keeps its rows. It latches KYRO_ENOSPACE for the next kyro_sync. So do, as
+ * slots of -1, while q_start_loc keeps its rows. It latches KYRO_ENOSPACE for the next kyro_sync, also if that comes
+ * behind the rest of the step, whose appends skip its rows. So do, as
  * KYRO_EINVAL, a state row that is out of range or named twice, a request whose record is not one, a length past
  * max_state_blocks or max_blocks_per_seq, new_rows < 0 (counted as 0) and rows past max_rows.
  */

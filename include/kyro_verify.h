@@ -393,7 +393,8 @@ typedef struct kyro_kv_append_params {
  *   key_cache, value_cache [num_blocks, Hkv, block_size, D]  cache_dtype (written in place; a bf16 row widens exactly into an f32 cache)
  * Only the new rows' slots are written. Two sequences must not map a new row to the same slot
  * (shared prefix blocks hold only old tokens). A bad block id, context length or q_start_loc
- * latches KYRO_EINVAL for the next kyro_sync and the offending rows are not written.
+ * latches KYRO_EINVAL for the next kyro_sync and the offending rows are not written (rows of a sequence of context
+ * length 0 leave the KYRO_ENOSPACE of a kyro_tables_extend that had no blocks for it).
  */
 int kyro_paged_kv_append(kyro_ctx ctx, const kyro_kv_append_params* params,
                          const void* key, const void* value, const int32_t* q_start_loc,
@@ -444,7 +445,8 @@ typedef struct kyro_qkv_append_params {
  *   cos, sin [max_position, R/2] f32 (R = 0: NULL); q_weight, k_weight [D] weight_dtype, both or neither
  *   out_query may be query itself where that is contiguous and of cache_dtype; it overlaps no other input
  * Pointers are on 16-byte boundaries. Rows of no sequence are left alone. A bad block id, context length,
- * q_start_loc or position latches KYRO_EINVAL for the next kyro_sync, and such a row is not written.
+ * q_start_loc or position latches KYRO_EINVAL for the next kyro_sync, and such a row is not written (a context
+ * length of 0: as for kyro_paged_kv_append).
  */
 int kyro_qkv_append(kyro_ctx ctx, const kyro_qkv_append_params* params, const void* query, const void* key,
                     const void* value, const int32_t* q_start_loc, const int64_t* positions,

@@ -20,7 +20,8 @@ enum ErrorBits : int {
     ERR_REQUEST = 512,  // tables: a request's record whose numbers do not fit each other
     ERR_POOL = 1024,    // tables: pool_count outside [0, pool_capacity], or blocks that would pass it
     ERR_NO_BLOCKS = 2048, // tables: the pool has too few blocks (KYRO_ENOSPACE)
-    ERR_GROUPS = 4096   // shared attention: group_starts not monotone or out of range, or group_blocks out of range
+    ERR_GROUPS = 4096,  // shared attention: group_starts not monotone or out of range, or group_blocks out of range
+    ERR_CTX_EMPTY = 8192 // append: rows of a sequence of context length 0, as the tables leave one without blocks
 };
 
 

@@ -92,7 +92,7 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvAppendArgs a) {
         return;
     }
     if (ctx < q_len || ctx > (int64_t)a.max_blocks * a.bs) {
-        if (lead) latch_error(a.err, ERR_CTX_LEN);
+        if (lead) latch_error(a.err, ctx == 0 ? ERR_CTX_EMPTY : ERR_CTX_LEN);
         return;
     }
     const int v = blockIdx.x * kThreads + (int)threadIdx.x;  // 8-element vector within the rows

@@ -171,7 +171,7 @@ __global__ __launch_bounds__(kThreads) void qkv_append_kernel(QkvAppendArgs a) {
     }
     const int64_t ctx = a.ctx_lens[b];
     if (ctx < r1 - r0 || ctx > (int64_t)a.max_blocks * a.bs) {
-        if (lane == 0) latch_error(a.err, ERR_CTX_LEN);
+        if (lane == 0) latch_error(a.err, ctx == 0 ? ERR_CTX_EMPTY : ERR_CTX_LEN);
         return;
     }
     const int slot = (int)(ctx - (r1 - r0) + (r - r0));  // below max_blocks * bs, which fits

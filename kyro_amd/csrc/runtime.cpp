@@ -136,9 +136,11 @@ int sync_and_report(kyro_ctx ctx) {
     KYRO_HIP(hipMemcpy(&err, ctx->err, sizeof(int), hipMemcpyDeviceToHost));
     if (err == 0) return KYRO_OK;
     KYRO_HIP(hipMemset(ctx->err, 0, sizeof(int)));
+    // The rows of a request that the pool had no blocks for are skipped by the appends of its step: that is no error beside it.
+    const bool no_space = (err & kyro::ERR_NO_BLOCKS) && !(err & ~(kyro::ERR_NO_BLOCKS | kyro::ERR_CTX_EMPTY));
     std::string msg = "device-side validation failed:";
     if (err & kyro::ERR_BLOCK_ID) msg += " block_table entry outside [0, num_blocks);";
-    if (err & kyro::ERR_CTX_LEN)
+    if (!no_space && (err & (kyro::ERR_CTX_LEN | kyro::ERR_CTX_EMPTY)))
         msg += " context length < 0 or > max_blocks_per_seq * block_size (or max_tokens, or below the rows of an append);";
     if (err & kyro::ERR_Q_LAYOUT) msg += " q_start_loc not monotone / out of range, or q_len > max_q_len;";
     if (err & kyro::ERR_TOKEN) msg += " a draft, bias or penalty token id >= vocab_size, or a mask_row >= num_masks;";
@@ -153,7 +155,7 @@ int sync_and_report(kyro_ctx ctx) {
     if (err & kyro::ERR_POOL) msg += " pool_count outside [0, pool_capacity], or more blocks than the pool holds;";
     if (err & kyro::ERR_GROUPS) msg += " group_starts not monotone / out of range, or group_blocks out of range;";
     if (err & kyro::ERR_NO_BLOCKS) msg += " not enough free blocks in the pool;";
-    return fail(err == kyro::ERR_NO_BLOCKS ? KYRO_ENOSPACE : KYRO_EINVAL, "%s", msg.c_str());
+    return fail(no_space ? KYRO_ENOSPACE : KYRO_EINVAL, "%s", msg.c_str());
 }
 
 }  // namespace
