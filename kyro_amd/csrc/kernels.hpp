@@ -272,10 +272,9 @@ constexpr int kSharedAll = 1 << 30;  // in an entry's tiles: common tokens, whic
 // limit, as over own ones, where it is memory: weights of 3 : 2 put small units of many sequences into one share and
 // made each batch slower.
 constexpr int kSharedUnitCost = 3;
-// Tiles below which a cut is moved to the unit's end: 2 for 1 took 24.7 us for 22.9 where 4 samples share 1000
-// tokens, 52.5 for 42.4 in f32, whose tiles are long, and the others within 3 %.
-constexpr int kSharedLeastPart = 1;
-constexpr int kSharedLeastShare = kSharedUnitCost + 2 * kSharedLeastPart;
+// A piece of a unit may be one tile: moving cuts so that none is shorter than two took 24.7 us for 22.9 where 4 samples
+// share 1000 tokens, 52.5 for 42.4 in f32, whose tiles are long, and the others within 3 %. A share is two tiles at least.
+constexpr int kSharedLeastShare = kSharedUnitCost + 2;
 // Tiles that a unit costs more where a group shares: its state is written and merged. 8 prompts of 100 to 300 rows behind
 // 6000 tokens, which save 4 of 54 row groups, take 205 us shared and 202 not, 64 sequences of 30 rows behind 4096
 // (4 of 64) 230 and 214, 4 prompts of 75 rows behind 6000 (2 of 12) 59.6 and 62.9: all at 4.5 to 6.

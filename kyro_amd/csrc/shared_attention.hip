@@ -41,8 +41,9 @@ __device__ __forceinline__ int row_groups_of(const SharedArgs& s, int rows) {
 }
 
 // A unit of T tiles at `at` on the line whose shares are `share` long: workgroups first .. last hold a piece
-// of it, and cut(w) is the tile where the piece of workgroup w + 1 begins. Cuts near an end are moved to it, so that
-// no piece is a few tiles; the pieces that are left follow each other (a share is longer than what two cuts are moved).
+// of it, and cut(w) is the tile where the piece of workgroup w + 1 begins. A cut inside the unit's fixed cost, which is at
+// its start, is moved to the first tile, and workgroup `first` then has no piece; a share is longer than that cost, so
+// that the other cuts lie between tiles and the pieces follow each other.
 struct Pieces {
     int at, share, T, first, last;
     __device__ Pieces(int pos, int tiles, int len) : at(pos), share(len), T(tiles) {
@@ -53,11 +54,10 @@ struct Pieces {
     __device__ int cut(int w) const {
         if (w < first) return 0;
         if (w >= last) return T;
-        const int k = (w + 1) * share - at - kSharedUnitCost;
-        return k < kSharedLeastPart ? 0 : k > T - kSharedLeastPart ? T : k;
+        return max((w + 1) * share - at - kSharedUnitCost, 0);  // below T: workgroup w + 1 begins before end()
     }
     __device__ int first_piece() const { return first + (first < last && cut(first) == 0); }
-    __device__ int pieces() const { return last - (first < last && cut(last - 1) == T) + 1 - first_piece(); }
+    __device__ int pieces() const { return last - first_piece() + 1; }
     // Whether the line's share w begins, or ends, in the unit.
     __device__ bool begins(int w) const { return w * share >= at; }
     __device__ bool ends(int w, int line) const { return w < last || (w + 1) * share == end() || end() == line; }

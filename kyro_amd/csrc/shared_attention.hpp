@@ -55,7 +55,7 @@ __global__ __launch_bounds__(kPfThreads, shared_wgs_per_cu(BF16, DR)) void attn_
         const bool first = u == range.x;
         const int4 e0 = first ? first0 : s.list[2 * (u + wg)], e1 = first ? first1 : s.list[2 * (u + wg) + 1];
         const int b = __builtin_amdgcn_readfirstlane(e0.x);
-        if (b < 0) continue;  // the unit begins or ends a few tiles past this workgroup's share
+        if (b < 0) continue;  // this workgroup's share of the unit has no tile of it
         const int ctx = __builtin_amdgcn_readfirstlane(e0.w);
         const int row0 = __builtin_amdgcn_readfirstlane(e1.x);
         const int tile0 = __builtin_amdgcn_readfirstlane(e1.y);
