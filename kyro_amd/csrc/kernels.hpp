@@ -260,9 +260,11 @@ hipError_t launch_attention_prefill(const PrefillArgs& p, hipStream_t stream);
 // this one's weights, and the workgroups of the kernel a CU holds (registers, and LDS). At head dim 64 a tile has as much
 // vector work as products, and three workgroups without that pipeline are no slower than two with it: prompts 149 us
 // either way, decode of 64 behind 8192 tokens 36.2 for 40.3, 78 sequences of up to 700 tokens with 32 heads 54.6 for 63.8
-// (four: 150, 38.2, 54.0). At 80 and 96 they are: 176 us for 162 and 180 for 170, though 62 for 67 and 66 for 77.
+// (four: 150, 38.2, 54.0). At 80 and 96 they are: 176 us for 162 and 180 for 170, though 62 for 67 and 66 for 77. In f32 a
+// third leaves too few registers for sums in short chains (27 spilled): 63 sequences of 7 rows behind 3200 tokens, 16/8
+// heads, 133 us for 125, though 8 prompts of 200 rows behind 6000 391 for 398.
 __host__ __device__ constexpr bool shared_pipelined(bool bf16, int D) { return bf16 && D > 64 && D <= 128; }
-__host__ __device__ constexpr int shared_wgs_per_cu(bool bf16, int D) { return D <= 64 ? 3 : 2; }
+__host__ __device__ constexpr int shared_wgs_per_cu(bool bf16, int D) { return bf16 && D <= 64 ? 3 : 2; }
 constexpr int kSharedAll = 1 << 30;  // in an entry's tiles: common tokens, which every row sees
 // A unit is a row group (128 rows of one kv head) over a group's common tokens, or of a sequence over its own. The units
 // of a kv head, the common ones first, lie on a line, each as long as its tiles and kSharedUnitCost more, which is cut

@@ -45,7 +45,9 @@ struct PfCfg {
     // against 64 bits is then level with the vector kernel's over 33 to 4000 tokens (prompts of 200 tokens,
     // head dims 64 / 80 / 96 / 112, 1e-7: 1.15 1.22 1.24 1.23 here, 1.16 1.22 1.26 1.23 there; with two
     // chains per score, as at 128, 1.82 at 112). At head dim 128 two long chains per score and one per
-    // output are already closer than the one-block kernel's single chain (1.89 against 2.80).
+    // output are already closer than the one-block kernel's single chain (1.89 against 2.80). Over shared prefixes (160
+    // sequences of 400 tokens, the same head dims; chains of 8 in a score, 4 in an output): 1.75 1.87 1.89 1.85 here, 1.76
+    // 1.84 1.92 1.87 there; 2.23 2.49 2.56 2.62 with the chains of head dim 128, which are 1.03 to 1.11 times as fast.
     static constexpr bool TREE = !BF16 && DR < 128;
     // K rows: chunk c of token t sits in slot c ^ swk(t) of its column group, so that the 16
     // tokens of an operand read (same c) spread over all banks.
@@ -129,18 +131,21 @@ __device__ __forceinline__ f32x16 mfma_bf16(const uint4& x, const uint4& y, cons
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), z, 0, 0, 0);
 }
 
+__device__ __forceinline__ f32x16 zeros() {
+    f32x16 z;
+#pragma unroll
+    for (int x = 0; x < 16; ++x) z[x] = 0.f;
+    return z;
+}
+
 // S^T of 32 tokens (those of tt) of a tile: K at kb in LDS, the wave's rows in q.
 template <class C>
 __device__ __forceinline__ f32x16 tile_scores(const char* kb, const uint4* q, const TileLane<C>& at, int tt) {
-    f32x16 half[2];
-#pragma unroll
-    for (int y = 0; y < 2; ++y)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) half[y][x] = 0.f;
     if constexpr (C::BF) {
+        f32x16 sum = zeros();
 #pragma unroll
         for (int s = 0; s < C::KS; ++s)
-            half[0] = mfma_bf16(k_operand<C>(kb, at, tt, s), q[s], half[0]);
+            sum = mfma_bf16(k_operand<C>(kb, at, tt, s), q[s], sum);
         // Keep operand reads in flight ahead of the products (the compiler's own order waits for each).
         constexpr int kAhead = C::R < 256 ? 4 : 1;
         __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
@@ -150,16 +155,31 @@ __device__ __forceinline__ f32x16 tile_scores(const char* kb, const uint4* q, co
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
-        return half[0];
+        return sum;
     } else {
+        // Two chains of additions; with TREE two new ones of eight for every four steps, which are then added up.
+        constexpr int kSteps = C::TREE ? 4 : C::KS;
+        f32x16 sum, chain[2] = {zeros(), zeros()};
 #pragma unroll
         for (int s = 0; s < C::KS; ++s) {
-            const f32x4 kf = __builtin_bit_cast(f32x4, k_operand<C>(kb, at, tt, s)), qf = __builtin_bit_cast(f32x4, q[s]);
+            const f32x4 kf = __builtin_bit_cast(f32x4, k_operand<C>(kb, at, tt, s));
+            f32x4 qf = __builtin_bit_cast(f32x4, q[s]);
+            if (s > 0 && s % kSteps == 0) {
+                // The products behind depend on the sum before them. Left alone the compiler puts all additions at the
+                // end, with every chain in registers of its own: 295 spilled at head dim 112, where this spills none.
+                float q0 = qf[0], q1 = qf[1];
+                asm volatile("" : "+v"(sum), "+v"(q0), "+v"(q1));
+                qf[0] = q0;
+                qf[1] = q1;
+            }
 #pragma unroll
-            for (int e = 0; e < 4; ++e)  // two chains of additions
-                half[e % 2] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[e], qf[e], half[e % 2], 0, 0, 0);
+            for (int e = 0; e < 4; ++e) chain[e % 2] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[e], qf[e], chain[e % 2], 0, 0, 0);
+            if ((s + 1) % kSteps != 0 && s + 1 < C::KS) continue;
+            if (s < kSteps) sum = chain[0] + chain[1];
+            else sum += chain[0] + chain[1];
+            chain[0] = chain[1] = zeros();
         }
-        return half[0] + half[1];
+        return sum;
     }
 }
 
@@ -182,27 +202,43 @@ __device__ __forceinline__ void tile_output(const char* vb, const f32x16& p, con
     } else {
         // A tile's products are summed on their own and then added: the chain of additions into O^T is one per tile
         // instead of one per two tokens.
-        constexpr int W = 2;  // column tiles side by side
+        // With TREE that sum is one of four chains of four, two at a time.
+        auto product = [&](int dt, int x, const f32x16& to) -> f32x16 {
+            const float vv = *reinterpret_cast<const float*>(vb + at.v32 + (2 * tt + x / 8) * (C::SLAB * 16) + (8 * dt / C::CW) * kTileGroupBytes<C> +
+                                                             (8 * ((x / 4) % 2) + x % 4) * (C::CW * 16) + (8 * dt % C::CW) * 16);
+            return __builtin_amdgcn_mfma_f32_32x32x2f32(vv, p[x], to, 0, 0, 0);
+        };
+        if constexpr (C::TREE) {
 #pragma unroll
-        for (int d0 = 0; d0 < C::DT; d0 += W) {
-            f32x16 sum[W];
+            for (int dt = 0; dt < C::DT; ++dt) {
+                f32x16 sum;
 #pragma unroll
-            for (int w = 0; w < W; ++w)
+                for (int y = 0; y < 2; ++y) {
+                    f32x16 chain[2] = {zeros(), zeros()};
 #pragma unroll
-                for (int x = 0; x < 16; ++x) sum[w][x] = 0.f;
-#pragma unroll
-            for (int x = 0; x < 16; ++x)
-#pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    if (d0 + w >= C::DT) continue;
-                    const float vv = *reinterpret_cast<const float*>(
-                        vb + at.v32 + (2 * tt + x / 8) * (C::SLAB * 16) + (8 * (d0 + w) / C::CW) * kTileGroupBytes<C> +
-                        (8 * ((x / 4) % 2) + x % 4) * (C::CW * 16) + (8 * (d0 + w) % C::CW) * 16);
-                    sum[w] = __builtin_amdgcn_mfma_f32_32x32x2f32(vv, p[x], sum[w], 0, 0, 0);
+                    for (int x = 8 * y; x < 8 * y + 8; ++x) chain[x % 2] = product(dt, x, chain[x % 2]);
+                    if (y == 0) sum = chain[0] + chain[1];
+                    else sum += chain[0] + chain[1];
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+                o[dt] += sum;
+            }
+        } else {
+            constexpr int W = 2;  // column tiles side by side
 #pragma unroll
-            for (int w = 0; w < W; ++w)
-                if (d0 + w < C::DT) o[d0 + w] += sum[w];
+            for (int d0 = 0; d0 < C::DT; d0 += W) {
+                f32x16 sum[W];
+#pragma unroll
+                for (int w = 0; w < W; ++w) sum[w] = zeros();
+#pragma unroll
+                for (int x = 0; x < 16; ++x)
+#pragma unroll
+                    for (int w = 0; w < W; ++w)
+                        if (d0 + w < C::DT) sum[w] = product(d0 + w, x, sum[w]);
+#pragma unroll
+                for (int w = 0; w < W; ++w)
+                    if (d0 + w < C::DT) o[d0 + w] += sum[w];
+            }
         }
     }
 }
