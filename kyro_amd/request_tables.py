@@ -96,11 +96,11 @@ class RequestTables:
         elif entries > self.requests.shape[0]:
             raise ValueError("without state_rows every entry of the batch needs a request of the state")
 
-    def _context(self):
+    def _context(self, context=None):
         idx = self._index
         if idx < 0:
             raise ValueError("RequestTables runs on a GPU device; got " + str(self.device))
-        ctx = _lib.context(idx)
+        ctx = context if context is not None else _lib.context(idx)
         ctx.set_stream(_lib.current_stream(idx))
         return ctx
 
@@ -108,8 +108,11 @@ class RequestTables:
         return _lib.pack_tables(self.block_size, entries, width, self.requests.shape[0], self.blocks.shape[1],
                                 self.num_blocks, self.pool.shape[0], max_rows, plus)
 
-    def extend_async(self, state_rows, new_rows, *, total_q, max_blocks_per_seq=None, out=None) -> StepTables:
-        """Queues the work on torch's current stream; see :meth:`extend`."""
+    def extend_async(self, state_rows, new_rows, *, total_q, max_blocks_per_seq=None, out=None,
+                     context=None) -> StepTables:
+        """Queues the work on torch's current stream; see :meth:`extend`. ``context`` (a ``kyro_amd.Context``) runs
+        the call on that context and its arena instead of the process-wide one, for programs that keep a context a
+        stream."""
         if not isinstance(new_rows, torch.Tensor):
             raise TypeError("new_rows must be a torch.Tensor")
         entries = new_rows.shape[0] if new_rows.dim() == 1 else -1
@@ -138,7 +141,7 @@ class RequestTables:
             out.positions.fill_(-1)
             out.slots.fill_(-1)
             return out
-        ctx = self._context()
+        ctx = self._context(context)
         _lib.check(_lib.lib().kyro_tables_extend(
             ctx.handle, self._params(entries, width, total_q), None if state_rows is None else state_rows.data_ptr(),
             new_rows.data_ptr(), self.requests.data_ptr(), self.blocks.data_ptr(), self.pool.data_ptr(),
@@ -159,8 +162,8 @@ class RequestTables:
         _lib.context(self.device.index or 0).sync()
         return step
 
-    def keep_async(self, state_rows, context_lens, q_start_loc, kept, *, plus=0, out=None):
-        """Queues the work on torch's current stream; see :meth:`keep`."""
+    def keep_async(self, state_rows, context_lens, q_start_loc, kept, *, plus=0, out=None, context=None):
+        """Queues the work on torch's current stream; see :meth:`keep` (``context`` as for :meth:`extend_async`)."""
         if not isinstance(context_lens, torch.Tensor):
             raise TypeError("context_lens must be a torch.Tensor")
         entries = context_lens.shape[0] if context_lens.dim() == 1 else -1
@@ -174,7 +177,7 @@ class RequestTables:
             self._vector(out, "out", torch.int64, entries)
         if entries == 0:
             return out
-        ctx = self._context()
+        ctx = self._context(context)
         _lib.check(_lib.lib().kyro_tables_keep(
             ctx.handle, self._params(entries, plus=int(plus)), None if state_rows is None else state_rows.data_ptr(),
             context_lens.data_ptr(), q_start_loc.data_ptr(), kept.data_ptr(), self.requests.data_ptr(),
@@ -191,15 +194,15 @@ class RequestTables:
         _lib.context(self.device.index or 0).sync()
         return out
 
-    def release_async(self, state_rows) -> None:
-        """Queues the work on torch's current stream; see :meth:`release`."""
+    def release_async(self, state_rows, *, context=None) -> None:
+        """Queues the work on torch's current stream; see :meth:`release` (``context`` as for :meth:`extend_async`)."""
         if not isinstance(state_rows, torch.Tensor):
             raise TypeError("state_rows must be a torch.Tensor")
         entries = state_rows.shape[0] if state_rows.dim() == 1 else -1
         self._batch(state_rows, entries)
         if entries == 0:
             return
-        ctx = self._context()
+        ctx = self._context(context)
         _lib.check(_lib.lib().kyro_tables_release(
             ctx.handle, self._params(entries), state_rows.data_ptr(), self.requests.data_ptr(), self.blocks.data_ptr(),
             self.pool.data_ptr(), self.pool_count.data_ptr()))
