@@ -36,10 +36,10 @@ extern "C" {
 
 typedef struct kyro_tables_params {
     int32_t block_size;          /* tokens per block */
-    int32_t batch_size;          /* B */
-    int32_t max_blocks_per_seq;  /* width of block_table (extend) */
+    int32_t batch_size;          /* B, below 2^24 */
+    int32_t max_blocks_per_seq;  /* width of block_table (extend), at most 2^31 - 2048 */
     int32_t num_state_rows;      /* requests the state holds, at most 131072 */
-    int32_t max_state_blocks;    /* blocks a request may hold */
+    int32_t max_state_blocks;    /* blocks a request may hold: at most 2^31 - 2048, and below 2^31 tokens */
     int32_t num_blocks;          /* leading dim of the caches; ids outside [0, num_blocks) latch KYRO_EINVAL */
     int32_t pool_capacity;
     int32_t max_rows;            /* entries of positions and slots (extend): rows of the step */

@@ -647,6 +647,8 @@ int tables_setup(const kyro_tables_params* p, const char* call, bool extend, con
         return fail(KYRO_EINVAL, "%s: sizes must be positive (batch_size, pool_capacity, max_rows >= 0)", call);
     if (p->num_state_rows > kyro::kTablesMaxRows)
         return fail(KYRO_EUNSUPPORTED, "%s: num_state_rows %d (at most %d)", call, p->num_state_rows, kyro::kTablesMaxRows);
+    if (p->max_state_blocks > kyro::kTablesMaxWidth || (extend && p->max_blocks_per_seq > kyro::kTablesMaxWidth))
+        return fail(KYRO_EUNSUPPORTED, "%s: rows of at most %d blocks", call, kyro::kTablesMaxWidth);
     if ((int64_t)p->max_state_blocks * p->block_size > INT32_MAX)
         return fail(KYRO_EUNSUPPORTED, "%s: a request of more than 2^31 tokens (max_state_blocks x block_size)", call);
     if (!state_rows && p->batch_size > p->num_state_rows)
@@ -751,6 +753,7 @@ int kyro_tables_keep(kyro_ctx ctx, const kyro_tables_params* params, const int32
         mem.add("kept", kept, (uint64_t)a.B * 4, false);
         mem.add("out_context_lens", out_context_lens, (uint64_t)a.B * 8, true);
         if (int rc = mem.check(call)) return rc;
+        if (a.B > (int)(0xffffffffu / 256)) return too_large(call);  // as for the others, with a workgroup an entry
         if (int rc = check_ctx(ctx)) return rc;
         DeviceGuard dg(ctx->device);
         KYRO_HIP(dg.status);

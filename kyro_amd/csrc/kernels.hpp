@@ -480,6 +480,7 @@ struct alignas(16) TablesEntry {
     char bytes[kTablesEntryBytes];
 };
 constexpr int kTablesMaxRows = 131072;  // requests of a state: two bits each in LDS
+constexpr int kTablesMaxWidth = INT32_MAX - 2047;  // entries of a table row: its last 2048 end below 2^31
 // Batches whose tables have up to so many entries and whose rows are up to so many are one launch.
 constexpr int kTablesOneEntries = 32768;
 constexpr int kTablesOneRows = 4096;

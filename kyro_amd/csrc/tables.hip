@@ -20,6 +20,7 @@ constexpr int kTabThreads = 1024;
 constexpr int kTabWaves = kTabThreads / 64;
 constexpr int kFillThreads = 256;
 constexpr int kFillEntries = 2048;  // table entries or freed blocks of one fill workgroup
+static_assert(kTablesMaxWidth + (int64_t)kFillEntries <= (int64_t)INT32_MAX + 1, "ends of workgroups in 32 bits");
 constexpr int kFillRows = 512;      // rows of one fill workgroup: what a row reads follows from what it read before
 
 // What the scan hands to the fill, for each entry of the batch.
