@@ -19,7 +19,7 @@
  *   pool       [pool_capacity] int64            ids of free blocks, a stack:
  *   pool_count [1] int32                        its first *pool_count entries
  * Entry b of a batch is request r = state_rows[b] (NULL: r = b). A negative r is padding: no request, of context
- * length 0. Two entries may not name one request.
+ * length 0. Two entries may not name one request. With batch_size 0 no call reads or writes anything.
  * Sums over the batch follow its order, so that results do not depend on the order of execution.
  */
 #ifndef KYRO_TABLES_H

@@ -173,10 +173,12 @@ class PagedAttention:
         for all its rows. ``group_starts`` (int32 [G + 1]): the sequences of group g are [group_starts[g],
         group_starts[g + 1]); ``group_blocks`` (int32 [G]): the leading blocks their tables have in common (0: none),
         which are read from the table of the first sequence that shares them (one without a context, as padding, need
-        not name them). :meth:`kyro_amd.BlockManager.prefix_groups` finds both. The result is that of :meth:`forward`, but for rounding, which also takes calls too small for
-        sharing to pay, with the groups unread. Sequences whose context does not
-        reach past the common tokens read their own table. The call synchronises, so errors the device detects raise
-        KyroError here; :meth:`forward_shared_async` is the non-blocking variant."""
+        not name them). :meth:`kyro_amd.BlockManager.prefix_groups` finds both. The result is that of :meth:`forward`, but
+        for rounding, which also takes calls too small for sharing to pay, with the groups unread; that is told from the
+        width of ``block_table``, so on tables much wider than the contexts, and where own tokens outweigh the common
+        ones, :meth:`forward` can be faster. Sequences whose context does not reach past the common tokens read their own
+        table. The call synchronises, so errors the device detects raise KyroError here; :meth:`forward_shared_async` is
+        the non-blocking variant."""
         out = self.forward_shared_async(query, key_cache, value_cache, block_table, context_lens, group_starts,
                                         group_blocks, q_start_loc=q_start_loc, max_q_len=max_q_len, causal=causal,
                                         out_dtype=out_dtype, scale=scale, out=out, kv_reuse=kv_reuse)

@@ -10,11 +10,13 @@
 //   * attn_shared_kernel (shared_attention.hpp) walks a share. With 8 kv heads the dispatcher's round-robin over the 8
 //     XCDs keeps every head's K/V in one XCD's L2.
 //   * attn_shared_combine_kernel merges each row's partial states, common ones and own ones.
-// Three kernels of one call, on MI355X, bf16, 32/8 heads of 128 (us, and what the call has to move or multiply):
-//   64 sequences of 1 row behind 8192 tokens, 16 to 1000 of their own   5.8 + 36.0 +  5.2   168 MB: 26 at 6.5 TB/s
-//   64 of 8 rows behind 4096, 100 to 1500 of their own                  6.1 + 70.5 + 10.5   237 MB: 36, and 41 GFLOP: 35
-//   32 of 1 row behind 32768, 20 to 300 of their own                    5.5 + 34.1 +  6.8   156 MB: 24
-//   8 of 100 to 300 rows behind 6000                                    6.3 + 181  + 17.5   160 GFLOP: 134 at 1.2 PFLOP/s
+// Three kernels of one call, on MI355X, bf16, 32/8 heads of 128 (us, medians of 20 calls, and what the call has to move or
+// multiply):
+//   64 sequences of 1 row behind 8192 tokens, 16 to 1000 of their own   5.7 + 36.0 +  5.2   168 MB: 26 at 6.5 TB/s
+//   64 of 8 rows behind 4096, 100 to 1500 of their own                  5.9 + 71.1 + 10.5   237 MB: 36, and 41 GFLOP: 35
+//   32 of 1 row behind 32768, 20 to 300 of their own                    5.7 + 33.7 +  7.0   156 MB: 24
+//   8 of 100 to 300 rows behind 6000                                    6.3 + 204  + 19.5   160 GFLOP: 134 at 1.2 PFLOP/s
+// (the last one's first calls, before the clock falls: 177 and 17.4).
 // The first and third stream: 4.7 TB/s over the main kernel, whose workgroups' states (64 KiB each, 33 MB) are written and
 // read beside that. What bounds the others stands at the loop (shared_attention.hpp).
 // Common tokens are taken in whole tiles (64 tokens, 32 in f32 and above head dim 128), so that no tile needs a

@@ -7,9 +7,12 @@
 // left has no order: table rows, positions and slots are written by as many workgroups as they fill
 // (tables_fill_kernel), or, where they are few, by the first one right away, which saves the second launch.
 //
-// What bounds it: latency. One request: 4.8 us, 64 with tables of 264 blocks and 8 rows each: 10.7 in one launch (6.7 + 3.6
-// in two, and 3.4 more of the host), both less than the call from Python (11.6). 264 entries with tables of 8192 blocks, 28 MB
-// to move: 4.2 + 8.6, the second at 3.3 TB/s. Rows that stay: 3.8 us for 64 requests, 7.1 for 1024.
+// What bounds it: latency. One request: 5.4 us, 64 with tables of 264 blocks and 8 rows each: 11.7 in one launch (6.7 + 3.6
+// in two, and 3.4 more of the host), both no more than the call from Python (11.6). 264 entries with tables of 8192 blocks,
+// 28 MB to move: 5.7 + 9.5, the second at 2.9 TB/s. Rows that stay: 5.6 us for 64 requests that give 23 blocks back, 10.1
+// for 1024 that give 1898. Requests that end: 3.3 + 2.6 for 64 of 110 blocks each, 3.7 + 6.6 for 256 of 1580. All these on a
+// state that is put back before each call, so that blocks move; a repeated call, which moves none, takes 4.8, 10.7, 4.2 +
+// 8.6, 3.8 and 7.1.
 #include "common.hpp"
 
 namespace kyro {
