@@ -652,8 +652,8 @@ int shared_check(const kyro_paged_attention_params* p, int32_t num_groups) {
 // and what several of them read comes from the caches. Sequences with all but 16 tokens in common, 32/8 heads of
 // 128 in bf16, shared and not: 16 of one row behind 2000 tokens (132 MB if each reads its own) 21.7 us and 16.9, behind
 // 4000 23.4 and 33.0; 16 of 8 rows 27.8 and 27.3, 34.3 and 42.7. In f32, where products are the limit, rows count as
-// well: 24 of 5 rows, 14/2 heads of 96, behind 1000 (38 MB) 38.5 and 34.9, behind 2000 41.9 and 58.2; of one row behind
-// 4000 (149 MB) 41.0 and 35.4, and a wave's 32 rows are mostly empty for 34 sequences of 5 rows with 8 kv heads of 128 and
+// well: 24 of 5 rows, 14/2 heads of 96, behind 1000 (38 MB) 36.6 and 32.8, behind 2000 39.2 and 53.2; of one row behind
+// 4000 (149 MB) 36.5 and 31.6, and a wave's 32 rows are mostly empty for 34 sequences of 5 rows with 8 kv heads of 128 and
 // up to 1800 tokens (515 MB): 109 and 46, against 139 and 264 for 63 of 7 rows behind 6400 (2.1 GB). Prompts are split
 // over tokens here and not there, 4 of 40 rows behind 1000 take 25.8 and 37.7; but up to 80 rows a kv head, or short
 // contexts, are faster there: 5 sequences of 64 rows of 1600 tokens 22.4 and 15.5, 4 of up to 216 over 390 tokens 22.5 and
